@@ -8,7 +8,7 @@ Option names, meanings and defaults are those of ``python -m tinyvllm``
 one JSON line per token id as it comes; the reference streams the text of one
 prompt); prefill reservations are zero as there (:137-138).  Added: --prompt-ids
 (token ids, the engine's native input), --random-weights SEED, --kv-block-size,
-float32 as a dtype.  Not offered: chat, attention backends, prefix caching.
+float32 as a dtype, --repetition-penalty, --presence-penalty, --frequency-penalty.  Not offered: chat, attention backends, prefix caching.
 Prints one JSON object ``{"outputs": [...]}`` (:155-163).
 """
 
@@ -46,6 +46,9 @@ def main(argv=None) -> None:
     parser.add_argument("--temperature", type=float, default=0.0)
     parser.add_argument("--top-k", type=int, default=0)
     parser.add_argument("--top-p", type=float, default=1.0)
+    parser.add_argument("--repetition-penalty", type=float, default=1.0)
+    parser.add_argument("--presence-penalty", type=float, default=0.0)
+    parser.add_argument("--frequency-penalty", type=float, default=0.0)
     parser.add_argument("--seed", type=int, default=0)
     parser.add_argument("--ignore-eos", action="store_true")
     parser.add_argument("--enforce-eager", action="store_true",
@@ -66,7 +69,9 @@ def main(argv=None) -> None:
 
     sampling = SamplingParams(
         max_new_tokens=args.max_new_tokens, temperature=args.temperature, top_k=args.top_k,
-        top_p=args.top_p, seed=args.seed, ignore_eos=args.ignore_eos)
+        top_p=args.top_p, seed=args.seed, ignore_eos=args.ignore_eos,
+        repetition_penalty=args.repetition_penalty, presence_penalty=args.presence_penalty,
+        frequency_penalty=args.frequency_penalty)
     config = EngineConfig(
         model=args.model, dtype=args.dtype, enforce_eager=args.enforce_eager,
         max_model_len=args.max_model_len, max_num_seqs=args.max_num_seqs,

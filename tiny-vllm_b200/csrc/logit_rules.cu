@@ -1,0 +1,251 @@
+// Rules on logits, before a token is drawn from them: for token v of a row whose request holds slot s,
+//
+//   x = logit(v)
+//   x = x > 0 ? x / repetition : x * repetition                       if v is among the request's tokens (prompt or answer)
+//   x = x - frequency * count(v) - presence * (count(v) > 0)          count: occurrences in the answer alone
+//   x = x + (sum of the request's biases of v)
+//   x = -inf                                                          if the request's mask has a zero bit at v
+//
+// in float32, rounded once to the type of the logits.  The counts are made anew from the request's tokens in every call:
+// a CTA takes one slice of one row, counts the tokens that fall into it in shared memory (a word a token: the count, one
+// bit for "in the prompt", one for "has a bias"), and then passes over its slice once.  Integer atomics and one thread a
+// logit: the result does not depend on the order in which anything runs.
+//
+// Bound by reading and writing the logits; the loads of the slice are issued first, so that the chain slot -> lengths ->
+// tokens -> counts runs under them.
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int SLICE = 4096;                        // tokens of the vocabulary a CTA takes
+constexpr int MAX_BIASES = 1024;                   // biases of a slot
+constexpr uint32_t HAS_BIAS = 1u << 31, IN_PROMPT = 1u << 30, COUNT = IN_PROMPT - 1;
+
+struct Rules {
+    const int* slots;                              // [rows]; one outside [0, slot_count): no rules
+    const float* penalties;                        // [slot_count, 3] repetition, presence, frequency
+    const int* lengths;                            // [slot_count, 2] tokens, of them the prompt's
+    const int* history;                            // [slot_count, room]
+    const int* bias_tokens;                        // [slot_count, biases] or null; -1: none
+    const float* bias_values;
+    const uint32_t* masks;                         // [mask_count, mask_words] or null
+    const int* mask_rows;                          // [slot_count]; one outside [0, mask_count): every token is allowed
+    int slot_count, room, biases, mask_count, mask_words;
+};
+
+template <typename T, int VEC> __device__ __forceinline__ void load_vec(const T* p, float* v) {
+    if constexpr (VEC == 1) {
+        v[0] = to_float<T>(*p);
+    } else if constexpr (sizeof(T) == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p);
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+        unpack_bf16x8(*reinterpret_cast<const uint4*>(p), v);
+    }
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, const float* v) {
+    if constexpr (VEC == 1) *p = from_float<T>(v[0]);
+    else if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint4*>(p) = pack_bf16x8(v);
+}
+
+// logits may be out itself (every thread reads what it will write before it writes): plain pointers
+template <typename T, int VEC>
+__global__ void __launch_bounds__(THREADS)
+logit_rules_kernel(const T* logits, int64_t row_stride, T* out, int64_t out_stride, int vocab, int slices, Rules rules) {
+    __shared__ __align__(16) uint32_t words[SLICE];
+    __shared__ int any_twice;
+    extern __shared__ float bias[];                // [SLICE] where there are biases
+    constexpr int PASSES = SLICE / (THREADS * VEC);
+    const int tid = threadIdx.x;
+    const int row = blockIdx.x / slices, begin = (blockIdx.x % slices) * SLICE;
+    const int count = min(SLICE, vocab - begin);
+    const T* x = logits + (int64_t)row * row_stride + begin;
+    T* y = out + (int64_t)row * out_stride + begin;
+
+    float v[PASSES][VEC];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int at = (p * THREADS + tid) * VEC;
+        if (at + VEC <= count) load_vec<T, VEC>(x + at, v[p]);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[p][e] = at + e < count ? to_float<T>(x[at + e]) : 0.0f;
+    }
+    const int slot = rules.slots[row];
+    const bool ruled = (unsigned)slot < (unsigned)rules.slot_count;       // the same for the whole CTA
+    float repetition = 1.0f, presence = 0.0f, frequency = 0.0f;
+    const uint32_t* mask = nullptr;
+    bool counted = false, biased = false;
+    if (ruled) {
+        repetition = rules.penalties[3 * (int64_t)slot];
+        presence = rules.penalties[3 * (int64_t)slot + 1];
+        frequency = rules.penalties[3 * (int64_t)slot + 2];
+        if (rules.masks) {
+            const int m = rules.mask_rows[slot];
+            if ((unsigned)m < (unsigned)rules.mask_count) mask = rules.masks + (int64_t)m * rules.mask_words;
+        }
+        const int total = min(max(rules.lengths[2 * (int64_t)slot], 0), rules.room);
+        const int prompt = min(max(rules.lengths[2 * (int64_t)slot + 1], 0), total);
+        // without a penalty for repetition the prompt is not looked at
+        const int first = repetition == 1.0f ? (presence == 0.0f && frequency == 0.0f ? total : prompt) : 0;
+        counted = first < total;
+        biased = rules.biases > 0;
+        if (counted || biased) {
+            for (int i = 4 * tid; i < SLICE; i += 4 * THREADS) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
+            if (tid == 0) any_twice = 0;
+            __syncthreads();
+            const int* history = rules.history + (int64_t)slot * rules.room;
+#pragma unroll 4
+            for (int i = first + tid; i < total; i += THREADS) {
+                const unsigned at = (unsigned)history[i] - (unsigned)begin;
+                if (at < (unsigned)count) {
+                    if (i >= prompt) atomicAdd(words + at, 1u);
+                    else atomicOr(words + at, IN_PROMPT);
+                }
+            }
+            if (biased) {
+                const int* tokens = rules.bias_tokens + (int64_t)slot * rules.biases;
+                const float* values = rules.bias_values + (int64_t)slot * rules.biases;
+                for (int i = tid; i < rules.biases; i += THREADS) {
+                    const int token = tokens[i];
+                    const unsigned at = (unsigned)token - (unsigned)begin;
+                    if (token >= 0 && at < (unsigned)count) {
+                        if (atomicOr(words + at, HAS_BIAS) & HAS_BIAS) any_twice = 1;
+                        else bias[at] = values[i];
+                    }
+                }
+                __syncthreads();
+                if (any_twice) {
+                    // a token named more than once: its first entry adds them all up, in their order
+                    for (int i = tid; i < rules.biases; i += THREADS) {
+                        const int token = tokens[i];
+                        const unsigned at = (unsigned)token - (unsigned)begin;
+                        if (token < 0 || at >= (unsigned)count) continue;
+                        bool first_entry = true;
+                        float sum = 0.0f;
+                        for (int j = 0; j < rules.biases && first_entry; ++j)
+                            if (tokens[j] == token) {
+                                if (j < i) first_entry = false;
+                                else sum = __fadd_rn(sum, values[j]);
+                            }
+                        if (first_entry) bias[at] = sum;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int at = (p * THREADS + tid) * VEC;
+        if (at >= count) break;
+        if (counted || biased) {
+            uint32_t word[VEC];
+            if constexpr (VEC == 1) word[0] = words[at];
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) *reinterpret_cast<uint4*>(word + e) = *reinterpret_cast<const uint4*>(words + at + e);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (word[e] == 0) continue;
+                float f = v[p][e];
+                if (word[e] & ~HAS_BIAS) {
+                    f = f > 0.0f ? __fdiv_rn(f, repetition) : __fmul_rn(f, repetition);
+                    const uint32_t times = word[e] & COUNT;
+                    if (times) f = __fsub_rn(__fsub_rn(f, __fmul_rn(frequency, (float)times)), presence);
+                }
+                if (word[e] & HAS_BIAS) f = __fadd_rn(f, bias[at + e]);
+                v[p][e] = f;
+            }
+        }
+        if (mask) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int token = begin + at + e;
+                if (at + e < count && !(mask[token >> 5] >> (token & 31) & 1u)) v[p][e] = -INFINITY;
+            }
+        }
+        if (at + VEC <= count) store_vec<T, VEC>(y + at, v[p]);
+        else
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (at + e < count) y[at + e] = from_float<T>(v[p][e]);
+    }
+}
+
+// lengths[slot] grows by one for every row that holds the slot, and the rows' tokens join its history, in the order of the
+// rows.  A full history stays as it is.  One CTA: a row counts those before it that hold its slot.
+__global__ void append_tokens_kernel(const int* slots, const int* tokens, int rows, int* lengths, int* history, int slot_count,
+                                     int room) {
+    extern __shared__ int held[];
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) held[i] = slots[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+        const int slot = held[i];
+        if ((unsigned)slot >= (unsigned)slot_count) continue;
+        int place = min(max(lengths[2 * (int64_t)slot], 0), room);
+        for (int j = 0; j < i; ++j) place += held[j] == slot;
+        if (place < room) history[(int64_t)slot * room + place] = tokens[i];
+    }
+    __syncthreads();                               // every length has been read
+    for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+        const int slot = held[i];
+        if ((unsigned)slot >= (unsigned)slot_count) continue;
+        int more = 1;
+        bool last = true;
+        for (int j = 0; j < rows; ++j) {
+            more += j < i && held[j] == slot;
+            last = last && !(j > i && held[j] == slot);
+        }
+        // a slot's last row alone writes its length
+        if (last) lengths[2 * (int64_t)slot] = min(min(max(lengths[2 * (int64_t)slot], 0), room) + more, room);
+    }
+}
+
+template <typename T, int VEC>
+int launch_rules(const void* logits, long long row_stride, void* out, long long out_stride, int rows, int vocab, const Rules& rules,
+                 cudaStream_t stream) {
+    const int slices = (vocab + SLICE - 1) / SLICE;
+    if ((long long)rows * slices > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
+    const size_t shared = rules.biases > 0 ? SLICE * 4 : 0;
+    logit_rules_kernel<T, VEC><<<rows * slices, THREADS, shared, stream>>>((const T*)logits, row_stride, (T*)out, out_stride, vocab,
+                                                                          slices, rules);
+    return tvb_last_error();
+}
+
+}  // namespace
+
+extern "C" int tvb_logit_rules_max_biases() { return MAX_BIASES; }
+
+extern "C" int tvb_logit_rules(const void* logits, long long row_stride, void* out, long long out_stride, int rows, int vocab,
+                               const int* slots, const float* penalties, const int* lengths, const int* history,
+                               const int* bias_tokens, const float* bias_values, const void* masks, const int* mask_rows,
+                               int slot_count, int room, int biases, int mask_count, int mask_words, int dtype, void* stream) {
+    if (rows <= 0 || vocab <= 0) return 0;
+    if (slot_count < 0 || room < 0 || biases < 0 || biases > MAX_BIASES || (biases > 0 && (!bias_tokens || !bias_values)) ||
+        (masks && (!mask_rows || (long long)mask_words * 32 < vocab)))
+        return TVB_BAD_ARGUMENT;
+    const Rules rules{slots, penalties, lengths, history, bias_tokens, bias_values, (const uint32_t*)masks, mask_rows,
+                      slot_count, room, biases, mask_count, mask_words};
+    cudaStream_t s = (cudaStream_t)stream;
+    const int size = dtype == TVB_F32 ? 4 : 2;
+    const bool wide = !(((uintptr_t)logits | (uintptr_t)out) & 15) && row_stride * size % 16 == 0 && out_stride * size % 16 == 0;
+    if (dtype == TVB_F32)
+        return wide ? launch_rules<float, 4>(logits, row_stride, out, out_stride, rows, vocab, rules, s)
+                    : launch_rules<float, 1>(logits, row_stride, out, out_stride, rows, vocab, rules, s);
+    if (dtype == TVB_BF16)
+        return wide ? launch_rules<bf16, 8>(logits, row_stride, out, out_stride, rows, vocab, rules, s)
+                    : launch_rules<bf16, 1>(logits, row_stride, out, out_stride, rows, vocab, rules, s);
+    return TVB_BAD_ARGUMENT;
+}
+
+extern "C" int tvb_append_tokens(const int* slots, const int* tokens, int rows, int* lengths, int* history, int slot_count, int room,
+                                 void* stream) {
+    if (rows <= 0) return 0;
+    if (rows > 8192 || slot_count < 0 || room < 0) return TVB_BAD_ARGUMENT;
+    const int threads = rows >= 256 ? 256 : (rows + 31) / 32 * 32;
+    append_tokens_kernel<<<1, threads, rows * 4, (cudaStream_t)stream>>>(slots, tokens, rows, lengths, history, slot_count, room);
+    return tvb_last_error();
+}

@@ -30,6 +30,7 @@ from ..config.engine import EngineConfig
 from ..ops import kernels
 from ..config.registry import read_model_config
 from ..sampling.params import SamplingParams
+from ..sampling.rules import LogitRules
 from ..sampling.sampler import Sampler
 from .graphs import DecodeGraphs
 from .model import Model
@@ -128,6 +129,7 @@ class _LoweredStep:
     draws: list
     bucket: object = None                 # (bucket, rows) of a decode graph, or
     prepared: object = None               # a PreparedStep of the step runner
+    rule_slots: list | None = None        # slots of the sampled rows' rules (-1: none), if any row has some
 
 
 class Engine:
@@ -149,6 +151,7 @@ class Engine:
         self.prompt_tokens = 0          # tokens of prompt portions run so far
         self.decode_tokens = 0          # single tokens run so far (one per request and decode step)
         self.lowering_failures = 0      # steps that failed before launch and were rolled back
+        self.rules: LogitRules | None = None        # made for the first request that has rules
         self._run = None            # (scheduled run, run in flight on the graphs, request ids) between calls
 
     # ---------------------------------------------------------- construction
@@ -223,6 +226,8 @@ class Engine:
         for token in prompt:
             if type(token) is not int or not 0 <= token < self.runner.vocab_size:
                 raise ValueError(f"{token!r} is not a token id below {self.runner.vocab_size}")
+        if isinstance(sampling, SamplingParams) and sampling.has_rules:
+            self._rules_for(sampling)
         if request_id is None:
             request_id = self._next_id
         if type(request_id) is not int or request_id < 0:
@@ -235,6 +240,15 @@ class Engine:
         self.scheduler.add(Request(request_id, prompt, sampling, arrival_ns=arrival_ns), now)
         self._next_id = max(self._next_id, request_id + 1)
         return request_id
+
+    def _rules_for(self, sampling: SamplingParams) -> LogitRules:
+        """The engine's rules, made when the first request with some is submitted: a slot for every state slot of the
+        cache, each with room for the longest request."""
+        if self.rules is None:
+            self.rules = LogitRules(vocab=self.runner.vocab_size, slots=self.runner.manager.slots.num_slots,
+                                    room=self.runner.max_model_len, device=self.runner.device)
+        self.rules.check(sampling)
+        return self.rules
 
     def cancel(self, request_id: int) -> bool:
         self._check_usable()
@@ -287,7 +301,9 @@ class Engine:
         self.scheduler.advance(now)
         if self._run is not None:
             return self._continue_run(now if explicit else None)
-        if self.decode_run_steps > 1 and self.graphs.bucket_for(len(self.scheduler.decoding)) is not None:
+        # (a run's steps sample inside their graph, without rules)
+        if (self.decode_run_steps > 1 and self.graphs.bucket_for(len(self.scheduler.decoding)) is not None
+                and not any(self.scheduler.requests[i].sampling.has_rules for i in self.scheduler.decoding)):
             run = self.scheduler.schedule_decode_run(self.decode_run_steps, now)
             if run is not None:
                 self._start_run(run)
@@ -410,6 +426,13 @@ class Engine:
                 draws.append(len(request.output_token_ids))
                 sample_ids.append(item.request_id)
         lowered = _LoweredStep(sample_ids, params, draws)
+        if any(p.has_rules for p in params):
+            held = {p.request_id: p.state_slot for p in scheduled.cache_plan.entries}
+            lowered.rule_slots = [held[i] if p.has_rules else -1 for i, p in zip(sample_ids, params)]
+            for request_id, slot, drawn in zip(sample_ids, lowered.rule_slots, draws):
+                if slot >= 0 and drawn == 0:             # from here on the slot follows the request's tokens by itself
+                    request = requests[request_id]
+                    self._rules_for(request.sampling).set(slot, request.sampling, request.prompt_token_ids)
         decode_only = all(item.count == 1 and item.sample for item in scheduled.items)
         if decode_only and self.graphs is not None:
             lowered.bucket = self.graphs.prepare(scheduled.cache_plan, entries, params, draws)
@@ -422,12 +445,17 @@ class Engine:
         """The device half: run the step, sample, read the tokens (the step's one device-to-host read)."""
         tokens_device = None
         if lowered.bucket is not None:
-            tokens_device = self.graphs.launch(lowered.bucket, scheduled.cache_plan)[0]
+            tokens_device, logits = self.graphs.launch(lowered.bucket, scheduled.cache_plan)
             self.graph_steps += 1
+            if lowered.rule_slots is not None:           # the graph sampled without the rules: sample again
+                tokens_device = self.sampler.sample(logits, lowered.params, lowered.draws, rules=self.rules,
+                                                    slots=lowered.rule_slots)
         else:
             logits = self.runner.launch(lowered.prepared)
             if logits is not None:
-                tokens_device = self.sampler.sample(logits, lowered.params, lowered.draws)
+                tokens_device = self.sampler.sample(
+                    logits, lowered.params, lowered.draws, slots=lowered.rule_slots or (),
+                    rules=self.rules if lowered.rule_slots is not None else None)
         if tokens_device is None:
             return {}
         host = tokens_device.tolist()

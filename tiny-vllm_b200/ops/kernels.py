@@ -1982,6 +1982,116 @@ def sample_rows(logits: torch.Tensor, packed: torch.Tensor, out: torch.Tensor | 
     return out
 
 
+def _here(who: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse tensors that are not on the current CUDA device, whose current stream the kernel is launched on."""
+    for tensor in tensors:
+        if tensor is not None and not tensor.is_cuda:
+            raise KernelError("the kernels run on CUDA tensors only; there is no CPU path")
+    index = torch._C._cuda_getDevice()
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != index:
+            raise KernelError(f"{who}: every tensor has to be on the current device (cuda:{index}; "
+                              f"torch.cuda.device(...) makes another one current), got {tensor.device}")
+
+
+def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the memory from the first to the last element of two tensors has bytes in common."""
+    def span(t):
+        last = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+# ------------------------------------------------------------ rules on logits
+LOGIT_RULES_MAX_BIASES = 1024      # MAX_BIASES of logit_rules.cu
+APPEND_MAX_ROWS = 8192
+
+
+def _is(t: torch.Tensor, dtype: torch.dtype, *shape: int) -> bool:
+    return t.dtype == dtype and t.shape == shape and t.is_contiguous()
+
+
+def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.Tensor, lengths: torch.Tensor,
+                history: torch.Tensor, bias_tokens: torch.Tensor | None = None, bias_values: torch.Tensor | None = None,
+                masks: torch.Tensor | None = None, mask_rows: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """The logits [rows, vocab] (float32 or bfloat16, rows may be strided) under the rules of the rows' requests.
+
+    Row r belongs to the request in slot ``slots[r]`` (int32 [rows]; a negative number, or one past the last slot: the row
+    comes back as it is).  Of every slot there are ``penalties`` (float32 [slots, 3]: repetition > 0, presence, frequency),
+    ``lengths`` (int32 [slots, 2]: tokens in its history, how many of them are the prompt) and ``history`` (int32
+    [slots, room]: the prompt's tokens, then the answer's; lengths are cut at ``room``).  For a token among all of them
+    the logit is divided by the penalty for repetition where it is positive, else multiplied with it; then frequency *
+    count and, if the count is not 0, presence are taken off, the count being that in the answer.  ``bias_tokens`` and
+    ``bias_values`` (int32 and float32 [slots, up to 1024]; token -1: none) are added (a token named twice gets both, in
+    their order).  Last, with ``masks`` (int32 [masks, at least vocab / 32 words]: bit v % 32 of word v // 32 is token v)
+    and ``mask_rows`` (int32 [slots]; a number outside the masks: all tokens), tokens whose bit is 0 become -inf, whatever
+    they were; a mask of zeros leaves -inf alone.  Tokens outside the vocabulary are passed over.
+
+    Computed in float32 and rounded once to the type of the logits.  ``out``: where the result goes, ``logits`` itself
+    among others (in place); else a new tensor."""
+    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise KernelError("logit_rules wants logits [rows, vocab] whose rows are contiguous")
+    tag = dtype_tag(logits.dtype)
+    (rows, vocab), (count, room) = logits.shape, history.shape if history.dim() == 2 else (-1, 0)
+    if not _is(slots, torch.int32, rows):
+        raise KernelError(f"logit_rules: slots must be contiguous int32 [{rows}]")
+    if count < 0 or history.dtype != torch.int32 or not history.is_contiguous():
+        raise KernelError("logit_rules: history must be contiguous int32 [slots, room]")
+    if not _is(penalties, torch.float32, count, 3) or not _is(lengths, torch.int32, count, 2):
+        raise KernelError(f"logit_rules: penalties must be contiguous float32 [{count}, 3], lengths int32 [{count}, 2]")
+    if (bias_tokens is None) != (bias_values is None) or (masks is None) != (mask_rows is None):
+        raise KernelError("logit_rules: bias_tokens and bias_values, masks and mask_rows come together")
+    biases = mask_count = words = 0
+    if bias_tokens is not None:
+        biases = bias_tokens.shape[1] if bias_tokens.dim() == 2 else -1
+        if not 0 <= biases <= LOGIT_RULES_MAX_BIASES or not _is(bias_tokens, torch.int32, count, biases) \
+                or not _is(bias_values, torch.float32, count, biases):
+            raise KernelError(f"logit_rules: biases must be contiguous int32 and float32 [{count}, up to {LOGIT_RULES_MAX_BIASES}]")
+    if masks is not None:
+        mask_count, words = masks.shape if masks.dim() == 2 else (-1, 0)
+        if mask_count < 0 or masks.dtype != torch.int32 or not masks.is_contiguous() or words * 32 < vocab \
+                or not _is(mask_rows, torch.int32, count):
+            raise KernelError(f"logit_rules: masks must be contiguous int32 [masks, at least {-(-vocab // 32)}], "
+                              f"mask_rows int32 [{count}]")
+    if out is None:
+        _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows)
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+    else:
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1 and vocab > 1 \
+                or rows > 1 and out.stride(0) < vocab:
+            raise KernelError("logit_rules: out must be [rows, vocab] of the type of the logits with contiguous rows of its own")
+        if (out.data_ptr() != logits.data_ptr() or out.stride(0) != logits.stride(0)) and _overlaps(out, logits):
+            raise KernelError("logit_rules: out is the logits themselves, or memory of its own")
+        _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows, out)
+    fn = _fn("logit_rules", "tvb_logit_rules",
+             [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p])
+    _check(fn(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, slots.data_ptr(),
+              penalties.data_ptr(), lengths.data_ptr(), history.data_ptr(), _ptr(bias_tokens), _ptr(bias_values), _ptr(masks),
+              _ptr(mask_rows), count, room, biases, mask_count, words, tag, _stream()), "logit_rules")
+    return out
+
+
+def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.Tensor, history: torch.Tensor) -> None:
+    """``tokens[r]`` (int32 [rows]) becomes the last token of the history in slot ``slots[r]`` (as :func:`logit_rules` reads
+    it; rows without a slot are passed over, rows that share one follow one another).  A history that is full stays so."""
+    if tokens.dim() != 1 or tokens.dtype != torch.int32 or not tokens.is_contiguous() or tokens.shape[0] > APPEND_MAX_ROWS \
+            or not _is(slots, torch.int32, *tokens.shape):
+        raise KernelError(f"append_tokens: tokens and slots must be contiguous int32 [rows], up to {APPEND_MAX_ROWS} rows")
+    if history.dim() != 2 or history.dtype != torch.int32 or not history.is_contiguous() \
+            or not _is(lengths, torch.int32, history.shape[0], 2):
+        raise KernelError("append_tokens: history must be contiguous int32 [slots, room], lengths int32 [slots, 2]")
+    _here("append_tokens", tokens, slots, lengths, history)
+    fn = _fn("logit_rules", "tvb_append_tokens", [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
+    _check(fn(slots.data_ptr(), tokens.data_ptr(), tokens.shape[0], lengths.data_ptr(), history.data_ptr(), history.shape[0],
+              history.shape[1], _stream()), "append_tokens")
+
+
 # ------------------------------------------------- tiled attention (bfloat16)
 DECODE_MAX_PIECES = 8
 

@@ -1,4 +1,5 @@
 from .params import SamplingParams
+from .rules import LogitRules
 from .sampler import Sampler
 
-__all__ = ["Sampler", "SamplingParams"]
+__all__ = ["LogitRules", "Sampler", "SamplingParams"]

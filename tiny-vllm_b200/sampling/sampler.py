@@ -17,6 +17,7 @@ import torch
 
 from ..ops import kernels
 from .params import SamplingParams
+from .rules import LogitRules
 
 ROW_WORDS = 7        # temperature, top_p (float bits), top_k, seed lo/hi, draw lo/hi
 
@@ -49,10 +50,20 @@ def sample_packed(logits: torch.Tensor, packed: torch.Tensor, out: torch.Tensor 
 
 class Sampler:
     def sample(self, logits: torch.Tensor, params: Sequence[SamplingParams],
-               draws: Sequence[int]) -> torch.Tensor:
+               draws: Sequence[int], *, rules: LogitRules | None = None, slots: Sequence[int] = ()) -> torch.Tensor:
         """int32 tokens on the device, one per row; ``draws[i]`` counts the tokens
-        row i's request has drawn before."""
+        row i's request has drawn before.  With ``rules`` the tokens are drawn from the logits under
+        the rules of ``slots`` (one a row; -1: a row without rules) and join what the slots remember;
+        the logits are changed in place."""
         if logits.shape[0] != len(params) or len(params) != len(draws):
             raise ValueError("params and draws must align with the rows of logits")
-        packed = torch.from_numpy(pack_rows(params, draws)).to(logits.device, non_blocking=True)
-        return sample_packed(logits, packed)
+        packed = pack_rows(params, draws)
+        if rules is None:
+            return sample_packed(logits, torch.from_numpy(packed).to(logits.device, non_blocking=True))
+        if len(slots) != len(params):
+            raise ValueError("slots must align with the rows of logits")
+        both = np.concatenate([packed, np.array([slots], dtype=np.int32)])            # one copy
+        both = torch.from_numpy(both).to(logits.device, non_blocking=True)
+        tokens = sample_packed(rules.apply(logits, both[ROW_WORDS], out=logits), both[:ROW_WORDS])
+        rules.append(tokens, both[ROW_WORDS])
+        return tokens
