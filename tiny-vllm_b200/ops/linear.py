@@ -64,6 +64,47 @@ def _linear_f32(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None,
     return kernels.gemm_nt_simt(x, weight, out=out, weight_constant=weight_constant)
 
 
+def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,
+                   scales: torch.Tensor | None = None, *, out_dtype: torch.dtype | None = None,
+                   out: torch.Tensor | None = None, weight_constant: bool = False) -> torch.Tensor:
+    """:func:`linear` with a low-rank adapter of each row's own: row t of the result is x[t] W^T + s (x[t] A^T) B^T with
+    A = ``down[ids[t]]`` ([adapters, rank, k]), B = ``up[ids[t]]`` ([adapters, n, rank]), s = ``scales[ids[t]]`` (float32
+    [adapters]; None: 1).  ``ids`` (int32 [m]) may come in any order; a row whose number names no adapter (-1) has the
+    projection alone.  Adapters of lower rank are filled up with zeros; ranks up to 256.
+
+    x A^T stays float32; the adapter's part is added to the projection as that was rounded, and the sum rounded to the
+    result's type (a float32 result is not rounded in between)."""
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.dtype != x.dtype or x.shape[1] < 1:
+        raise kernels.KernelError("linear_adapted wants x [m, k] and a weight [n, k] of its type")
+    (m, k), n = x.shape, weight.shape[0]
+    kernels.dtype_tag(x.dtype)
+    adapters, rank = down.shape[:2] if down.dim() == 3 else (0, 0)
+    if not kernels._is(down, x.dtype, adapters, rank, k) or not kernels._is(up, x.dtype, adapters, n, rank) or adapters < 1 \
+            or not 1 <= rank <= kernels.ADAPTERS_MAX_RANK:
+        raise kernels.KernelError(f"linear_adapted: down and up must be contiguous [adapters, rank, {k}] and [adapters, {n}, rank] "
+                                  f"of the type of x, at least one adapter, ranks from 1 to {kernels.ADAPTERS_MAX_RANK}")
+    if not kernels._is(ids, torch.int32, m):
+        raise kernels.KernelError(f"linear_adapted: ids must be contiguous int32 [{m}]")
+    if scales is not None and not kernels._is(scales, torch.float32, adapters):
+        raise kernels.KernelError(f"linear_adapted: scales must be contiguous float32 [{adapters}]")
+    if x.stride(1) != 1 and k > 1:
+        raise kernels.KernelError("linear_adapted: the rows of x must be contiguous")
+    out_dtype = out_dtype or (x.dtype if out is None else out.dtype)
+    if out_dtype not in (x.dtype, torch.float32):
+        raise kernels.KernelError("linear_adapted: the result has the type of x, or float32")
+    if out is not None and (out.shape != (m, n) or out.dtype != out_dtype or out.stride(1) != 1 and n > 1
+                            or m > 1 and out.stride(0) < n or any(kernels._overlaps(out, t) for t in (x, weight, down, up))):
+        raise kernels.KernelError(f"linear_adapted: out must be {out_dtype} [{m}, {n}] with contiguous rows, in memory of its own")
+    kernels._here("linear_adapted", x, weight, down, up, ids, scales, out)
+    if m == 0 or n == 0:
+        return torch.empty((m, n), dtype=out_dtype, device=x.device) if out is None else out
+    # the short product first: the projection's kernel may then ask for its weight while that ends
+    part = kernels.adapters_shrink(x, down, ids)
+    y = linear(x, weight, out_dtype=out_dtype, out=out, weight_constant=weight_constant)
+    kernels.adapters_expand(part, up, ids, scales, y, k)
+    return y
+
+
 def linear_silu(x: torch.Tensor, gate_up_weight: torch.Tensor, *, weight_constant: bool = False) -> torch.Tensor:
     """round(round(silu(x . gate^T)) * (x . up^T)) for a packed [gate | up] weight, [m, inter].  ``weight_constant``: as in
     :func:`linear`."""
