@@ -1,0 +1,616 @@
+// Attention over the paged cache for tokens of which groups have their first keys in common: several answers to one prompt,
+// or requests behind one system prompt.  softmax(q K^T scale) V over the keys 0 .. position of every token, where the keys
+// below the group's shared length are read once for a tile of the group's query rows (tokens x query heads of one key/value
+// head) instead of once a token.
+//
+// Softmax over a union of key ranges from the ranges' own results: a range gives its maximum m, l = sum exp(s - m) and
+// O = sum exp(s - m) v, and ranges join as l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).  So one launch takes pieces of
+// the shared keys (a tile of query rows each) and pieces of what every token has behind them (its own query heads), all
+// side by side, and leaves their m, l and O in float32 scratch; a second joins every token's pieces in their order.
+//
+// bfloat16: mma.sync m16n8k16 over tiles of 64 keys that cp.async brings two deep; a warp of a shared piece has 16 query
+// rows and every key, the warps of a token's own piece share the keys of a tile among them.  P is rounded to bfloat16 for
+// the second product, the denominator sums what was not rounded.  float32: the float32 cores, tiles of 32 keys.
+//
+// Bound by reading keys and values while a group has few query rows, by the tensor cores once it has many.
+#include "common.cuh"
+
+namespace {
+
+constexpr int THREADS = 128, WARPS = 4;
+constexpr int KEYS = 64;                        // keys of a bfloat16 tile
+constexpr int KEYS32 = 32;                      // keys of a float32 tile
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Attend {
+    const void* q;
+    int64_t q_stride;
+    const void* keys;                           // [pages, kv heads, page size, D]
+    const void* values;
+    const int* tables;                          // [rows, width]
+    const int* token_row;                       // [tokens]
+    const int* positions;                       // [tokens]
+    const int* group_starts;                    // [groups + 1]
+    const int* shared_lens;                     // [groups]
+    float* part_o;                              // [tokens, q heads, pieces, D]
+    float* part_ml;                             // [tokens, q heads, pieces, 2]
+    void* out;
+    int64_t out_stride;
+    int tokens, rows, width, groups, pages, page_size, num_q, num_kv;
+    int shared_pieces, own_pieces, shared_items, own_tiles;
+    float scale_log2;
+};
+
+struct Range { int first, end; };
+
+// piece c of n keys in up to `pieces`: whole tiles of 64
+__device__ __forceinline__ int piece_keys(int n, int pieces) { return max(KEYS, ((n + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS); }
+
+__device__ __forceinline__ int row_of(const Attend& a, int token) {
+    const int row = a.token_row[token];
+    return (unsigned)row < (unsigned)a.rows && a.positions[token] >= 0 ? row : -1;
+}
+// keys a token reads: its position's and those before it, as far as its table goes
+__device__ __forceinline__ int keys_of(const Attend& a, int token) {
+    return (int)min((int64_t)a.positions[token] + 1, (int64_t)a.width * a.page_size);
+}
+__device__ __forceinline__ int shared_of_group(const Attend& a, int group) {
+    return (int)min((int64_t)max(a.shared_lens[group], 0), (int64_t)a.width * a.page_size);
+}
+// the shared keys of the token's group, if it reads all of them (else it reads what it has by itself)
+__device__ __forceinline__ int shared_of(const Attend& a, int token) {
+    int lo = 0, hi = a.groups;                  // the last group that starts at or before the token
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (a.group_starts[mid] <= token) lo = mid; else hi = mid - 1;
+    }
+    if (lo >= a.groups || a.group_starts[lo] > token) return 0;
+    const int shared = shared_of_group(a, lo);
+    return keys_of(a, token) >= shared ? shared : 0;
+}
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, const bf16* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
+}
+
+// One piece: ROWS query rows (token, head) of one kv head over the keys [range.first, range.end) of the request with this
+// block table.
+struct Piece {
+    Range range;
+    const int* table;
+    int kv_head, slot;                          // slot: where the piece's results go among the token's
+    int token0, rows, row0;                     // row r: token token0 + (row0 + r) / heads, head (row0 + r) % heads
+};
+
+// Which piece this CTA has; false: none.  TILE: query rows of a shared piece, OWN: of a token's own.
+template <int TILE, int OWN>
+__device__ __forceinline__ bool find_piece(const Attend& a, Piece& p, bool& shared) {
+    const int heads = a.num_q / a.num_kv;
+    int item = blockIdx.x;
+    shared = item < a.shared_items;
+    if (shared) {
+        const int piece = item % a.shared_pieces;
+        item /= a.shared_pieces;
+        p.kv_head = item % a.num_kv;
+        int tile = item / a.num_kv;
+        // the group that has the tile: 32 groups at a time
+        const int lane = threadIdx.x & 31;
+        for (int g0 = 0; g0 < a.groups; g0 += 32) {
+            int start = 0, count = 0;
+            if (g0 + lane < a.groups) {
+                start = min(max(a.group_starts[g0 + lane], 0), a.tokens);
+                const int end = min(max(a.group_starts[g0 + lane + 1], start), a.tokens);
+                count = shared_of_group(a, g0 + lane) > 0 ? ((end - start) * heads + TILE - 1) / TILE : 0;
+            }
+            int upto = count;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += other;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, upto > tile);
+            if (past == 0) { tile -= __shfl_sync(0xffffffffu, upto, 31); continue; }
+            const int at = __ffs(past) - 1, group = g0 + at;
+            tile -= __shfl_sync(0xffffffffu, upto - count, at);
+            start = __shfl_sync(0xffffffffu, start, at);
+            const int end = min(max(a.group_starts[group + 1], start), a.tokens);
+            const int n = shared_of_group(a, group), per = piece_keys(n, a.shared_pieces);
+            p.range = Range{piece * per, min(n, (piece + 1) * per)};
+            if (p.range.first >= n) return false;
+            // the table of the first token that reads all of the shared keys
+            int row = -1;
+            for (int token = start; token < end && row < 0; ++token) {
+                row = row_of(a, token);
+                if (row >= 0 && keys_of(a, token) < n) row = -1;
+            }
+            if (row < 0) return false;
+            p.table = a.tables + (int64_t)row * a.width;
+            p.token0 = start;
+            p.row0 = tile * TILE;
+            p.rows = min(TILE, (end - start) * heads - p.row0);
+            p.slot = piece;
+            return true;
+        }
+        return false;
+    }
+    item -= a.shared_items;
+    const int piece = item % a.own_pieces;
+    item /= a.own_pieces;
+    const int tile = item % a.own_tiles;
+    item /= a.own_tiles;
+    p.kv_head = item % a.num_kv;
+    p.token0 = item / a.num_kv;
+    const int row = row_of(a, p.token0);
+    if (row < 0) return false;
+    const int first = shared_of(a, p.token0), n = keys_of(a, p.token0) - first, per = piece_keys(n, a.own_pieces);
+    p.range = Range{first + piece * per, first + min(n, (piece + 1) * per)};
+    if (piece * per >= n) return false;
+    p.table = a.tables + (int64_t)row * a.width;
+    p.row0 = tile * OWN;
+    p.rows = min(OWN, heads - p.row0);
+    p.slot = a.shared_pieces + piece;
+    return true;
+}
+__device__ __forceinline__ int token_of(const Attend& a, const Piece& p, int r, int& head) {
+    const int heads = a.num_q / a.num_kv, at = p.row0 + r;
+    head = p.kv_head * heads + at % heads;
+    return p.token0 + at / heads;
+}
+__device__ __forceinline__ int64_t part_of(const Attend& a, int token, int head, int slot) {
+    return ((int64_t)token * a.num_q + head) * (a.shared_pieces + a.own_pieces) + slot;
+}
+// a row of a shared tile that takes part: the token is one, and reads all of the shared keys
+__device__ __forceinline__ bool takes_part(const Attend& a, bool shared, int token) {
+    return !shared || (row_of(a, token) >= 0 && shared_of(a, token) > 0);
+}
+// place of a key's row in the cache, in rows of D; -1: no such page
+__device__ __forceinline__ int64_t cache_row(const Attend& a, const Piece& p, int key) {
+    const int page = p.table[key / a.page_size];
+    return (unsigned)page < (unsigned)a.pages ? ((int64_t)page * a.num_kv + p.kv_head) * a.page_size + key % a.page_size : -1;
+}
+
+// ------------------------------------------------------------------ bfloat16
+template <int D> struct Tiles {
+    static constexpr int PITCH = D + 8;
+    static constexpr int TILE = KEYS * PITCH;                                   // elements of a K or V tile
+    static constexpr int BYTES = (64 + 4 * KEYS) * PITCH * 2 + 3 * KEYS * 8 + 3 * 2 * 4;
+};
+
+// SHARED: the tile's 64 query rows, 16 a warp, every warp over every key.  Else: up to 16 query rows, a warp over 16 keys of
+// every tile, the warps' results joined at the end.
+template <int D, bool SHARED>
+__device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, unsigned char* raw) {
+    constexpr int PITCH = Tiles<D>::PITCH, ROWS = SHARED ? 64 : 16;
+    constexpr int NK = SHARED ? KEYS : KEYS / WARPS;                            // keys of a tile that a warp has
+    bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [ROWS][PITCH]
+    bf16* k_s = q_s + 64 * PITCH;                                               // [2][KEYS][PITCH]
+    bf16* v_s = k_s + 2 * Tiles<D>::TILE;
+    // of a tile's keys: the place of their rows (-1: none), and which there are.  Three tiles of them: one warp may look up
+    // those of a tile while another still reads the bits of the one two before.
+    int64_t* at_s = reinterpret_cast<int64_t*>(v_s + 2 * Tiles<D>::TILE);       // [3][KEYS]
+    uint32_t* there_s = reinterpret_cast<uint32_t*>(at_s + 3 * KEYS);           // [3][2]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const bf16* keys = reinterpret_cast<const bf16*>(a.keys);
+    const bf16* values = reinterpret_cast<const bf16*>(a.values);
+    const int tiles = (p.range.end - p.range.first + KEYS - 1) / KEYS;
+
+    auto place = [&](int tile) {                                                // the first two warps
+        const int slot = tile % 3;
+        if (tid < KEYS) {
+            const int key = p.range.first + tile * KEYS + tid;
+            const int64_t at = key < p.range.end ? cache_row(a, p, key) : -1;
+            at_s[slot * KEYS + tid] = at;
+            const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+            if (lane == 0) there_s[slot * 2 + warp] = there;
+        }
+    };
+    auto load = [&](int tile) {
+        const int buffer = tile & 1, slot = tile % 3;
+        constexpr int WORDS = D / 8;
+#pragma unroll 4
+        for (int i = tid; i < KEYS * WORDS; i += THREADS) {
+            const int key = i / WORDS, word = i % WORDS;
+            const int64_t at = at_s[slot * KEYS + key];
+            const int64_t from = (at < 0 ? 0 : at) * D + word * 8;
+            cp_async_16(k_s + buffer * Tiles<D>::TILE + key * PITCH + word * 8, keys + from, at >= 0);
+            cp_async_16(v_s + buffer * Tiles<D>::TILE + key * PITCH + word * 8, values + from, at >= 0);
+        }
+        cp_async_commit();
+    };
+    place(0);
+    for (int i = tid; i < ROWS * (D / 8); i += THREADS) {
+        const int r = i / (D / 8), word = i % (D / 8);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < p.rows) {
+            int head;
+            const int token = token_of(a, p, r, head);
+            if (takes_part(a, SHARED, token))
+                v = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + token * a.q_stride + head * D + word * 8);
+        }
+        *reinterpret_cast<uint4*>(q_s + r * PITCH + word * 8) = v;
+    }
+    __syncthreads();
+    load(0);
+    const bf16* q_rows = q_s + (SHARED ? warp * 16 : 0) * PITCH + (lane & 15) * PITCH + (lane >> 4) * 8;
+    uint32_t q_frag[D <= 128 ? D / 16 : 1][4];
+    if constexpr (D <= 128)
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) ldmatrix_x4(q_frag[ks], q_rows + ks * 16);
+
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const int key_at = SHARED ? 0 : warp * NK;
+
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int buffer = tile & 1;
+        if (tile + 1 < tiles) place(tile + 1);
+        cp_async_wait<0>();
+        __syncthreads();                                                        // the tile is there; places of the next too
+        if (tile + 1 < tiles) load(tile + 1);
+        const bf16* k_tile = k_s + buffer * Tiles<D>::TILE + key_at * PITCH;
+        const bf16* v_tile = v_s + buffer * Tiles<D>::TILE + key_at * PITCH;
+        float s[NK / 8][4];
+#pragma unroll
+        for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+            uint32_t q_now[4];
+            if constexpr (D > 128) ldmatrix_x4(q_now, q_rows + ks * 16);
+            const uint32_t (&q4)[4] = D <= 128 ? q_frag[D <= 128 ? ks : 0] : q_now;
+#pragma unroll
+            for (int np = 0; np < NK / 16; ++np) {
+                uint32_t b[4];
+                const int matrix = lane >> 3;
+                ldmatrix_x4(b, k_tile + (np * 16 + (matrix >> 1) * 8 + (lane & 7)) * PITCH + ks * 16 + (matrix & 1) * 8);
+                mma_16816(s[2 * np], q4, b[0], b[1]);
+                mma_16816(s[2 * np + 1], q4, b[2], b[3]);
+            }
+        }
+        const uint64_t there = (uint64_t)there_s[tile % 3 * 2] | (uint64_t)there_s[tile % 3 * 2 + 1] << 32;
+        float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[n][i] *= a.scale_log2;
+                if (~there != 0 && !(there >> (key_at + n * 8 + 2 * t4 + (i & 1)) & 1)) s[n][i] = -INFINITY;
+                most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
+            }
+        float subtract[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+            const float now = fmaxf(m[h], most[h]);
+            subtract[h] = now == -INFINITY ? 0.0f : now;                        // no inf - inf where no key was seen yet
+            const float factor = exp2_unit(m[h] - subtract[h]);
+            m[h] = now;
+            l[h] *= factor;
+            most[h] = factor;
+        }
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][i] *= most[i >> 1];
+#pragma unroll
+        for (int kk = 0; kk < NK / 16; ++kk) {
+            uint32_t weights[4];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int n = 2 * kk + half;
+                float w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = exp2_unit(s[n][i] - subtract[i >> 1]);
+                    l[i >> 1] += w[i];
+                }
+                weights[2 * half] = pack_bf16x2(w[0], w[1]);
+                weights[2 * half + 1] = pack_bf16x2(w[2], w[3]);
+            }
+#pragma unroll
+            for (int dp = 0; dp < D / 16; ++dp) {
+                uint32_t b[4];
+                const int matrix = lane >> 3;
+                ldmatrix_x4_trans(b, v_tile + (kk * 16 + (matrix & 1) * 8 + (lane & 7)) * PITCH + dp * 16 + (matrix >> 1) * 8);
+                mma_16816(o[2 * dp], weights, b[0], b[1]);
+                mma_16816(o[2 * dp + 1], weights, b[2], b[3]);
+            }
+        }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    if constexpr (SHARED) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = warp * 16 + g + 8 * h;
+            if (r >= p.rows) continue;
+            int head;
+            const int token = token_of(a, p, r, head);
+            if (!takes_part(a, true, token)) continue;
+            const int64_t part = part_of(a, token, head, p.slot);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float2*>(a.part_o + part * D + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[h], l[h]);
+        }
+    } else {
+        // the warps' results, over the tiles' memory: [warp][16][D + 4] and [warp][16][2]
+        constexpr int OP = D + 4;
+        float* o_w = reinterpret_cast<float*>(k_s);
+        float* ml_w = o_w + WARPS * 16 * OP;
+        static_assert(WARPS * 16 * (OP + 2) * 4 <= 4 * Tiles<D>::TILE * 2, "the warps' results lie over the tiles");
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = warp * 16 + g + 8 * h;
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float2*>(o_w + r * OP + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if (t4 == 0) { ml_w[2 * r] = m[h]; ml_w[2 * r + 1] = l[h]; }
+        }
+        __syncthreads();
+        for (int i = tid; i < p.rows * (D / 4); i += THREADS) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml_w[2 * (w * 16 + r)]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+            float4 sum = make_float4(0, 0, 0, 0);
+            float total = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = exp2_unit(ml_w[2 * (w * 16 + r)] - ref);
+                const float4 v = *reinterpret_cast<const float4*>(o_w + (w * 16 + r) * OP + d);
+                sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+                total += f * ml_w[2 * (w * 16 + r) + 1];
+            }
+            int head;
+            const int token = token_of(a, p, r, head);
+            const int64_t part = part_of(a, token, head, p.slot);
+            *reinterpret_cast<float4*>(a.part_o + part * D + d) = sum;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, total);
+        }
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS) attend_bf16_kernel(Attend a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    pdl_wait();
+    pdl_launch_dependents();
+    Piece p;
+    bool shared;
+    if (!find_piece<64, 16>(a, p, shared)) return;                              // the whole CTA
+    if (shared) attend_piece<D, true>(a, p, raw);
+    else attend_piece<D, false>(a, p, raw);
+}
+
+// ------------------------------------------------------------------- float32
+// 16 query rows, four a warp: a lane has a key of the tile for the scores, D / 32 values of every row for the sums.
+template <int D>
+__global__ void __launch_bounds__(THREADS) attend_f32_kernel(Attend a) {
+    constexpr int PITCH = D + 4, VALUES = D / 32;
+    extern __shared__ __align__(16) float tiles_s[];
+    float* k_s = tiles_s;                                                       // [KEYS32][PITCH]
+    float* v_s = k_s + KEYS32 * PITCH;
+    float* q_s = v_s + KEYS32 * PITCH;                                          // [16][D]
+    __shared__ uint32_t there_s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    Piece p;
+    bool shared;
+    if (!find_piece<16, 16>(a, p, shared)) return;
+    const float* keys = reinterpret_cast<const float*>(a.keys);
+    const float* values = reinterpret_cast<const float*>(a.values);
+    for (int i = tid; i < 16 * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float4 v = make_float4(0, 0, 0, 0);
+        if (r < p.rows) {
+            int head;
+            const int token = token_of(a, p, r, head);
+            if (takes_part(a, shared, token))
+                v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D + d);
+        }
+        *reinterpret_cast<float4*>(q_s + r * D + d) = v;
+    }
+    float o[4][VALUES] = {}, m[4], l[4] = {};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) m[r] = -INFINITY;
+    const bool works = warp * 4 < p.rows;
+    for (int key0 = p.range.first; key0 < p.range.end; key0 += KEYS32) {
+        __syncthreads();                                                        // the tile before is through
+        // a warp brings the keys warp, warp + 4, ..
+        for (int key = warp; key < KEYS32; key += WARPS) {
+            const int64_t at = key0 + key < p.range.end ? cache_row(a, p, key0 + key) : -1;
+            for (int d = lane * 4; d < D; d += 128) {
+                const float4 zero = make_float4(0, 0, 0, 0);
+                *reinterpret_cast<float4*>(k_s + key * PITCH + d) = at < 0 ? zero : *reinterpret_cast<const float4*>(keys + at * D + d);
+                *reinterpret_cast<float4*>(v_s + key * PITCH + d) = at < 0 ? zero : *reinterpret_cast<const float4*>(values + at * D + d);
+            }
+        }
+        if (warp == 0) {
+            const uint32_t there = __ballot_sync(0xffffffffu, key0 + lane < p.range.end && cache_row(a, p, key0 + lane) >= 0);
+            if (lane == 0) there_s = there;
+        }
+        __syncthreads();
+        if (!works) continue;
+        float s[4] = {};
+#pragma unroll 8
+        for (int d = 0; d < D; d += 4) {
+            const float4 kv = *reinterpret_cast<const float4*>(k_s + lane * PITCH + d);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float4 qv = *reinterpret_cast<const float4*>(q_s + (warp * 4 + r) * D + d);
+                s[r] = fmaf(qv.x, kv.x, s[r]); s[r] = fmaf(qv.y, kv.y, s[r]);
+                s[r] = fmaf(qv.z, kv.z, s[r]); s[r] = fmaf(qv.w, kv.w, s[r]);
+            }
+        }
+        const bool there = there_s >> lane & 1;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            s[r] = there ? s[r] * a.scale_log2 : -INFINITY;
+            const float now = fmaxf(m[r], warp_max(s[r])), subtract = now == -INFINITY ? 0.0f : now;
+            const float factor = exp2f(m[r] - subtract);
+            m[r] = now;
+            s[r] = exp2f(s[r] - subtract);
+            l[r] = l[r] * factor + s[r];                                        // a lane's own share
+#pragma unroll
+            for (int e = 0; e < VALUES; ++e) o[r][e] *= factor;
+        }
+#pragma unroll 8
+        for (int key = 0; key < KEYS32; ++key) {
+            float v[VALUES];
+#pragma unroll
+            for (int e = 0; e < VALUES; ++e) v[e] = v_s[key * PITCH + e * 32 + lane];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = __shfl_sync(0xffffffffu, s[r], key);
+#pragma unroll
+                for (int e = 0; e < VALUES; ++e) o[r][e] = fmaf(w, v[e], o[r][e]);
+            }
+        }
+    }
+    if (!works) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float total = warp_sum(l[r]);
+        if (warp * 4 + r >= p.rows) continue;
+        int head;
+        const int token = token_of(a, p, warp * 4 + r, head);
+        if (!takes_part(a, shared, token)) continue;
+        const int64_t part = part_of(a, token, head, p.slot);
+#pragma unroll
+        for (int e = 0; e < VALUES; ++e) a.part_o[part * D + e * 32 + lane] = o[r][e];
+        if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[r], total);
+    }
+}
+
+// ----------------------------------------------------------- joining the pieces
+// a warp a (token, head)
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS) join_kernel(Attend a) {
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    pdl_wait();
+    pdl_launch_dependents();
+    const int token = (int)(at / a.num_q), head = (int)(at % a.num_q);
+    if (token >= a.tokens) return;
+    constexpr int VALUES = D / 32;
+    float sum[VALUES] = {}, total = 0.0f;
+    if (row_of(a, token) >= 0) {
+        const int first = shared_of(a, token), own = keys_of(a, token) - first;
+        const int shared_used = first > 0 ? (first + piece_keys(first, a.shared_pieces) - 1) / piece_keys(first, a.shared_pieces) : 0;
+        const int own_used = own > 0 ? (own + piece_keys(own, a.own_pieces) - 1) / piece_keys(own, a.own_pieces) : 0;
+        float top = -INFINITY;
+        const int64_t part = part_of(a, token, head, 0);
+        auto slot_of = [&](int i) { return i < shared_used ? i : a.shared_pieces + i - shared_used; };
+        for (int i = 0; i < shared_used + own_used; ++i) top = fmaxf(top, a.part_ml[(part + slot_of(i)) * 2]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+        for (int i = 0; i < shared_used + own_used; ++i) {
+            const int64_t from = part + slot_of(i);
+            const float f = exp2f(a.part_ml[from * 2] - ref);
+            total = fmaf(f, a.part_ml[from * 2 + 1], total);
+#pragma unroll
+            for (int e = 0; e < VALUES; ++e) sum[e] = fmaf(f, a.part_o[from * D + e * 32 + lane], sum[e]);
+        }
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;                  // a token that is none, or sees no key: zeros
+    T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D;
+#pragma unroll
+    for (int e = 0; e < VALUES; ++e) out[e * 32 + lane] = from_float<T>(sum[e] * inverse);
+}
+
+// ------------------------------------------------------------------ host side
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+struct Plan { long long shared_items, own_items; int shared_pieces, own_pieces, own_tiles; };
+
+// Into how many pieces the keys are cut: enough for about three CTAs an SM, none shorter than MIN_KEYS.
+Plan plan_of(int tokens, int groups, int num_q, int num_kv, int max_shared, int max_own, int dtype) {
+    constexpr int MIN_KEYS = 128, CTAS = 3 * 148;
+    const int heads = num_q / num_kv, tile = dtype == TVB_F32 ? 16 : 64;
+    const long long tiles = groups > 0 && max_shared > 0 ? (long long)tokens * heads / tile + groups : 0;
+    auto pieces_of = [&](long long items, int keys) {
+        const long long wanted = items > 0 ? ceil_div(CTAS, items) : 1;
+        return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1), MIN_KEYS)), 64ll));
+    };
+    Plan p;
+    p.own_tiles = (heads + 15) / 16;
+    p.shared_pieces = tiles > 0 ? pieces_of(tiles * num_kv, max_shared) : 0;
+    p.own_pieces = pieces_of((long long)tokens * num_kv * p.own_tiles, max_own);
+    p.shared_items = tiles * num_kv * p.shared_pieces;
+    p.own_items = (long long)tokens * num_kv * p.own_tiles * p.own_pieces;
+    return p;
+}
+
+template <typename K> int launch(K kernel, long long grid, size_t shared, int pdl, cudaStream_t stream, const Attend& a) {
+    if (shared > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (e != cudaSuccess) return (int)e;
+    }
+    TvbLaunch at(dim3((unsigned)grid), dim3(THREADS), shared, stream, pdl);
+    const cudaError_t e = cudaLaunchKernelEx(&at.config, kernel, a);
+    return e == cudaSuccess ? tvb_last_error() : (int)e;
+}
+
+template <int D> int launch_all(const Attend& a, long long items, int dtype, int pdl, cudaStream_t s) {
+    const int e = dtype == TVB_F32 ? launch(attend_f32_kernel<D>, items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, s, a)
+                                   : launch(attend_bf16_kernel<D>, items, Tiles<D>::BYTES, pdl, s, a);
+    if (e) return e;
+    const long long joins = ceil_div((long long)a.tokens * a.num_q, WARPS);
+    return dtype == TVB_F32 ? launch(join_kernel<float, D>, joins, 0, pdl, s, a) : launch(join_kernel<bf16, D>, joins, 0, pdl, s, a);
+}
+
+}  // namespace
+
+// float32 of scratch
+extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int num_q, int num_kv, int head_dim, int max_shared, int max_own,
+                                                  int dtype) {
+    if (tokens <= 0 || num_kv <= 0) return 0;
+    const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
+    return (long long)tokens * num_q * (p.shared_pieces + p.own_pieces) * (head_dim + 2);
+}
+
+extern "C" int tvb_attention_shared(const void* q, long long q_stride, const void* keys, const void* values, const int* tables, int rows,
+                                    int width, const int* token_row, const int* positions, const int* group_starts, const int* shared_lens,
+                                    int groups, float* scratch, void* out, long long out_stride, int tokens, int pages, int page_size,
+                                    int num_q, int num_kv, int head_dim, int max_shared, int max_own, float scale, int dtype, int pdl,
+                                    void* stream) {
+    if (tokens <= 0) return 0;
+    if ((dtype != TVB_F32 && dtype != TVB_BF16) || num_kv <= 0 || num_q <= 0 || num_q % num_kv || page_size <= 0 || groups < 0 || rows < 0 ||
+        width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096)
+        return TVB_BAD_ARGUMENT;
+    const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
+    if (p.shared_items + p.own_items > 0x7fffffffLL || (long long)tokens * num_q > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
+    Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, scratch, nullptr, out, out_stride,
+             tokens, rows, width, p.shared_items > 0 ? groups : 0, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces,
+             (int)p.shared_items, p.own_tiles, scale * LOG2E};
+    a.part_ml = scratch + (long long)tokens * num_q * (p.shared_pieces + p.own_pieces) * head_dim;
+    cudaStream_t s = (cudaStream_t)stream;
+    const long long items = p.shared_items + p.own_items;
+    if (head_dim == 64) return launch_all<64>(a, items, dtype, pdl, s);
+    if (head_dim == 128) return launch_all<128>(a, items, dtype, pdl, s);
+    if (head_dim == 256) return launch_all<256>(a, items, dtype, pdl, s);
+    return TVB_BAD_ARGUMENT;
+}

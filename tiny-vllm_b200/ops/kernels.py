@@ -42,13 +42,13 @@ _launches = 0
 # Programmatic dependent launch for the kernels that wait for their predecessor themselves
 # (griddepcontrol.wait): they may start, and fetch weights, while the kernel before them ends.
 # TINYVLLM_B200_PDL=0 turns it off; a comma-separated list (gemm,norm,attention,attention_few,prefill,
-# sample,sample_second) keeps it for those kernels only (attention: the decode attention at every batch size;
+# sample,sample_second,attention_shared) keeps it for those kernels only (attention: the decode attention at every batch size;
 # attention_few: with up to PDL_ATTENTION_ROWS rows and only where the launch runs as CTAs of eight
 # warps that are all on the GPU at once, which find the SMs free: batch 1 to 3 gain 3 to 4 %, batch
 # 4 is level and batch 6 loses 3 %, its clusters waiting for room beside the projection's CTAs; prefill: the prompt's q/k norm, rotation and cache write,
 # and the tcgen05 attention; sample_second: the launch for the sampled rows of a large batch behind the one
 # for its greedy rows).
-_PDL_DEFAULT = ("gemm", "norm", "attention_few", "sample_second")
+_PDL_DEFAULT = ("gemm", "norm", "attention_few", "sample_second", "attention_shared")
 PDL_ATTENTION_ROWS = 3
 _setting = os.environ.get("TINYVLLM_B200_PDL", "1")
 PDL = frozenset() if _setting == "0" else frozenset(_PDL_DEFAULT if _setting == "1" else _setting.split(","))
@@ -2118,6 +2118,71 @@ def adapters_expand(part: torch.Tensor, up: torch.Tensor, ids: torch.Tensor, sca
              [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong] + [c_int] * 8 + [c_void_p])
     _check(fn(part.data_ptr(), up.data_ptr(), ids.data_ptr(), _ptr(scales), y.data_ptr(), y.stride(0), m, n, k, rank, adapters,
               dtype_tag(up.dtype), dtype_tag(y.dtype), _pdl("gemm"), _stream()), "adapters_expand")
+
+
+# ------------------------------------------ attention over keys in common (paged)
+def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                     block_tables: torch.Tensor, token_row: torch.Tensor, positions: torch.Tensor, *,
+                     group_starts: torch.Tensor, shared_lens: torch.Tensor, num_q: int, num_kv: int, head_dim: int,
+                     scale: float, max_shared: int | None = None, max_own: int | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Paged causal attention, as :func:`attention_rows` (``q`` with the heads of token t at t * q_token_stride; caches
+    [pages, num_kv, page_size, head_dim]; int32 tables, rows and positions; a token whose row or position is negative is
+    padding and gets zeros), for tokens of which groups share their first keys.
+
+    Group g is the tokens ``group_starts[g]`` to ``group_starts[g + 1]`` - 1 (int32 [groups + 1], ascending); its first
+    ``shared_lens[g]`` (int32 [groups]) positions hold the same keys and values for all of them, which are read once, through
+    the table of the group's first token that reaches them all.  A token that ends before them, or stands in no group, reads
+    its keys by itself.  ``max_shared`` and ``max_own``: no group shares more, no token has more keys behind its group's;
+    by them the work is cut up, the result does not depend on them beyond rounding (default: what the tables hold).  A key
+    whose page is no page of the cache is not seen.  bfloat16 and float32, head sizes 64, 128 and 256."""
+    tokens = positions.shape[0] if positions.dim() == 1 else -1
+    tag = dtype_tag(q.dtype)
+    if head_dim not in DECODE_HEAD_DIMS or num_kv < 1 or num_q < 1 or num_q % num_kv:
+        raise KernelError(f"attention_shared takes head sizes {DECODE_HEAD_DIMS} and whole groups of q heads "
+                          f"(head_dim {head_dim}, {num_q} / {num_kv} heads)")
+    if key_cache.dim() != 4 or key_cache.shape[1] != num_kv or key_cache.shape[3] != head_dim or key_cache.shape[2] < 1 \
+            or key_cache.dtype != q.dtype or not key_cache.is_contiguous() or value_cache.shape != key_cache.shape \
+            or value_cache.dtype != q.dtype or not value_cache.is_contiguous():
+        raise KernelError("attention_shared: caches must be contiguous [pages, num_kv, page_size, head_dim] of the type of q")
+    if tokens < 0 or not _is(positions, torch.int32, tokens) or not _is(token_row, torch.int32, tokens):
+        raise KernelError("attention_shared: token_row and positions must be contiguous int32 [tokens]")
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous():
+        raise KernelError("attention_shared: block_tables must be contiguous int32 [requests, blocks]")
+    groups = shared_lens.shape[0] if shared_lens.dim() == 1 else -1
+    if groups < 0 or not _is(shared_lens, torch.int32, groups) or not _is(group_starts, torch.int32, groups + 1):
+        raise KernelError("attention_shared: shared_lens must be contiguous int32 [groups], group_starts int32 [groups + 1]")
+    size, width = q.element_size(), num_q * head_dim
+    last = q.stride(-1) if q.dim() else 0
+    if last != 1 or q_token_stride < width or q_token_stride * size % 16 or q.data_ptr() % 16 \
+            or tokens > 0 and q.untyped_storage().nbytes() < (q.storage_offset() + (tokens - 1) * q_token_stride + width) * size:
+        raise KernelError("attention_shared: the heads of token t stand at q + t * q_token_stride, on 16 bytes, inside its memory")
+    held = block_tables.shape[1] * key_cache.shape[2]
+    max_shared = held if max_shared is None else min(max_shared, held)
+    max_own = held if max_own is None else min(max_own, held)
+    if max_shared < 0 or max_own < 0:
+        raise KernelError("attention_shared: max_shared and max_own are not negative")
+    if out is None:
+        _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
+        out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
+    else:
+        if out.shape != (tokens, width) or out.dtype != q.dtype or out.stride(1) != 1 or tokens > 1 and out.stride(0) < width:
+            raise KernelError("attention_shared: out must be [tokens, num_q * head_dim] of the type of q with contiguous rows")
+        _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
+    if tokens == 0:
+        return out
+    need = _fn("attention_shared", "tvb_attention_shared_scratch", [c_int] * 8, c_longlong)(
+        tokens, groups, num_q, num_kv, head_dim, max_shared, max_own, tag)
+    scratch = torch.empty(need, dtype=torch.float32, device=q.device)
+    fn = _fn("attention_shared", "tvb_attention_shared",
+             [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+              c_void_p, c_void_p, c_longlong] + [c_int] * 8 + [c_float, c_int, c_int, c_void_p])
+    _check(fn(q.data_ptr(), q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
+              block_tables.shape[0], block_tables.shape[1], token_row.data_ptr(), positions.data_ptr(), group_starts.data_ptr(),
+              shared_lens.data_ptr(), groups, scratch.data_ptr(), out.data_ptr(), out.stride(0), tokens, key_cache.shape[0],
+              key_cache.shape[2], num_q, num_kv, head_dim, max_shared, max_own, scale, tag, _pdl("attention_shared"), _stream()),
+           "attention_shared", 2)
+    return out
 
 
 # ------------------------------------------------- tiled attention (bfloat16)
