@@ -2,25 +2,31 @@
 //
 //   y[t] + s_a (x[t] A_a^T) B_a^T        a = ids[t]; rows whose number names no adapter stay as they are
 //
-// with A [adapters, rank, k] and B [adapters, n, rank].  Two kernels: `shrink` makes u = x A^T (float32, summed over k in
-// pieces that are added in order), `expand` takes u through B and adds it to y.  Rows come in any order; a tile of rows
-// goes once over every adapter that one of its rows has.
+// with A [adapters, rank, k] and B [adapters, n, rank].  Two kernels: `shrink` makes u = s x A^T (float32 sums over k in
+// pieces that the CTAs of a cluster add in order, through distributed shared memory), `expand` takes u through B and adds
+// it to y.  Rows come in any order; a tile of rows goes once over every adapter that one of its rows has, the adapters of a
+// tile side by side in the grid as far as it goes.
 //
-// bfloat16: mma.sync m16n8k16 straight from global memory to registers (the products are a hundredth of the projection's,
-// and a rank of 16 is one step of k: there is nothing for a pipeline through shared memory to hide behind).  A thread
-// loads 16 bytes, eight neighbouring k, of each row; which k a fragment's place stands for is permuted alike in both
-// operands.  u enters the second product as two bfloat16 whose sum is u to 2^-17 of it, so that no rounding of u is seen
-// beside that of the result.  A row takes the sums of its own adapter alone: what other adapters hold, infinities among
-// them, does not reach it.
+// bfloat16: mma.sync m16n8k16 (the products are a hundredth of the projection's: what counts is that A, B, x and y come in
+// with enough of them in flight).  Up to FEW_ROWS rows a CTA of `shrink` has 16 rows and loads straight into registers: a
+// thread takes 16 bytes, eight neighbouring k, of each row, and which k a fragment's place stands for is permuted alike in
+// both operands.  More rows go 64 a CTA through a ring in shared memory that cp.async fills.  u leaves in two bfloat16 whose
+// sum is u to 2^-17 of it, so that no rounding of u is seen beside that of the result.  A row takes the sums of its own
+// adapter alone: what other adapters hold, infinities among them, does not reach it.
 // float32: the float32 cores.
 //
-// Bound by reading A, B and x and by reading and writing y.
+// Bound by the latency of their chains of loads for few rows, by reading x and reading and writing y for many.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int MAX_RANK = 256;
+constexpr int MAX_SPLITS = 8;                   // pieces of k: the CTAs of a cluster
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -50,27 +56,99 @@ template <bool WIDE> __device__ __forceinline__ uint2 load_4(const bf16* row, in
     }
 }
 
+__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
+}
+
+// What both kernels agree on: u as `hi` and `lo` rows [m][2][padded rank] (bfloat16), or [m][rank] (float32).
+__device__ __forceinline__ int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
+
+// u of a row and rank: scaled, in two parts; places behind the rank are zeros
+__device__ __forceinline__ void store_u(bf16* u, int row, int rank, int padded, float value) {
+    const bf16 hi = from_float<bf16>(value);
+    u[((int64_t)row * 2) * padded + rank] = hi;
+    u[((int64_t)row * 2 + 1) * padded + rank] = from_float<bf16>(value - to_float<bf16>(hi));
+}
+
 struct Shrink {
     const bf16* x;
     int64_t ldx;
     const bf16* down;
     const int* ids;
-    float* part;                                // [splits, m, rank]
+    const float* scales;                        // [adapters] or null
+    bf16* u;
     int m, k, rank, adapters;
-    int splits, blocks_per_split;               // blocks of 32 k
+    int splits, per_split;                      // pieces of k (CTAs of a cluster); blocks of 32 (few rows) or stages in each
 };
 
-// One pass over k blocks first, first + step, .. < end: sums[j] += 16 rows of x times 8 ranks from 8 j on.
-template <int NR, bool WIDE>
-__device__ __forceinline__ void shrink_pass(const Shrink& s, const bf16* lo, const bf16* hi, bool lo_there, bool hi_there, const bf16* down,
-                                            int ranks, int first, int step, int end, float (&sums)[NR][4]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr int AHEAD = NR <= 2 ? 4 : 2;      // blocks in flight
-    for (int b0 = first; b0 < end; b0 += AHEAD * step) {
+// The adapters of a tile's rows, each once, in the order of the rows; `ids` of the rows (-1: none).  All threads call.
+template <int ROWS> __device__ __forceinline__ int find_adapters(const int* all, int m, int adapters, int row0, int* ids, int* distinct) {
+    static_assert(ROWS <= 64, "two warps");
+    __shared__ int counts[2];
+    const int tid = threadIdx.x;
+    if (tid < ROWS) {
+        const int id = row0 + tid < m ? all[row0 + tid] : -1;
+        ids[tid] = (unsigned)id < (unsigned)adapters ? id : -1;
+    }
+    if (tid < 2) counts[tid] = 0;
+    __syncthreads();
+    bool first = false;
+    uint32_t firsts = 0;
+    if (tid < 64) {                             // whole warps
+        if (tid < ROWS && ids[tid] >= 0) {
+            first = true;
+            for (int j = 0; j < tid; ++j) first = first && ids[j] != ids[tid];
+        }
+        firsts = __ballot_sync(0xffffffffu, first);
+        if ((tid & 31) == 0) counts[tid >> 5] = __popc(firsts);
+    }
+    __syncthreads();
+    if (first) distinct[(tid >= 32 ? counts[0] : 0) + __popc(firsts & ((1u << (tid & 31)) - 1u))] = ids[tid];
+    __syncthreads();
+    return counts[0] + counts[1];
+}
+
+// ---- up to FEW_ROWS rows: 16 rows, 16 ranks and one adapter (the blockIdx.z-th of the rows') a CTA, its warps share k
+template <bool WIDE>
+__global__ void __launch_bounds__(THREADS) shrink_few_kernel(Shrink s) {
+    constexpr int NR = 2, AHEAD = 4;            // groups of 8 ranks; blocks of 32 k in flight
+    __shared__ float met[WARPS][16][8 * NR];
+    __shared__ float pieces[MAX_SPLITS][16 * 8 * NR];                           // of the cluster's first CTA
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster_arrive_relaxed();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % s.splits, rank0 = blockIdx.x / s.splits * 8 * NR, ranks = s.rank - rank0;
+    const int row0 = blockIdx.y * 16;
+    const int end = min((s.k + 31) / 32, (split + 1) * s.per_split);
+    pdl_wait();
+    pdl_launch_dependents();
+    // lanes 0 .. 15: a row's adapter, and the rows that share it
+    int id = -1;
+    if (lane < 16 && row0 + lane < s.m) {
+        id = s.ids[row0 + lane];
+        if ((unsigned)id >= (unsigned)s.adapters) id = -1;
+    }
+    const uint32_t alike = __match_any_sync(0xffffffffu, id);
+    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
+    for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
+    if (leaders == 0) {                         // the whole cluster
+        cluster_wait();
+        return;
+    }
+    const int leader = __ffs(leaders) - 1;
+    const int adapter = __shfl_sync(0xffffffffu, id, leader);
+    const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader);
+    const bf16* down = s.down + ((int64_t)adapter * s.rank + rank0) * s.k;
+    const bool lo_there = rows >> g & 1, hi_there = rows >> (g + 8) & 1;
+    const bf16* lo = s.x + (int64_t)(row0 + g) * s.ldx;
+    const bf16* hi = s.x + (int64_t)(row0 + g + 8) * s.ldx;
+    float sums[NR][4] = {};
+    for (int b0 = split * s.per_split + warp; b0 < end; b0 += AHEAD * WARPS) {
         uint4 xl[AHEAD], xh[AHEAD], w[AHEAD][NR];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int b = b0 + i * step, at = b * 32 + 8 * t;
+            const int b = b0 + i * WARPS, at = b * 32 + 8 * t;
             xl[i] = load_8<WIDE>(lo, at, s.k, lo_there && b < end);
             xh[i] = load_8<WIDE>(hi, at, s.k, hi_there && b < end);
 #pragma unroll
@@ -85,372 +163,410 @@ __device__ __forceinline__ void shrink_pass(const Shrink& s, const bf16* lo, con
                 mma_16816(sums[j], xl[i].z, xh[i].z, xl[i].w, xh[i].w, w[i][j].z, w[i][j].w);
             }
     }
+#pragma unroll
+    for (int j = 0; j < NR; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) met[warp][e < 2 ? g : g + 8][8 * j + 2 * t + (e & 1)] = sums[j][e];
+    __syncthreads();
+    cluster_wait();                             // the first CTA runs
+    float* first_pieces = cluster.map_shared_rank(&pieces[0][0], 0);
+    for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
+        const int row = i / (8 * NR), rank = i % (8 * NR);
+        float sum = met[0][row][rank];
+#pragma unroll
+        for (int w = 1; w < WARPS; ++w) sum += met[w][row][rank];
+        first_pieces[split * 16 * 8 * NR + i] = sum;
+    }
+    cluster_arrive();
+    cluster_wait();
+    if (split != 0) return;
+    const float scale = s.scales ? s.scales[adapter] : 1.0f;
+    const int padded = padded_rank(s.rank);
+    for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
+        const int row = i / (8 * NR), rank = i % (8 * NR);
+        if (!(rows >> row & 1)) continue;
+        float sum = pieces[0][i];
+        for (int p = 1; p < s.splits; ++p) sum += pieces[p][i];
+        store_u(s.u, row0 + row, rank0 + rank, padded, rank < ranks ? sum * scale : 0.0f);
+    }
 }
 
-// BY_ROWS: a warp has 16 rows of its own, over all k of the split, and goes through their adapters in turn.  Else: the CTA
-// has 16 rows and the blockIdx.z-th of their adapters; its warps share k and meet in shared memory.
-template <int NR, bool BY_ROWS, bool WIDE>
-__global__ void __launch_bounds__(THREADS) shrink_kernel(Shrink s) {
-    __shared__ float met[BY_ROWS ? 1 : WARPS][16][8 * NR];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % s.splits, rank0 = blockIdx.x / s.splits * 8 * NR, ranks = s.rank - rank0;
-    const int row0 = BY_ROWS ? (blockIdx.y * WARPS + warp) * 16 : blockIdx.y * 16;
-    const int first = split * s.blocks_per_split, end = min((s.k + 31) / 32, first + s.blocks_per_split);
+// ---- more rows: 64 rows and RANKS ranks a CTA, 16 rows a warp; stages of 64 k
+constexpr int STAGE_K = 64, STAGES = 4, STAGE_PITCH = STAGE_K + 8;
+template <int RANKS> struct ManyShared {
+    static constexpr int STAGE = (64 + RANKS) * STAGE_PITCH;                    // elements
+    static constexpr int SUM_PITCH = RANKS + 4;
+    static constexpr int RING_BYTES = STAGES * STAGE * 2, SUM_BYTES = 64 * SUM_PITCH * 4;
+    static constexpr int BYTES = RING_BYTES > SUM_BYTES ? RING_BYTES : SUM_BYTES;
+};
+template <int RANKS, bool WIDE>
+__global__ void __launch_bounds__(THREADS) shrink_many_kernel(Shrink s) {
+    using Shared = ManyShared<RANKS>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ int ids[64], distinct[64];
+    bf16* ring = reinterpret_cast<bf16*>(raw);
+    float* sums_s = reinterpret_cast<float*>(raw);                              // [64][SUM_PITCH], over the ring
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x % s.splits, rank0 = blockIdx.x / s.splits * RANKS, ranks = min(RANKS, s.rank - rank0);
+    const int row0 = blockIdx.y * 64, padded = padded_rank(s.rank);
+    const int first = split * s.per_split, stages = max(0, min((s.k + STAGE_K - 1) / STAGE_K, first + s.per_split) - first);
     pdl_wait();
     pdl_launch_dependents();
-    if (BY_ROWS && row0 >= s.m) return;
-    // lanes 0 .. 15: a row's adapter, and the rows that share it
-    int id = -1;
-    if (lane < 16 && row0 + lane < s.m) {
-        id = s.ids[row0 + lane];
-        if ((unsigned)id >= (unsigned)s.adapters) id = -1;
-    }
-    const uint32_t alike = __match_any_sync(0xffffffffu, id);
-    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
-    if constexpr (!BY_ROWS) {
-        for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
-        if (leaders == 0) return;               // the whole CTA
-        leaders &= -leaders;
-    }
-    const int lo_row = row0 + g, hi_row = row0 + g + 8;
-    const bf16* lo = s.x + (int64_t)lo_row * s.ldx;
-    const bf16* hi = s.x + (int64_t)hi_row * s.ldx;
-    while (leaders) {
-        const int leader = __ffs(leaders) - 1;
-        leaders &= leaders - 1;
-        const int adapter = __shfl_sync(0xffffffffu, id, leader);
-        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader);
+    const int count = find_adapters<64>(s.ids, s.m, s.adapters, row0, ids, distinct);
+    for (int d = blockIdx.z; d < count; d += gridDim.z) {                       // the same for the whole cluster
+        const int adapter = distinct[d];
         const bf16* down = s.down + ((int64_t)adapter * s.rank + rank0) * s.k;
-        const bool lo_there = rows >> g & 1, hi_there = rows >> (g + 8) & 1;
-        float sums[NR][4] = {};
-        shrink_pass<NR, WIDE>(s, lo, hi, lo_there, hi_there, down, ranks, BY_ROWS ? first : first + warp, BY_ROWS ? 1 : WARPS, end, sums);
-        if constexpr (BY_ROWS) {
-#pragma unroll
-            for (int j = 0; j < NR; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int rank = 8 * j + 2 * t + (e & 1);
-                    if ((e < 2 ? lo_there : hi_there) && rank < ranks)
-                        s.part[((int64_t)split * s.m + (e < 2 ? lo_row : hi_row)) * s.rank + rank0 + rank] = sums[j][e];
+        auto load = [&](int stage) {
+            if (stage < stages) {
+                bf16* x_s = ring + stage % STAGES * Shared::STAGE;
+                bf16* a_s = x_s + 64 * STAGE_PITCH;
+                const int k0 = (first + stage) * STAGE_K;
+                for (int i = tid; i < (64 + RANKS) * (STAGE_K / 8); i += THREADS) {
+                    const int row = i / (STAGE_K / 8), at = k0 + i % (STAGE_K / 8) * 8;
+                    const bool of_x = row < 64;
+                    const bool there = of_x ? ids[row] == adapter : row - 64 < ranks;
+                    const bf16* from = of_x ? s.x + (int64_t)(there ? row0 + row : 0) * s.ldx : down + (int64_t)(there ? row - 64 : 0) * s.k;
+                    bf16* to = (of_x ? x_s + row * STAGE_PITCH : a_s + (row - 64) * STAGE_PITCH) + i % (STAGE_K / 8) * 8;
+                    if constexpr (WIDE) cp_async_16(to, from + (at < s.k ? at : 0), there && at < s.k);
+                    else *reinterpret_cast<uint4*>(to) = load_8<false>(from, at, s.k, there);
                 }
-        } else {
+            }
+            cp_async_commit();
+        };
 #pragma unroll
-            for (int j = 0; j < NR; ++j)
+        for (int i = 0; i < STAGES - 1; ++i) load(i);
+        float sums[RANKS / 8][4] = {};
+        for (int stage = 0; stage < stages; ++stage) {
+            cp_async_wait<STAGES - 2>();
+            __syncthreads();                    // the stage is there, and the one that the next load overwrites is through
+            load(stage + STAGES - 1);
+            const bf16* x_s = ring + stage % STAGES * Shared::STAGE + (warp * 16 + (lane & 15)) * STAGE_PITCH + (lane >> 4) * 8;
+            const bf16* a_s = ring + stage % STAGES * Shared::STAGE + 64 * STAGE_PITCH;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) met[warp][e < 2 ? g : g + 8][8 * j + 2 * t + (e & 1)] = sums[j][e];
-            __syncthreads();
-            for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
-                const int row = i / (8 * NR), rank = i % (8 * NR);
-                if (!(rows >> row & 1) || rank >= ranks) continue;
-                float sum = met[0][row][rank];
+            for (int kk = 0; kk < STAGE_K / 16; ++kk) {
+                uint32_t a[4];
+                ldmatrix_x4(a, x_s + kk * 16);
 #pragma unroll
-                for (int w = 1; w < WARPS; ++w) sum += met[w][row][rank];
-                s.part[((int64_t)split * s.m + row0 + row) * s.rank + rank0 + rank] = sum;
+                for (int j = 0; j < RANKS / 16; ++j) {
+                    uint32_t b[4];
+                    const int matrix = lane >> 3;
+                    ldmatrix_x4(b, a_s + (j * 16 + (matrix >> 1) * 8 + (lane & 7)) * STAGE_PITCH + kk * 16 + (matrix & 1) * 8);
+                    mma_16816(sums[2 * j], a[0], a[1], a[2], a[3], b[0], b[1]);
+                    mma_16816(sums[2 * j + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+                }
             }
         }
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < RANKS / 8; ++j)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                *reinterpret_cast<float2*>(sums_s + (warp * 16 + g + 8 * half) * Shared::SUM_PITCH + 8 * j + 2 * t) =
+                    make_float2(sums[j][2 * half], sums[j][2 * half + 1]);
+        cluster_arrive();
+        cluster_wait();
+        // a CTA adds the pieces of its share of the rows
+        const float scale = s.scales ? s.scales[adapter] : 1.0f;
+        const int share = 64 / s.splits;
+        for (int i = tid; i < share * RANKS; i += THREADS) {
+            const int row = split * share + i / RANKS, rank = i % RANKS;
+            if (ids[row] != adapter || rank0 + rank >= padded) continue;
+            float piece[MAX_SPLITS];
+#pragma unroll
+            for (int p = 0; p < MAX_SPLITS; ++p)
+                piece[p] = p < s.splits ? cluster.map_shared_rank(sums_s, p)[row * Shared::SUM_PITCH + rank] : 0.0f;
+            float sum = piece[0];
+#pragma unroll
+            for (int p = 1; p < MAX_SPLITS; ++p) sum += piece[p];
+            store_u(s.u, row0 + row, rank0 + rank, padded, rank < ranks ? sum * scale : 0.0f);
+        }
+        cluster_arrive();                       // nobody reads these sums any more
+        cluster_wait();
     }
 }
 
 struct Expand {
-    const float* part;
+    const void* u;
     const void* up;                             // [adapters, n, rank]
     const int* ids;
-    const float* scales;                        // [adapters] or null
     void* y;
     int64_t ldy;
-    int m, n, rank, adapters, splits;
+    int m, n, rank, adapters;
 };
 
-// u of a tile's rows, scaled, from its pieces in order; what a row without an adapter has is of no account
-template <typename F> __device__ __forceinline__ void gather_u(const Expand& s, int row0, int rows, const int* ids, F&& put) {
-    for (int i = threadIdx.x; i < rows * s.rank; i += blockDim.x) {
-        const int row = i / s.rank, rank = i % s.rank;
-        float sum = 0.0f;
-        if (ids[row] >= 0) {
-            const float* at = s.part + ((int64_t)row0 + row) * s.rank + rank;
-            for (int p = 0; p < s.splits; ++p) sum += at[(int64_t)p * s.m * s.rank];
-            if (s.scales) sum *= s.scales[ids[row]];
-        }
-        put(row, rank, sum);
-    }
-}
-
-// the numbers of a tile's rows (-1: none), and the tile's adapters, each once, in `distinct`
-template <int ROWS> __device__ __forceinline__ int find_adapters(const Expand& s, int row0, int* ids, int* distinct, int* count) {
-    const int tid = threadIdx.x;
-    if (tid == 0) *count = 0;
-    if (tid < ROWS) {
-        int id = row0 + tid < s.m ? s.ids[row0 + tid] : -1;
-        ids[tid] = (unsigned)id < (unsigned)s.adapters ? id : -1;
-    }
-    __syncthreads();
-    if (tid < ROWS && ids[tid] >= 0) {
-        bool first = true;
-        for (int j = 0; j < tid; ++j) first = first && ids[j] != ids[tid];
-        // (in any order: a row adds the sums of one adapter)
-        if (first) distinct[atomicAdd(count, 1)] = ids[tid];
-    }
-    __syncthreads();
-    return *count;
-}
-
-// A tile of 16 MT rows and 128 columns of y, 32 columns a warp.  The columns of an n-tile are spread so that a thread holds
-// eight neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.
+// A tile of 16 MT rows and 128 columns of y, 32 columns a warp, one adapter after another.  The columns of an n-tile are
+// spread so that a thread holds eight neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.
 template <int MT, typename Y, bool WIDE>
 __global__ void __launch_bounds__(THREADS) expand_kernel(Expand s) {
-    constexpr int ROWS = 16 * MT, NT = 4;
-    extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ int ids[ROWS], distinct[ROWS], distinct_count;
-    const int padded = (s.rank + 15) / 16 * 16, pitch = padded + 8;
-    bf16* u_hi = reinterpret_cast<bf16*>(raw);                                  // [ROWS][pitch]
-    bf16* u_lo = u_hi + ROWS * pitch;
+    constexpr int ROWS = 16 * MT, NT = 4, STEPS = 4;                            // steps of 16 ranks whose B is held
+    __shared__ int ids[ROWS], distinct[ROWS];
+    const int padded = padded_rank(s.rank);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = blockIdx.y * ROWS, n0 = blockIdx.x * 128 + warp * 32;
-    const int rows = min(ROWS, s.m - row0);
-    const bf16* up = reinterpret_cast<const bf16*>(s.up);
+    const int row0 = blockIdx.y * ROWS, n0 = blockIdx.x * 128 + warp * 32, column = n0 + 8 * t;
+    const bf16* u = reinterpret_cast<const bf16*>(s.u);
+    const bool whole = WIDE && column + 8 <= s.n;
     pdl_wait();
     pdl_launch_dependents();
-    const int count = find_adapters<ROWS>(s, row0, ids, distinct, &distinct_count);
-    if (count == 0) return;
-    for (int i = threadIdx.x; i < ROWS * pitch; i += THREADS) { u_hi[i] = from_float<bf16>(0.0f); u_lo[i] = from_float<bf16>(0.0f); }
-    __syncthreads();
-    gather_u(s, row0, rows, ids, [&](int row, int rank, float u) {
-        const bf16 hi = from_float<bf16>(u);
-        u_hi[row * pitch + rank] = hi;
-        u_lo[row * pitch + rank] = from_float<bf16>(u - to_float<bf16>(hi));
-    });
-    __syncthreads();
-    float total[MT][NT][4] = {};
-    for (int d = 0; d < count; ++d) {
+    const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
+    for (int d = blockIdx.z; d < count; d += gridDim.z) {
         const int adapter = distinct[d];
-        const bf16* b = up + (int64_t)adapter * s.n * s.rank;
-        float sums[MT][NT][4] = {};
-        for (int r0 = 0; r0 < padded; r0 += 16) {
-            uint2 w[NT];
+        const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
+        bool mine[MT][2];
+        uint4 old[MT][2][sizeof(Y) / 2];                                        // of y, asked for first
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const int column = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
-                w[j] = load_4<WIDE>(b + (int64_t)column * s.rank, r0 + 4 * t, s.rank, column < s.n);
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = 16 * i + g + 8 * half;
+                mine[i][half] = ids[row] == adapter;
+                if (mine[i][half] && whole) {
+                    const uint4* y = reinterpret_cast<const uint4*>(reinterpret_cast<const Y*>(s.y) + (int64_t)(row0 + row) * s.ldy + column);
+#pragma unroll
+                    for (int q = 0; q < (int)sizeof(Y) / 2; ++q) old[i][half][q] = y[q];
+                }
             }
+        float sums[MT][NT][4] = {};
+        for (int r0 = 0; r0 < padded; r0 += 16 * STEPS) {
+            uint2 w[STEPS][NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const bf16* at = u_hi + (16 * i + g) * pitch + r0 + 4 * t;
-                const uint2 hl = *reinterpret_cast<const uint2*>(at), hh = *reinterpret_cast<const uint2*>(at + 8 * pitch);
-                const bf16* rest = at + ROWS * pitch;
-                const uint2 ll = *reinterpret_cast<const uint2*>(rest), lh = *reinterpret_cast<const uint2*>(rest + 8 * pitch);
+            for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    mma_16816(sums[i][j], hl.x, hh.x, hl.y, hh.y, w[j].x, w[j].y);
-                    mma_16816(sums[i][j], ll.x, lh.x, ll.y, lh.y, w[j].x, w[j].y);
+                    const int at = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
+                    w[k][j] = load_4<WIDE>(b + (int64_t)at * s.rank, r0 + 16 * k + 4 * t, s.rank, at < s.n);
                 }
-            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int k = 0; k < STEPS; ++k) {
+                    if (r0 + 16 * k >= padded) break;
+                    const bf16* at = u + ((int64_t)(row0 + 16 * i + g) * 2) * padded + r0 + 16 * k + 4 * t;
+                    const uint2 none = make_uint2(0, 0);
+                    const uint2 hl = mine[i][0] ? *reinterpret_cast<const uint2*>(at) : none;
+                    const uint2 ll = mine[i][0] ? *reinterpret_cast<const uint2*>(at + padded) : none;
+                    const uint2 hh = mine[i][1] ? *reinterpret_cast<const uint2*>(at + 16 * padded) : none;
+                    const uint2 lh = mine[i][1] ? *reinterpret_cast<const uint2*>(at + 17 * padded) : none;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        mma_16816(sums[i][j], hl.x, hh.x, hl.y, hh.y, w[k][j].x, w[k][j].y);
+                        mma_16816(sums[i][j], ll.x, lh.x, ll.y, lh.y, w[k][j].x, w[k][j].y);
+                    }
+                }
         }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const bool lo = ids[16 * i + g] == adapter, hi = ids[16 * i + g + 8] == adapter;
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int half = 0; half < 2; ++half) {
+                if (!mine[i][half]) continue;
+                Y* y = reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + 16 * i + g + 8 * half) * s.ldy + column;
+                float add[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < 2 ? lo : hi) total[i][j][e] = sums[i][j][e];
-        }
-    }
-    const int column = n0 + 8 * t;
+                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[i][j][2 * half]; add[2 * j + 1] = sums[i][j][2 * half + 1]; }
+                if (whole) {
+                    if constexpr (sizeof(Y) == 2) {
+                        float v[8];
+                        unpack_bf16x8(old[i][half][0], v);
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+                        for (int e = 0; e < 8; ++e) add[e] += v[e];
+                        *reinterpret_cast<uint4*>(y) = pack_bf16x8(add);
+                    } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int row = 16 * i + g + 8 * half;
-            if (row >= rows || ids[row] < 0) continue;
-            Y* y = reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + row) * s.ldy + column;
-            float add[8];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) { add[2 * j] = total[i][j][2 * half]; add[2 * j + 1] = total[i][j][2 * half + 1]; }
-            if (WIDE && column + 8 <= s.n) {
-                if constexpr (sizeof(Y) == 2) {
-                    float old[8];
-                    unpack_bf16x8(*reinterpret_cast<const uint4*>(y), old);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) add[e] += old[e];
-                    *reinterpret_cast<uint4*>(y) = pack_bf16x8(add);
+                        for (int q = 0; q < 2; ++q) {
+                            const uint4 v = old[i][half][q];
+                            reinterpret_cast<float4*>(y)[q] =
+                                make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
+                                            __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
+                        }
+                    }
                 } else {
-                    const float4 a = reinterpret_cast<const float4*>(y)[0], c = reinterpret_cast<const float4*>(y)[1];
-                    reinterpret_cast<float4*>(y)[0] = make_float4(a.x + add[0], a.y + add[1], a.z + add[2], a.w + add[3]);
-                    reinterpret_cast<float4*>(y)[1] = make_float4(c.x + add[4], c.y + add[5], c.z + add[6], c.w + add[7]);
-                }
-            } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (column + e < s.n) y[e] = from_float<Y>(to_float<Y>(y[e]) + add[e]);
+                    for (int e = 0; e < 8; ++e)
+                        if (column + e < s.n) y[e] = from_float<Y>(to_float<Y>(y[e]) + add[e]);
+                }
             }
-        }
+    }
 }
 
-// ---- float32: a warp makes four ranks of a row over its split of k
+// ---- float32: a warp makes four ranks of a row over its piece of k
 struct Shrink32 {
     const float* x;
     int64_t ldx;
     const float* down;
     const int* ids;
-    float* part;
+    const float* scales;
+    float* u;                                   // [m, rank]
     int m, k, rank, adapters, splits, per_split;
 };
 template <int VEC> __global__ void __launch_bounds__(THREADS) shrink_f32_kernel(Shrink32 s) {
+    __shared__ float pieces[MAX_SPLITS][WARPS][4];                              // of the cluster's first CTA
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster_arrive_relaxed();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int per_row = s.splits * ((s.rank + 4 * WARPS - 1) / (4 * WARPS)), place = blockIdx.x % per_row;
     const int row = blockIdx.x / per_row, split = place % s.splits, rank0 = (place / s.splits * WARPS + warp) * 4;
     pdl_wait();
     pdl_launch_dependents();
     const int id = s.ids[row];
-    if ((unsigned)id >= (unsigned)s.adapters || rank0 >= s.rank) return;
-    const float* x = s.x + (int64_t)row * s.ldx;
-    const float* down = s.down + ((int64_t)id * s.rank + rank0) * s.k;
-    const int end = min(s.k, (split + 1) * s.per_split);
+    const bool any = (unsigned)id < (unsigned)s.adapters;                       // the same for the whole cluster
     float sums[4] = {};
-    for (int at = split * s.per_split + lane * VEC; at < end; at += 32 * VEC) {
-        float v[VEC], w[VEC];
-        load_values<VEC>(x + at, v);
+    if (any && rank0 < s.rank) {
+        const float* x = s.x + (int64_t)row * s.ldx;
+        const float* down = s.down + ((int64_t)id * s.rank + rank0) * s.k;
+        const int end = min(s.k, (split + 1) * s.per_split);
+#pragma unroll 2
+        for (int at = split * s.per_split + lane * VEC; at < end; at += 32 * VEC) {
+            float v[VEC], w[4][VEC];
+            load_values<VEC>(x + at, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (rank0 + j >= s.rank) break;
-            load_values<VEC>(down + (int64_t)j * s.k + at, w);
+            for (int j = 0; j < 4; ++j) load_values<VEC>(down + (int64_t)(rank0 + j < s.rank ? j : 0) * s.k + at, w[j]);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sums[j] = fmaf(v[e], w[e], sums[j]);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) sums[j] = fmaf(v[e], w[j][e], sums[j]);
         }
     }
+    cluster_wait();                             // the first CTA runs
+    float* first_pieces = cluster.map_shared_rank(&pieces[0][0][0], 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float sum = warp_sum(sums[j]);
-        if (lane == j && rank0 + j < s.rank) s.part[((int64_t)split * s.m + row) * s.rank + rank0 + j] = sum;
+        if (lane == j) first_pieces[(split * WARPS + warp) * 4 + j] = sum;
     }
+    cluster_arrive();
+    cluster_wait();
+    if (split != 0 || !any || lane >= 4 || rank0 + lane >= s.rank) return;
+    float sum = pieces[0][warp][lane];
+    for (int p = 1; p < s.splits; ++p) sum += pieces[p][warp][lane];
+    s.u[(int64_t)row * s.rank + rank0 + lane] = s.scales ? sum * s.scales[id] : sum;
 }
 
 // a thread makes one column of 16 rows
 template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(Expand s) {
     constexpr int ROWS = 16;
     extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ int ids[ROWS], distinct[ROWS], distinct_count;
-    float* u = reinterpret_cast<float*>(raw);                                   // [ROWS][pitch]
-    const int pitch = (s.rank + 3) / 4 * 4;
+    __shared__ int ids[ROWS], distinct[ROWS];
+    float* u = reinterpret_cast<float*>(raw);                                   // [ROWS][rank]
     const int row0 = blockIdx.y * ROWS, rows = min(ROWS, s.m - row0), column = blockIdx.x * THREADS + threadIdx.x;
     pdl_wait();
     pdl_launch_dependents();
-    const int count = find_adapters<ROWS>(s, row0, ids, distinct, &distinct_count);
-    if (count == 0) return;
-    gather_u(s, row0, rows, ids, [&](int row, int rank, float v) { u[row * pitch + rank] = v; });
-    __syncthreads();
+    for (int i = threadIdx.x; i < rows * s.rank; i += THREADS) u[i] = reinterpret_cast<const float*>(s.u)[(int64_t)row0 * s.rank + i];
+    const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
     if (column >= s.n) return;
     for (int d = 0; d < count; ++d) {
-        const float* b = reinterpret_cast<const float*>(s.up) + ((int64_t)distinct[d] * s.n + column) * s.rank;
-        float sums[ROWS] = {};
+        const int adapter = distinct[d];
+        const float* b = reinterpret_cast<const float*>(s.up) + ((int64_t)adapter * s.n + column) * s.rank;
+        float* y = reinterpret_cast<float*>(s.y) + (int64_t)row0 * s.ldy + column;
+        float sums[ROWS];
+#pragma unroll
+        for (int row = 0; row < ROWS; ++row) sums[row] = ids[row] == adapter ? y[row * s.ldy] : 0.0f;
+        float total[ROWS] = {};
+#pragma unroll 2
         for (int r = 0; r < s.rank; r += VEC) {
             float w[VEC];
             load_values<VEC>(b + r, w);
 #pragma unroll
             for (int row = 0; row < ROWS; ++row)
-                if (ids[row] == distinct[d])
+                if (ids[row] == adapter)
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) sums[row] = fmaf(u[row * pitch + r + e], w[e], sums[row]);
+                    for (int e = 0; e < VEC; ++e) total[row] = fmaf(u[row * s.rank + r + e], w[e], total[row]);
         }
 #pragma unroll
         for (int row = 0; row < ROWS; ++row)
-            if (row < rows && ids[row] == distinct[d]) {
-                float* y = reinterpret_cast<float*>(s.y) + (int64_t)(row0 + row) * s.ldy + column;
-                *y += sums[row];
-            }
+            if (ids[row] == adapter) y[row * s.ldy] = sums[row] + total[row];
     }
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int FEW_ROWS = 128;                   // rows up to which a CTA has 16 rows and one adapter
+constexpr int FEW_ROWS = 128;                   // rows up to which a CTA of `shrink` has 16 rows and one adapter
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// pieces of k, so that the grid fills the GPU about twice and a warp keeps a few blocks of 32
-int shrink_splits(int m, int k, int rank, int f32) {
-    const int blocks = ceil_div(k, 32);
-    if (f32) return max(1, min(min(8, k / 512), ceil_div(1184, m * ceil_div(rank, 16))));
-    if (m <= FEW_ROWS) return max(1, min(16, blocks / 8));
-    return max(1, min(min(8, blocks / 16), ceil_div(444, ceil_div(m, 64) * ceil_div(rank, 64))));
-}
-
-template <typename K, typename S> int launch(K kernel, dim3 grid, size_t shared, int pdl, cudaStream_t stream, const S& s) {
+template <typename K, typename S> int launch(K kernel, dim3 grid, size_t shared, int cluster, int pdl, cudaStream_t stream, const S& s) {
     if (shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * 64 * (MAX_RANK + 8) * 2);
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
         if (e != cudaSuccess) return (int)e;
     }
-    TvbLaunch at(grid, dim3(THREADS), shared, stream, pdl);
+    TvbLaunch at(grid, dim3(THREADS), shared, stream, pdl, cluster);
     const cudaError_t e = cudaLaunchKernelEx(&at.config, kernel, s);
     return e == cudaSuccess ? tvb_last_error() : (int)e;
 }
 
-}  // namespace
-
-extern "C" int tvb_adapters_max_rank() { return MAX_RANK; }
-
-// float32 of scratch: the pieces of u
-extern "C" long long tvb_adapters_scratch(int m, int k, int rank, int dtype) {
-    return m <= 0 ? 0 : (long long)shrink_splits(m, k, rank, dtype == TVB_F32) * m * rank;
+template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int pdl, cudaStream_t s) {
+    const dim3 grid(a.splits * chunks, ceil_div(a.m, 64), min(2, a.adapters));
+    return wide ? launch(shrink_many_kernel<RANKS, true>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a)
+                : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-extern "C" int tvb_adapters_shrink(const void* x, long long ldx, const void* down, const int* ids, float* part, int m, int k, int rank,
-                                   int adapters, int dtype, int pdl, void* stream) {
+template <int MT, typename Y> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
+    const dim3 grid(ceil_div(a.n, 128), ceil_div(a.m, 16 * MT), side_by_side);
+    return wide ? launch(expand_kernel<MT, Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<MT, Y, false>, grid, 0, 0, pdl, s, a);
+}
+
+}  // namespace
+
+// bytes of scratch: u
+extern "C" long long tvb_adapters_scratch(int m, int rank, int dtype) {
+    return m <= 0 ? 0 : (long long)m * (dtype == TVB_F32 ? rank * 4 : ceil_div(rank, 16) * 16 * 4);
+}
+
+extern "C" int tvb_adapters_shrink(const void* x, long long ldx, const void* down, const int* ids, const float* scales, void* u, int m,
+                                   int k, int rank, int adapters, int dtype, int pdl, void* stream) {
     if (m <= 0 || adapters <= 0) return 0;
-    if (k <= 0 || rank <= 0 || rank > MAX_RANK) return TVB_BAD_ARGUMENT;
+    if (k <= 0 || rank <= 0 || rank > MAX_RANK || ceil_div(m, 64) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    const int splits = shrink_splits(m, k, rank, dtype == TVB_F32);
     if (dtype == TVB_F32) {
         const bool wide = k % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)down) & 15);
-        const int per = ceil_div(ceil_div(k, splits), 4) * 4;
-        const Shrink32 a{(const float*)x, ldx, (const float*)down, ids, part, m, k, rank, adapters, splits, per};
-        const long long ctas = (long long)m * splits * ceil_div(rank, 4 * WARPS);
+        // pieces of at least 512 k, and not more CTAs than eight an SM
+        const int chunks = ceil_div(rank, 4 * WARPS);
+        int splits = 1;
+        while (splits < MAX_SPLITS && k / splits >= 1024 && (long long)m * chunks * splits < 8 * 148) splits *= 2;
+        const long long ctas = (long long)m * splits * chunks;
         if (ctas > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
+        const Shrink32 a{(const float*)x, ldx, (const float*)down, ids, scales, (float*)u, m, k, rank, adapters, splits,
+                         ceil_div(ceil_div(k, splits), 4) * 4};
         const dim3 grid((unsigned)ctas);
-        return wide ? launch(shrink_f32_kernel<4>, grid, 0, pdl, s, a) : launch(shrink_f32_kernel<1>, grid, 0, pdl, s, a);
+        return wide ? launch(shrink_f32_kernel<4>, grid, 0, splits, pdl, s, a) : launch(shrink_f32_kernel<1>, grid, 0, splits, pdl, s, a);
     }
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const bool wide = k % 8 == 0 && ldx % 8 == 0 && !(((uintptr_t)x | (uintptr_t)down) & 15);
-    const Shrink a{(const bf16*)x, ldx, (const bf16*)down, ids, part, m, k, rank, adapters, splits, ceil_div(ceil_div(k, 32), splits)};
+    Shrink a{(const bf16*)x, ldx, (const bf16*)down, ids, scales, (bf16*)u, m, k, rank, adapters, 1, 0};
     if (m <= FEW_ROWS) {
-        const dim3 grid(splits * ceil_div(rank, 16), ceil_div(m, 16), min(min(16, m), adapters));
-        return wide ? launch(shrink_kernel<2, false, true>, grid, 0, pdl, s, a) : launch(shrink_kernel<2, false, false>, grid, 0, pdl, s, a);
+        // a warp keeps a block of 32 k at least
+        while (a.splits < MAX_SPLITS && a.splits * 2 * WARPS <= ceil_div(k, 32)) a.splits *= 2;
+        a.per_split = ceil_div(ceil_div(k, 32), a.splits);
+        const dim3 grid(a.splits * ceil_div(rank, 16), ceil_div(m, 16), min(min(16, m), adapters));
+        return wide ? launch(shrink_few_kernel<true>, grid, 0, a.splits, pdl, s, a) : launch(shrink_few_kernel<false>, grid, 0, a.splits, pdl, s, a);
     }
-    if (ceil_div(m, 64) > 65535) return TVB_BAD_ARGUMENT;
-    if (rank <= 16) {
-        const dim3 grid(splits, ceil_div(m, 64));
-        return wide ? launch(shrink_kernel<2, true, true>, grid, 0, pdl, s, a) : launch(shrink_kernel<2, true, false>, grid, 0, pdl, s, a);
-    }
-    const dim3 grid(splits * ceil_div(rank, 64), ceil_div(m, 64));
-    return wide ? launch(shrink_kernel<8, true, true>, grid, 0, pdl, s, a) : launch(shrink_kernel<8, true, false>, grid, 0, pdl, s, a);
+    // as many pieces of k as give every SM two CTAs
+    const int chunks = rank <= 16 ? 1 : ceil_div(rank, 64), stages = ceil_div(k, STAGE_K);
+    while (a.splits < MAX_SPLITS && a.splits * 4 <= stages && ceil_div(m, 64) * chunks * a.splits < 2 * 148) a.splits *= 2;
+    a.per_split = ceil_div(stages, a.splits);
+    return rank <= 16 ? launch_many<16>(a, chunks, wide, pdl, s) : launch_many<64>(a, chunks, wide, pdl, s);
 }
 
 // dtype: of x, A and B; y_dtype: of y (float32 with either, bfloat16 with bfloat16)
-extern "C" int tvb_adapters_expand(const float* part, const void* up, const int* ids, const float* scales, void* y, long long ldy, int m,
-                                   int n, int k, int rank, int adapters, int dtype, int y_dtype, int pdl, void* stream) {
+extern "C" int tvb_adapters_expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank,
+                                   int adapters, int dtype, int y_dtype, int pdl, void* stream) {
     if (m <= 0 || n <= 0 || adapters <= 0) return 0;
-    if (rank <= 0 || rank > MAX_RANK) return TVB_BAD_ARGUMENT;
+    if (rank <= 0 || rank > MAX_RANK || ceil_div(m, 16) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    const Expand a{part, up, ids, scales, y, ldy, m, n, rank, adapters, shrink_splits(m, k, rank, dtype == TVB_F32)};
-    if (ceil_div(m, 16) > 65535) return TVB_BAD_ARGUMENT;
+    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters};
     if (dtype == TVB_F32) {
         if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
         const dim3 grid(ceil_div(n, THREADS), ceil_div(m, 16));
-        const size_t shared = 16 * (size_t)((rank + 3) / 4 * 4) * 4;
-        return rank % 4 == 0 && !((uintptr_t)up & 15) ? launch(expand_f32_kernel<4>, grid, shared, pdl, s, a)
-                                                     : launch(expand_f32_kernel<1>, grid, shared, pdl, s, a);
+        const size_t shared = 16 * (size_t)rank * 4;
+        return rank % 4 == 0 && !((uintptr_t)up & 15) ? launch(expand_f32_kernel<4>, grid, shared, 0, pdl, s, a)
+                                                     : launch(expand_f32_kernel<1>, grid, shared, 0, pdl, s, a);
     }
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const int size = y_dtype == TVB_F32 ? 4 : 2;
     const bool wide = rank % 4 == 0 && !((uintptr_t)up & 7) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
     const bool few = m <= FEW_ROWS;
-    const int rows = few ? 16 : 64;
-    const dim3 grid(ceil_div(n, 128), ceil_div(m, rows));
-    const size_t shared = 2 * (size_t)rows * ((rank + 15) / 16 * 16 + 8) * 2;
-    if (y_dtype == TVB_F32) {
-        if (few) return wide ? launch(expand_kernel<1, float, true>, grid, shared, pdl, s, a) : launch(expand_kernel<1, float, false>, grid, shared, pdl, s, a);
-        return wide ? launch(expand_kernel<4, float, true>, grid, shared, pdl, s, a) : launch(expand_kernel<4, float, false>, grid, shared, pdl, s, a);
-    }
+    const int side_by_side = few ? min(min(16, m), adapters) : 1;
+    if (y_dtype == TVB_F32)
+        return few ? launch_expand<1, float>(a, wide, side_by_side, pdl, s) : launch_expand<4, float>(a, wide, side_by_side, pdl, s);
     if (y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    if (few) return wide ? launch(expand_kernel<1, bf16, true>, grid, shared, pdl, s, a) : launch(expand_kernel<1, bf16, false>, grid, shared, pdl, s, a);
-    return wide ? launch(expand_kernel<4, bf16, true>, grid, shared, pdl, s, a) : launch(expand_kernel<4, bf16, false>, grid, shared, pdl, s, a);
+    return few ? launch_expand<1, bf16>(a, wide, side_by_side, pdl, s) : launch_expand<4, bf16>(a, wide, side_by_side, pdl, s);
 }

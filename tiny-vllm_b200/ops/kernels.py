@@ -2096,27 +2096,27 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
 ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
 
 
-def adapters_shrink(x: torch.Tensor, down: torch.Tensor, ids: torch.Tensor) -> torch.Tensor:
-    """The first half of :func:`tinyvllm_b200.ops.linear_adapted`: pieces of u = x . A^T (float32), for
-    :func:`adapters_expand`.  Arguments as checked there."""
+def adapters_shrink(x: torch.Tensor, down: torch.Tensor, ids: torch.Tensor, scales: torch.Tensor | None) -> torch.Tensor:
+    """The first half of :func:`tinyvllm_b200.ops.linear_adapted`: u = scale * x . A^T of every row, as
+    :func:`adapters_expand` reads it.  Arguments as checked there."""
     m, k = x.shape
-    adapters, rank = down.shape[0], down.shape[1]
+    adapters, rank, _ = down.shape
     tag = dtype_tag(x.dtype)
-    part = torch.empty(_fn("adapters", "tvb_adapters_scratch", [c_int, c_int, c_int, c_int], c_longlong)(m, k, rank, tag),
-                       dtype=torch.float32, device=x.device)
-    fn = _fn("adapters", "tvb_adapters_shrink", [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p])
-    _check(fn(x.data_ptr(), x.stride(0), down.data_ptr(), ids.data_ptr(), part.data_ptr(), m, k, rank, adapters, tag,
+    u = torch.empty(_fn("adapters", "tvb_adapters_scratch", [c_int, c_int, c_int], c_longlong)(m, rank, tag),
+                    dtype=torch.uint8, device=x.device)
+    fn = _fn("adapters", "tvb_adapters_shrink",
+             [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p])
+    _check(fn(x.data_ptr(), x.stride(0), down.data_ptr(), ids.data_ptr(), _ptr(scales), u.data_ptr(), m, k, rank, adapters, tag,
               _pdl("gemm"), _stream()), "adapters_shrink")
-    return part
+    return u
 
 
-def adapters_expand(part: torch.Tensor, up: torch.Tensor, ids: torch.Tensor, scales: torch.Tensor | None, y: torch.Tensor,
-                    k: int) -> None:
-    """The second half: y[t] += scale * u[t] . B^T in place, rounded once more to the type of y."""
+def adapters_expand(u: torch.Tensor, up: torch.Tensor, ids: torch.Tensor, y: torch.Tensor) -> None:
+    """The second half: y[t] += u[t] . B^T in place, rounded once more to the type of y."""
     (m, n), (adapters, _, rank) = y.shape, up.shape
     fn = _fn("adapters", "tvb_adapters_expand",
-             [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong] + [c_int] * 8 + [c_void_p])
-    _check(fn(part.data_ptr(), up.data_ptr(), ids.data_ptr(), _ptr(scales), y.data_ptr(), y.stride(0), m, n, k, rank, adapters,
+             [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong] + [c_int] * 7 + [c_void_p])
+    _check(fn(u.data_ptr(), up.data_ptr(), ids.data_ptr(), y.data_ptr(), y.stride(0), m, n, rank, adapters,
               dtype_tag(up.dtype), dtype_tag(y.dtype), _pdl("gemm"), _stream()), "adapters_expand")
 
 

@@ -99,9 +99,9 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     if m == 0 or n == 0:
         return torch.empty((m, n), dtype=out_dtype, device=x.device) if out is None else out
     # the short product first: the projection's kernel may then ask for its weight while that ends
-    part = kernels.adapters_shrink(x, down, ids)
+    u = kernels.adapters_shrink(x, down, ids, scales)
     y = linear(x, weight, out_dtype=out_dtype, out=out, weight_constant=weight_constant)
-    kernels.adapters_expand(part, up, ids, scales, y, k)
+    kernels.adapters_expand(u, up, ids, y)
     return y
 
 
