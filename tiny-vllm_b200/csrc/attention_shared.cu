@@ -4,22 +4,30 @@
 // head) instead of once a token.
 //
 // Softmax over a union of key ranges from the ranges' own results: a range gives its maximum m, l = sum exp(s - m) and
-// O = sum exp(s - m) v, and ranges join as l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).  So one launch takes pieces of
-// the shared keys (a tile of query rows each) and pieces of what every token has behind them (its own query heads), all
-// side by side, and leaves their m, l and O in float32 scratch; a second joins every token's pieces in their order.
+// O = sum exp(s - m) v, and ranges join as l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).  Two launches:
+//   attend_shared   pieces of the shared keys, a tile of query rows each; m, l and O go to float32 scratch;
+//   attend_own      what every token has behind them, a token's query heads of one kv head a cluster of CTAs that have a piece
+//                   of the keys each; they meet in distributed shared memory, join the shared pieces and store the result.
+// The second does not need the first before its end: launched programmatically it runs beside it (every CTA of the first
+// waits for the kernel before, so what that wrote is there for both) and waits for it before it reads the scratch.
 //
 // bfloat16: mma.sync m16n8k16 over tiles of 64 keys that cp.async brings two deep; a warp of a shared piece has 16 query
 // rows and every key, the warps of a token's own piece share the keys of a tile among them.  P is rounded to bfloat16 for
-// the second product, the denominator sums what was not rounded.  float32: the float32 cores, tiles of 32 keys.
+// the second product, the denominator sums what was not rounded.  float32: the float32 cores.
 //
 // Bound by reading keys and values while a group has few query rows, by the tensor cores once it has many.
+#include <cooperative_groups.h>
+
 #include "common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int KEYS = 64;                        // keys of a bfloat16 tile
 constexpr int KEYS32 = 32;                      // keys of a float32 tile
+constexpr int MAX_SHARED_PIECES = 64, MAX_OWN_PIECES = 8;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Attend {
@@ -32,12 +40,12 @@ struct Attend {
     const int* positions;                       // [tokens]
     const int* group_starts;                    // [groups + 1]
     const int* shared_lens;                     // [groups]
-    float* part_o;                              // [tokens, q heads, pieces, D]
-    float* part_ml;                             // [tokens, q heads, pieces, 2]
+    float* part_o;                              // [tokens, q heads, shared pieces, D]
+    float* part_ml;                             // [tokens, q heads, shared pieces, 2]
     void* out;
     int64_t out_stride;
     int tokens, rows, width, groups, pages, page_size, num_q, num_kv;
-    int shared_pieces, own_pieces, shared_items, own_tiles;
+    int shared_pieces, own_pieces, own_tiles;   // shared_pieces 0: every token reads all of its keys by itself
     float scale_log2;
 };
 
@@ -46,27 +54,42 @@ struct Range { int first, end; };
 // piece c of n keys in up to `pieces`: whole tiles of 64
 __device__ __forceinline__ int piece_keys(int n, int pieces) { return max(KEYS, ((n + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS); }
 
+// (plain loads may be served by an L1 that a kernel before filled: attend_own starts without waiting)
 __device__ __forceinline__ int row_of(const Attend& a, int token) {
-    const int row = a.token_row[token];
-    return (unsigned)row < (unsigned)a.rows && a.positions[token] >= 0 ? row : -1;
+    const int row = __ldcg(a.token_row + token);
+    return (unsigned)row < (unsigned)a.rows && __ldcg(a.positions + token) >= 0 ? row : -1;
 }
 // keys a token reads: its position's and those before it, as far as its table goes
 __device__ __forceinline__ int keys_of(const Attend& a, int token) {
-    return (int)min((int64_t)a.positions[token] + 1, (int64_t)a.width * a.page_size);
+    return (int)min((int64_t)__ldcg(a.positions + token) + 1, (int64_t)a.width * a.page_size);
 }
 __device__ __forceinline__ int shared_of_group(const Attend& a, int group) {
-    return (int)min((int64_t)max(a.shared_lens[group], 0), (int64_t)a.width * a.page_size);
+    return (int)min((int64_t)max(__ldcg(a.shared_lens + group), 0), (int64_t)a.width * a.page_size);
 }
-// the shared keys of the token's group, if it reads all of them (else it reads what it has by itself)
-__device__ __forceinline__ int shared_of(const Attend& a, int token) {
-    int lo = 0, hi = a.groups;                  // the last group that starts at or before the token
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (a.group_starts[mid] <= token) lo = mid; else hi = mid - 1;
-    }
-    if (lo >= a.groups || a.group_starts[lo] > token) return 0;
-    const int shared = shared_of_group(a, lo);
-    return keys_of(a, token) >= shared ? shared : 0;
+// What a token reads: the row of its table (-1: it is none), its keys, and how many of them its group reads for it (those it
+// shares if it reads them all, else none).  A whole warp asks, 32 groups at a time, all loads side by side.
+struct Facts { int row, keys, shared; };
+__device__ __forceinline__ Facts facts_of(const Attend& a, int token) {
+    const int lane = threadIdx.x & 31;
+    Facts f{__ldcg(a.token_row + token), __ldcg(a.positions + token), 0};
+    if (a.shared_pieces > 0)
+        for (int g0 = 0; g0 < a.groups; g0 += 32) {
+            int start = 0x7fffffff, end = 0, shared = 0;
+            if (g0 + lane < a.groups) {
+                start = __ldcg(a.group_starts + g0 + lane);
+                end = __ldcg(a.group_starts + g0 + lane + 1);
+                shared = shared_of_group(a, g0 + lane);
+            }
+            const uint32_t found = __ballot_sync(0xffffffffu, start <= token && token < end);
+            if (found) {
+                f.shared = __shfl_sync(0xffffffffu, shared, __ffs(found) - 1);
+                break;
+            }
+        }
+    if ((unsigned)f.row >= (unsigned)a.rows || f.keys < 0) f.row = -1;
+    f.keys = (int)min((int64_t)f.keys + 1, (int64_t)a.width * a.page_size);
+    if (f.keys < f.shared) f.shared = 0;
+    return f;
 }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -88,77 +111,78 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, const bf16* p) {
 struct Piece {
     Range range;
     const int* table;
-    int kv_head, slot;                          // slot: where the piece's results go among the token's
+    int kv_head, slot, keys;                    // slot: which of the shared pieces it is; keys: the group's shared ones
     int token0, rows, row0;                     // row r: token token0 + (row0 + r) / heads, head (row0 + r) % heads
 };
 
-// Which piece this CTA has; false: none.  TILE: query rows of a shared piece, OWN: of a token's own.
-template <int TILE, int OWN>
-__device__ __forceinline__ bool find_piece(const Attend& a, Piece& p, bool& shared) {
-    const int heads = a.num_q / a.num_kv;
+// The piece of the shared keys that this CTA has: `tile` query rows; false: none.
+__device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows, Piece& p) {
+    const int heads = a.num_q / a.num_kv, lane = threadIdx.x & 31;
     int item = blockIdx.x;
-    shared = item < a.shared_items;
-    if (shared) {
-        const int piece = item % a.shared_pieces;
-        item /= a.shared_pieces;
-        p.kv_head = item % a.num_kv;
-        int tile = item / a.num_kv;
-        // the group that has the tile: 32 groups at a time
-        const int lane = threadIdx.x & 31;
-        for (int g0 = 0; g0 < a.groups; g0 += 32) {
-            int start = 0, count = 0;
-            if (g0 + lane < a.groups) {
-                start = min(max(a.group_starts[g0 + lane], 0), a.tokens);
-                const int end = min(max(a.group_starts[g0 + lane + 1], start), a.tokens);
-                count = shared_of_group(a, g0 + lane) > 0 ? ((end - start) * heads + TILE - 1) / TILE : 0;
-            }
-            int upto = count;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, upto, d);
-                if (lane >= d) upto += other;
-            }
-            const uint32_t past = __ballot_sync(0xffffffffu, upto > tile);
-            if (past == 0) { tile -= __shfl_sync(0xffffffffu, upto, 31); continue; }
-            const int at = __ffs(past) - 1, group = g0 + at;
-            tile -= __shfl_sync(0xffffffffu, upto - count, at);
-            start = __shfl_sync(0xffffffffu, start, at);
-            const int end = min(max(a.group_starts[group + 1], start), a.tokens);
-            const int n = shared_of_group(a, group), per = piece_keys(n, a.shared_pieces);
-            p.range = Range{piece * per, min(n, (piece + 1) * per)};
-            if (p.range.first >= n) return false;
-            // the table of the first token that reads all of the shared keys
-            int row = -1;
-            for (int token = start; token < end && row < 0; ++token) {
-                row = row_of(a, token);
-                if (row >= 0 && keys_of(a, token) < n) row = -1;
-            }
-            if (row < 0) return false;
-            p.table = a.tables + (int64_t)row * a.width;
-            p.token0 = start;
-            p.row0 = tile * TILE;
-            p.rows = min(TILE, (end - start) * heads - p.row0);
-            p.slot = piece;
-            return true;
+    const int piece = item % a.shared_pieces;
+    item /= a.shared_pieces;
+    p.kv_head = item % a.num_kv;
+    int tile = item / a.num_kv;
+    // the group that has the tile: 32 groups at a time
+    for (int g0 = 0; g0 < a.groups; g0 += 32) {
+        int start = 0, count = 0;
+        if (g0 + lane < a.groups) {
+            start = min(max(__ldcg(a.group_starts + g0 + lane), 0), a.tokens);
+            const int end = min(max(__ldcg(a.group_starts + g0 + lane + 1), start), a.tokens);
+            count = shared_of_group(a, g0 + lane) > 0 ? ((end - start) * heads + tile_rows - 1) / tile_rows : 0;
         }
-        return false;
+        int upto = count;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += other;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, upto > tile);
+        if (past == 0) { tile -= __shfl_sync(0xffffffffu, upto, 31); continue; }
+        const int at = __ffs(past) - 1, group = g0 + at;
+        tile -= __shfl_sync(0xffffffffu, upto - count, at);
+        start = __shfl_sync(0xffffffffu, start, at);
+        const int end = min(max(__ldcg(a.group_starts + group + 1), start), a.tokens);
+        const int n = shared_of_group(a, group), per = piece_keys(n, a.shared_pieces);
+        p.range = Range{piece * per, min(n, (piece + 1) * per)};
+        if (p.range.first >= n) return false;
+        // the table of the first token that reads all of the shared keys
+        int row = -1;
+        for (int token = start; token < end && row < 0; token += 32) {
+            const int mine = token + lane < end ? row_of(a, token + lane) : -1;
+            const uint32_t reads = __ballot_sync(0xffffffffu, mine >= 0 && keys_of(a, token + lane) >= n);
+            if (reads) row = __shfl_sync(0xffffffffu, mine, __ffs(reads) - 1);
+        }
+        if (row < 0) return false;
+        p.keys = n;
+        p.table = a.tables + (int64_t)row * a.width;
+        p.token0 = start;
+        p.row0 = tile * tile_rows;
+        p.rows = min(tile_rows, (end - start) * heads - p.row0);
+        p.slot = piece;
+        return true;
     }
-    item -= a.shared_items;
+    return false;
+}
+
+// The piece of a token's own keys that this CTA of its cluster has (it may be empty), up to `tile` of its query heads, and
+// how many keys the token reads with its group; false: the token is padding.
+__device__ __forceinline__ bool find_own_piece(const Attend& a, int tile_rows, Piece& p, int& shared) {
+    int item = blockIdx.x;
     const int piece = item % a.own_pieces;
     item /= a.own_pieces;
     const int tile = item % a.own_tiles;
     item /= a.own_tiles;
     p.kv_head = item % a.num_kv;
     p.token0 = item / a.num_kv;
-    const int row = row_of(a, p.token0);
-    if (row < 0) return false;
-    const int first = shared_of(a, p.token0), n = keys_of(a, p.token0) - first, per = piece_keys(n, a.own_pieces);
-    p.range = Range{first + piece * per, first + min(n, (piece + 1) * per)};
-    if (piece * per >= n) return false;
-    p.table = a.tables + (int64_t)row * a.width;
-    p.row0 = tile * OWN;
-    p.rows = min(OWN, heads - p.row0);
-    p.slot = a.shared_pieces + piece;
+    p.row0 = tile * tile_rows;
+    p.rows = min(tile_rows, a.num_q / a.num_kv - p.row0);
+    const Facts f = facts_of(a, p.token0);
+    if (f.row < 0) return false;
+    shared = f.shared;
+    const int n = f.keys - shared, per = piece_keys(n, a.own_pieces);
+    p.range = Range{shared + min(n, piece * per), shared + min(n, (piece + 1) * per)};
+    p.table = a.tables + (int64_t)f.row * a.width;
     return true;
 }
 __device__ __forceinline__ int token_of(const Attend& a, const Piece& p, int r, int& head) {
@@ -167,48 +191,193 @@ __device__ __forceinline__ int token_of(const Attend& a, const Piece& p, int r, 
     return p.token0 + at / heads;
 }
 __device__ __forceinline__ int64_t part_of(const Attend& a, int token, int head, int slot) {
-    return ((int64_t)token * a.num_q + head) * (a.shared_pieces + a.own_pieces) + slot;
+    return ((int64_t)token * a.num_q + head) * a.shared_pieces + slot;
 }
-// a row of a shared tile that takes part: the token is one, and reads all of the shared keys
-__device__ __forceinline__ bool takes_part(const Attend& a, bool shared, int token) {
-    return !shared || (row_of(a, token) >= 0 && shared_of(a, token) > 0);
+// a token that takes part in its group's pieces: it is one, and reads all of the shared keys
+__device__ __forceinline__ bool takes_part(const Attend& a, const Piece& p, int token) {
+    const int row = __ldcg(a.token_row + token), position = __ldcg(a.positions + token);
+    return (unsigned)row < (unsigned)a.rows && position >= p.keys - 1;          // (no table is shorter than the shared keys)
 }
 // place of a key's row in the cache, in rows of D; -1: no such page
-__device__ __forceinline__ int64_t cache_row(const Attend& a, const Piece& p, int key) {
-    const int page = p.table[key / a.page_size];
+__device__ __forceinline__ int64_t row_in(const Attend& a, const Piece& p, int page, int key) {
     return (unsigned)page < (unsigned)a.pages ? ((int64_t)page * a.num_kv + p.kv_head) * a.page_size + key % a.page_size : -1;
+}
+__device__ __forceinline__ int64_t cache_row(const Attend& a, const Piece& p, int key) {
+    return row_in(a, p, __ldcg(p.table + key / a.page_size), key);
+}
+
+// ----------------------------------------------------------- joining the pieces
+// What a CTA of attend_own ends with, in shared memory: rows' O [OWN][D] and (m, l) of its piece.
+template <int D, int OWN> struct Ends {
+    static constexpr int PARTS = MAX_SHARED_PIECES + MAX_OWN_PIECES;
+    static constexpr int WARP_PITCH = D + 4;
+    static constexpr int FLOATS = WARPS * OWN * (WARP_PITCH + 2) + OWN * (D + 2) + 2 * OWN * PARTS;
+    float* warp_o;                              // [WARPS][OWN][WARP_PITCH], the warps' shares
+    float* warp_ml;                             // [WARPS][OWN][2]
+    float* o;                                   // [OWN][D], the CTA's
+    float* ml;                                  // [OWN][2]
+    float* weights;                             // [OWN][PARTS][2]: every part's m and l, then its factor in the first place
+    __device__ __forceinline__ explicit Ends(float* at) {
+        warp_o = at;
+        warp_ml = warp_o + WARPS * OWN * WARP_PITCH;
+        o = warp_ml + WARPS * OWN * 2;
+        ml = o + OWN * D;
+        weights = ml + OWN * 2;
+    }
+};
+
+// Every warp has stored its share (behind a barrier): the CTA's own, the cluster's, the shared pieces', the result.
+template <typename T, int D, int OWN>
+__device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int shared, const Ends<D, OWN>& e) {
+    using E = Ends<D, OWN>;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, own = a.own_pieces, rank = own > 1 ? (int)cluster.block_rank() : 0;
+    for (int i = tid; i < p.rows * (D / 4); i += THREADS) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, e.warp_ml[2 * (w * OWN + r)]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float4 sum = make_float4(0, 0, 0, 0);
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2f(e.warp_ml[2 * (w * OWN + r)] - ref);
+            const float4 v = *reinterpret_cast<const float4*>(e.warp_o + (w * OWN + r) * E::WARP_PITCH + d);
+            sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
+            total += f * e.warp_ml[2 * (w * OWN + r) + 1];
+        }
+        *reinterpret_cast<float4*>(e.o + r * D + d) = sum;
+        if (d == 0) { e.ml[2 * r] = top; e.ml[2 * r + 1] = total; }
+    }
+    if (own > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
+    const int used = shared > 0 ? (shared + piece_keys(shared, a.shared_pieces) - 1) / piece_keys(shared, a.shared_pieces) : 0;
+    if (a.shared_pieces > 0) pdl_wait();        // the shared pieces are there
+    const int parts = used + own;
+    for (int i = tid; i < p.rows * parts; i += THREADS) {
+        const int r = i / parts, part = i % parts;
+        float2 v;
+        if (part < used) {
+            int head;
+            const int token = token_of(a, p, r, head);
+            v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + part_of(a, token, head, part));
+        } else {
+            const float* ml = own > 1 ? cluster.map_shared_rank(e.ml, part - used) : e.ml;
+            v = make_float2(ml[2 * r], ml[2 * r + 1]);
+        }
+        e.weights[2 * (r * E::PARTS + part)] = v.x;
+        e.weights[2 * (r * E::PARTS + part) + 1] = v.y;
+    }
+    __syncthreads();
+    for (int r = tid >> 5; r < p.rows; r += WARPS) {                            // a warp a row
+        const int lane = tid & 31;
+        float top = -INFINITY;
+        for (int part = lane; part < parts; part += 32) top = fmaxf(top, e.weights[2 * (r * E::PARTS + part)]);
+        top = warp_max(top);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        for (int part = lane; part < parts; part += 32) {
+            float* at = e.weights + 2 * (r * E::PARTS + part);
+            at[0] = exp2f(at[0] - ref);
+            total = fmaf(at[0], at[1], total);
+        }
+        total = warp_sum(total);
+        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;              // no key is seen: zeros
+        for (int part = lane; part < parts; part += 32) e.weights[2 * (r * E::PARTS + part)] *= inverse;
+    }
+    __syncthreads();
+    for (int i = tid + THREADS * rank; i < p.rows * (D / 4); i += THREADS * own) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        int head;
+        const int token = token_of(a, p, r, head);
+        const float* from = a.part_o + part_of(a, token, head, 0) * D + d;
+        const float* weight = e.weights + 2 * r * E::PARTS;
+        float4 sum = make_float4(0, 0, 0, 0);
+        auto add = [&](float w, const float4& v) {
+            sum.x = fmaf(w, v.x, sum.x); sum.y = fmaf(w, v.y, sum.y); sum.z = fmaf(w, v.z, sum.z); sum.w = fmaf(w, v.w, sum.w);
+        };
+        int part = 0;
+        for (; part + 4 <= used; part += 4) {
+            float4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)(part + j) * D));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) add(weight[2 * (part + j)], v[j]);
+        }
+        for (; part < used; ++part) add(weight[2 * part], __ldcg(reinterpret_cast<const float4*>(from + (int64_t)part * D)));
+        for (int c = 0; c < own; ++c) {
+            const float* o = own > 1 ? cluster.map_shared_rank(e.o, c) : e.o;
+            add(weight[2 * (used + c)], *reinterpret_cast<const float4*>(o + r * D + d));
+        }
+        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + d;
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[j] = from_float<T>(v[j]);
+    }
+    if (own > 1) {                              // the others' shared memory is read until here
+        cluster_arrive();
+        cluster_wait();
+    }
+}
+
+// a token that is none: zeros
+template <typename T, int D> __device__ __forceinline__ void store_zeros(const Attend& a, const Piece& p) {
+    if (blockIdx.x % a.own_pieces != 0) return;
+    for (int i = threadIdx.x; i < p.rows * D; i += THREADS) {
+        int head;
+        const int token = token_of(a, p, i / D, head);
+        reinterpret_cast<T*>(a.out)[token * a.out_stride + head * D + i % D] = from_float<T>(0.0f);
+    }
+}
+
+// The kernels' waits (see the top).  attend_own waits at its start where there is no attend_shared before it, else before it
+// reads the shared pieces or ends.
+__device__ __forceinline__ void start_own(const Attend& a) {
+    if (a.shared_pieces == 0) pdl_wait();
+    pdl_launch_dependents();
 }
 
 // ------------------------------------------------------------------ bfloat16
 template <int D> struct Tiles {
     static constexpr int PITCH = D + 8;
     static constexpr int TILE = KEYS * PITCH;                                   // elements of a K or V tile
-    static constexpr int BYTES = (64 + 4 * KEYS) * PITCH * 2 + 3 * KEYS * 8 + 3 * 2 * 4;
+    static constexpr int bytes(int rows) { return (rows + 4 * KEYS) * PITCH * 2 + 3 * KEYS * 8 + 3 * 2 * 4 + 64; }
 };
 
 // SHARED: the tile's 64 query rows, 16 a warp, every warp over every key.  Else: up to 16 query rows, a warp over 16 keys of
 // every tile, the warps' results joined at the end.
 template <int D, bool SHARED>
-__device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, unsigned char* raw) {
+__device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, int shared, unsigned char* raw) {
     constexpr int PITCH = Tiles<D>::PITCH, ROWS = SHARED ? 64 : 16;
     constexpr int NK = SHARED ? KEYS : KEYS / WARPS;                            // keys of a tile that a warp has
     bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [ROWS][PITCH]
-    bf16* k_s = q_s + 64 * PITCH;                                               // [2][KEYS][PITCH]
+    bf16* k_s = q_s + ROWS * PITCH;                                              // [2][KEYS][PITCH]
     bf16* v_s = k_s + 2 * Tiles<D>::TILE;
     // of a tile's keys: the place of their rows (-1: none), and which there are.  Three tiles of them: one warp may look up
     // those of a tile while another still reads the bits of the one two before.
     int64_t* at_s = reinterpret_cast<int64_t*>(v_s + 2 * Tiles<D>::TILE);       // [3][KEYS]
     uint32_t* there_s = reinterpret_cast<uint32_t*>(at_s + 3 * KEYS);           // [3][2]
+    bool* takes_s = reinterpret_cast<bool*>(there_s + 6);                       // [ROWS] tokens that take part
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const bf16* keys = reinterpret_cast<const bf16*>(a.keys);
     const bf16* values = reinterpret_cast<const bf16*>(a.values);
     const int tiles = (p.range.end - p.range.first + KEYS - 1) / KEYS;
 
-    auto place = [&](int tile) {                                                // the first two warps
+    // (a page's number is asked for a tile before it is looked at)
+    auto page_of = [&](int tile) -> int {
+        const int key = p.range.first + tile * KEYS + tid;
+        return tid < KEYS && key < p.range.end ? __ldcg(p.table + key / a.page_size) : -1;
+    };
+    auto place = [&](int tile, int page) {                                      // the first two warps
         const int slot = tile % 3;
         if (tid < KEYS) {
             const int key = p.range.first + tile * KEYS + tid;
-            const int64_t at = key < p.range.end ? cache_row(a, p, key) : -1;
+            const int64_t at = key < p.range.end ? row_in(a, p, page, key) : -1;
             at_s[slot * KEYS + tid] = at;
             const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
             if (lane == 0) there_s[slot * 2 + warp] = there;
@@ -227,20 +396,28 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, un
         }
         cp_async_commit();
     };
-    place(0);
+    const int first_page = page_of(0);
+    int next_page = page_of(1);
+    if constexpr (SHARED) {
+        if (tid < ROWS) {
+            int head;
+            takes_s[tid] = tid < p.rows && takes_part(a, p, token_of(a, p, tid, head));
+        }
+    }
+#pragma unroll 4
     for (int i = tid; i < ROWS * (D / 8); i += THREADS) {
         const int r = i / (D / 8), word = i % (D / 8);
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < p.rows) {
             int head;
             const int token = token_of(a, p, r, head);
-            if (takes_part(a, SHARED, token))
-                v = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + token * a.q_stride + head * D + word * 8);
+            v = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + token * a.q_stride + head * D + word * 8));
         }
         *reinterpret_cast<uint4*>(q_s + r * PITCH + word * 8) = v;
     }
+    place(0, first_page);
     __syncthreads();
-    load(0);
+    if (tiles > 0) load(0);
     const bf16* q_rows = q_s + (SHARED ? warp * 16 : 0) * PITCH + (lane & 15) * PITCH + (lane >> 4) * 8;
     uint32_t q_frag[D <= 128 ? D / 16 : 1][4];
     if constexpr (D <= 128)
@@ -257,7 +434,10 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, un
 
     for (int tile = 0; tile < tiles; ++tile) {
         const int buffer = tile & 1;
-        if (tile + 1 < tiles) place(tile + 1);
+        if (tile + 1 < tiles) {
+            place(tile + 1, next_page);
+            next_page = page_of(tile + 2);
+        }
         cp_async_wait<0>();
         __syncthreads();                                                        // the tile is there; places of the next too
         if (tile + 1 < tiles) load(tile + 1);
@@ -342,10 +522,9 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, un
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = warp * 16 + g + 8 * h;
-            if (r >= p.rows) continue;
+            if (r >= p.rows || !takes_s[r]) continue;
             int head;
             const int token = token_of(a, p, r, head);
-            if (!takes_part(a, true, token)) continue;
             const int64_t part = part_of(a, token, head, p.slot);
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
@@ -353,83 +532,73 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, un
             if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[h], l[h]);
         }
     } else {
-        // the warps' results, over the tiles' memory: [warp][16][D + 4] and [warp][16][2]
-        constexpr int OP = D + 4;
-        float* o_w = reinterpret_cast<float*>(k_s);
-        float* ml_w = o_w + WARPS * 16 * OP;
-        static_assert(WARPS * 16 * (OP + 2) * 4 <= 4 * Tiles<D>::TILE * 2, "the warps' results lie over the tiles");
+        // the warps' shares lie over the tiles
+        using E = Ends<D, 16>;
+        static_assert(E::FLOATS * 4 <= 4 * Tiles<D>::TILE * 2, "room for what the CTA ends with");
+        const E e(reinterpret_cast<float*>(k_s));
         __syncthreads();
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = warp * 16 + g + 8 * h;
 #pragma unroll
             for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(o_w + r * OP + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-            if (t4 == 0) { ml_w[2 * r] = m[h]; ml_w[2 * r + 1] = l[h]; }
+                *reinterpret_cast<float2*>(e.warp_o + r * E::WARP_PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+            if (t4 == 0) { e.warp_ml[2 * r] = m[h]; e.warp_ml[2 * r + 1] = l[h]; }
         }
         __syncthreads();
-        for (int i = tid; i < p.rows * (D / 4); i += THREADS) {
-            const int r = i / (D / 4), d = i % (D / 4) * 4;
-            float top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml_w[2 * (w * 16 + r)]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-            float4 sum = make_float4(0, 0, 0, 0);
-            float total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = exp2_unit(ml_w[2 * (w * 16 + r)] - ref);
-                const float4 v = *reinterpret_cast<const float4*>(o_w + (w * 16 + r) * OP + d);
-                sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
-                total += f * ml_w[2 * (w * 16 + r) + 1];
-            }
-            int head;
-            const int token = token_of(a, p, r, head);
-            const int64_t part = part_of(a, token, head, p.slot);
-            *reinterpret_cast<float4*>(a.part_o + part * D + d) = sum;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, total);
-        }
+        join_pieces<bf16, D, 16>(a, p, shared, e);
     }
 }
 
-template <int D>
-__global__ void __launch_bounds__(THREADS) attend_bf16_kernel(Attend a) {
+template <int D> __global__ void __launch_bounds__(THREADS) attend_shared_bf16_kernel(Attend a) {
     extern __shared__ __align__(16) unsigned char raw[];
     pdl_wait();
     pdl_launch_dependents();
     Piece p;
-    bool shared;
-    if (!find_piece<64, 16>(a, p, shared)) return;                              // the whole CTA
-    if (shared) attend_piece<D, true>(a, p, raw);
-    else attend_piece<D, false>(a, p, raw);
+    if (find_shared_piece(a, 64, p)) attend_piece<D, true>(a, p, 0, raw);
+}
+
+template <int D> __global__ void __launch_bounds__(THREADS) attend_own_bf16_kernel(Attend a) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    start_own(a);
+    Piece p;
+    int shared = 0;
+    if (find_own_piece(a, 16, p, shared)) attend_piece<D, false>(a, p, shared, raw);
+    else {
+        store_zeros<bf16, D>(a, p);
+        if (a.shared_pieces > 0) pdl_wait();
+    }
 }
 
 // ------------------------------------------------------------------- float32
 // 16 query rows, four a warp: a lane has a key of the tile for the scores, D / 32 values of every row for the sums.
 template <int D>
-__global__ void __launch_bounds__(THREADS) attend_f32_kernel(Attend a) {
+__global__ void __launch_bounds__(THREADS) attend_shared_f32_kernel(Attend a) {
     constexpr int PITCH = D + 4, VALUES = D / 32;
     extern __shared__ __align__(16) float tiles_s[];
     float* k_s = tiles_s;                                                       // [KEYS32][PITCH]
     float* v_s = k_s + KEYS32 * PITCH;
     float* q_s = v_s + KEYS32 * PITCH;                                          // [16][D]
     __shared__ uint32_t there_s;
+    __shared__ bool takes_s[16];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     pdl_wait();
     pdl_launch_dependents();
     Piece p;
-    bool shared;
-    if (!find_piece<16, 16>(a, p, shared)) return;
+    if (!find_shared_piece(a, 16, p)) return;
     const float* keys = reinterpret_cast<const float*>(a.keys);
     const float* values = reinterpret_cast<const float*>(a.values);
+    if (tid < 16) {
+        int head;
+        takes_s[tid] = tid < p.rows && takes_part(a, p, token_of(a, p, tid, head));
+    }
     for (int i = tid; i < 16 * (D / 4); i += THREADS) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
         float4 v = make_float4(0, 0, 0, 0);
         if (r < p.rows) {
             int head;
             const int token = token_of(a, p, r, head);
-            if (takes_part(a, shared, token))
-                v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D + d);
+            v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D + d);
         }
         *reinterpret_cast<float4*>(q_s + r * D + d) = v;
     }
@@ -494,10 +663,9 @@ __global__ void __launch_bounds__(THREADS) attend_f32_kernel(Attend a) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         const float total = warp_sum(l[r]);
-        if (warp * 4 + r >= p.rows) continue;
+        if (warp * 4 + r >= p.rows || !takes_s[warp * 4 + r]) continue;
         int head;
         const int token = token_of(a, p, warp * 4 + r, head);
-        if (!takes_part(a, shared, token)) continue;
         const int64_t part = part_of(a, token, head, p.slot);
 #pragma unroll
         for (int e = 0; e < VALUES; ++e) a.part_o[part * D + e * 32 + lane] = o[r][e];
@@ -505,81 +673,140 @@ __global__ void __launch_bounds__(THREADS) attend_f32_kernel(Attend a) {
     }
 }
 
-// ----------------------------------------------------------- joining the pieces
-// a warp a (token, head)
-template <typename T, int D>
-__global__ void __launch_bounds__(THREADS) join_kernel(Attend a) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
-    pdl_wait();
-    pdl_launch_dependents();
-    const int token = (int)(at / a.num_q), head = (int)(at % a.num_q);
-    if (token >= a.tokens) return;
-    constexpr int VALUES = D / 32;
-    float sum[VALUES] = {}, total = 0.0f;
-    if (row_of(a, token) >= 0) {
-        const int first = shared_of(a, token), own = keys_of(a, token) - first;
-        const int shared_used = first > 0 ? (first + piece_keys(first, a.shared_pieces) - 1) / piece_keys(first, a.shared_pieces) : 0;
-        const int own_used = own > 0 ? (own + piece_keys(own, a.own_pieces) - 1) / piece_keys(own, a.own_pieces) : 0;
-        float top = -INFINITY;
-        const int64_t part = part_of(a, token, head, 0);
-        auto slot_of = [&](int i) { return i < shared_used ? i : a.shared_pieces + i - shared_used; };
-        for (int i = 0; i < shared_used + own_used; ++i) top = fmaxf(top, a.part_ml[(part + slot_of(i)) * 2]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-        for (int i = 0; i < shared_used + own_used; ++i) {
-            const int64_t from = part + slot_of(i);
-            const float f = exp2f(a.part_ml[from * 2] - ref);
-            total = fmaf(f, a.part_ml[from * 2 + 1], total);
+// Up to four query heads of a token: a warp takes every fourth key, a lane D / 32 neighbouring values of it.
+template <int D>
+__global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
+    constexpr int OWN = 4, V = D / 32, AHEAD = D <= 128 ? 4 : 2;                // keys of a warp in flight
+    using E = Ends<D, OWN>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    start_own(a);
+    Piece p;
+    int shared = 0;
+    if (!find_own_piece(a, OWN, p, shared)) {
+        store_zeros<float, D>(a, p);
+        if (a.shared_pieces > 0) pdl_wait();
+        return;
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const float* keys = reinterpret_cast<const float*>(a.keys);
+    const float* values = reinterpret_cast<const float*>(a.values);
+    auto load = [&](const float* from, float (&v)[V]) {
+        if constexpr (V == 2) {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(from + lane * V));
+            v[0] = f.x; v[1] = f.y;
+        } else {
 #pragma unroll
-            for (int e = 0; e < VALUES; ++e) sum[e] = fmaf(f, a.part_o[from * D + e * 32 + lane], sum[e]);
+            for (int i = 0; i < V; i += 4) {
+                const float4 f = __ldcg(reinterpret_cast<const float4*>(from + lane * V + i));
+                v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+            }
+        }
+    };
+    float q[OWN][V] = {}, o[OWN][V] = {}, m[OWN], l[OWN] = {};
+#pragma unroll
+    for (int r = 0; r < OWN; ++r) {
+        m[r] = -INFINITY;
+        if (r >= p.rows) continue;
+        int head;
+        const int token = token_of(a, p, r, head);
+        load(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D, q[r]);
+    }
+    for (int key0 = p.range.first + warp; key0 < p.range.end; key0 += AHEAD * WARPS) {
+        float k[AHEAD][V] = {}, v[AHEAD][V] = {};
+        bool there[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int key = key0 + i * WARPS;
+            const int64_t at = key < p.range.end ? cache_row(a, p, key) : -1;
+            there[i] = at >= 0;
+            if (there[i]) {
+                load(keys + at * D, k[i]);
+                load(values + at * D, v[i]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < OWN; ++r) {
+            if (r >= p.rows) continue;
+            float s[AHEAD], now = m[r];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                float dot = 0.0f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) dot = fmaf(q[r][e], k[i][e], dot);
+                s[i] = warp_sum(dot) * a.scale_log2;
+                if (!there[i]) s[i] = -INFINITY;
+                now = fmaxf(now, s[i]);
+            }
+            const float subtract = now == -INFINITY ? 0.0f : now, factor = exp2f(m[r] - subtract);
+            m[r] = now;
+            l[r] *= factor;
+#pragma unroll
+            for (int e = 0; e < V; ++e) o[r][e] *= factor;
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const float w = exp2f(s[i] - subtract);
+                l[r] += w;
+#pragma unroll
+                for (int e = 0; e < V; ++e) o[r][e] = fmaf(w, v[i][e], o[r][e]);
+            }
         }
     }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;                  // a token that is none, or sees no key: zeros
-    T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D;
+    const E e(reinterpret_cast<float*>(raw));
 #pragma unroll
-    for (int e = 0; e < VALUES; ++e) out[e * 32 + lane] = from_float<T>(sum[e] * inverse);
+    for (int r = 0; r < OWN; ++r) {
+        const int at = warp * OWN + r;
+#pragma unroll
+        for (int i = 0; i < V; ++i) e.warp_o[at * E::WARP_PITCH + lane * V + i] = o[r][i];
+        if (lane == 0) { e.warp_ml[2 * at] = m[r]; e.warp_ml[2 * at + 1] = l[r]; }
+    }
+    __syncthreads();
+    join_pieces<float, D, OWN>(a, p, shared, e);
 }
 
 // ------------------------------------------------------------------ host side
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
-struct Plan { long long shared_items, own_items; int shared_pieces, own_pieces, own_tiles; };
+struct Plan {
+    long long shared_items, own_items;
+    int shared_pieces, own_pieces, own_tiles;
+};
 
 // Into how many pieces the keys are cut: enough for about three CTAs an SM, none shorter than MIN_KEYS.
 Plan plan_of(int tokens, int groups, int num_q, int num_kv, int max_shared, int max_own, int dtype) {
     constexpr int MIN_KEYS = 128, CTAS = 3 * 148;
     const int heads = num_q / num_kv, tile = dtype == TVB_F32 ? 16 : 64;
     const long long tiles = groups > 0 && max_shared > 0 ? (long long)tokens * heads / tile + groups : 0;
-    auto pieces_of = [&](long long items, int keys) {
+    auto pieces_of = [&](long long items, int keys, int most) {
         const long long wanted = items > 0 ? ceil_div(CTAS, items) : 1;
-        return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1), MIN_KEYS)), 64ll));
+        return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1), MIN_KEYS)), (long long)most));
     };
     Plan p;
-    p.own_tiles = (heads + 15) / 16;
-    p.shared_pieces = tiles > 0 ? pieces_of(tiles * num_kv, max_shared) : 0;
-    p.own_pieces = pieces_of((long long)tokens * num_kv * p.own_tiles, max_own);
+    p.own_tiles = (int)ceil_div(heads, dtype == TVB_F32 ? 4 : 16);
+    p.shared_pieces = tiles > 0 ? pieces_of(tiles * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
+    p.own_pieces = pieces_of((long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
     p.shared_items = tiles * num_kv * p.shared_pieces;
     p.own_items = (long long)tokens * num_kv * p.own_tiles * p.own_pieces;
     return p;
 }
 
-template <typename K> int launch(K kernel, long long grid, size_t shared, int pdl, cudaStream_t stream, const Attend& a) {
+template <typename K> int launch(K kernel, long long grid, size_t shared, int pdl, int cluster, cudaStream_t stream, const Attend& a) {
     if (shared > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
         if (e != cudaSuccess) return (int)e;
     }
-    TvbLaunch at(dim3((unsigned)grid), dim3(THREADS), shared, stream, pdl);
+    TvbLaunch at(dim3((unsigned)grid), dim3(THREADS), shared, stream, pdl, cluster);
     const cudaError_t e = cudaLaunchKernelEx(&at.config, kernel, a);
     return e == cudaSuccess ? tvb_last_error() : (int)e;
 }
 
-template <int D> int launch_all(const Attend& a, long long items, int dtype, int pdl, cudaStream_t s) {
-    const int e = dtype == TVB_F32 ? launch(attend_f32_kernel<D>, items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, s, a)
-                                   : launch(attend_bf16_kernel<D>, items, Tiles<D>::BYTES, pdl, s, a);
-    if (e) return e;
-    const long long joins = ceil_div((long long)a.tokens * a.num_q, WARPS);
-    return dtype == TVB_F32 ? launch(join_kernel<float, D>, joins, 0, pdl, s, a) : launch(join_kernel<bf16, D>, joins, 0, pdl, s, a);
+template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int pdl, cudaStream_t s) {
+    const int cluster = p.own_pieces > 1 ? p.own_pieces : 0;
+    if (dtype == TVB_F32) {
+        const int e = p.shared_items == 0 ? 0 : launch(attend_shared_f32_kernel<D>, p.shared_items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, 0, s, a);
+        return e ? e : launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, cluster, s, a);
+    }
+    const int e = p.shared_items == 0 ? 0 : launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
+    return e ? e : launch(attend_own_bf16_kernel<D>, p.own_items, Tiles<D>::bytes(16), pdl, cluster, s, a);
 }
 
 }  // namespace
@@ -589,7 +816,12 @@ extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int nu
                                                   int dtype) {
     if (tokens <= 0 || num_kv <= 0) return 0;
     const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
-    return (long long)tokens * num_q * (p.shared_pieces + p.own_pieces) * (head_dim + 2);
+    return (long long)tokens * num_q * p.shared_pieces * (head_dim + 2);
+}
+
+// launches that a call takes
+extern "C" int tvb_attention_shared_launches(int tokens, int groups, int num_q, int num_kv, int max_shared, int max_own, int dtype) {
+    return tokens <= 0 || num_kv <= 0 ? 0 : plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype).shared_items > 0 ? 2 : 1;
 }
 
 extern "C" int tvb_attention_shared(const void* q, long long q_stride, const void* keys, const void* values, const int* tables, int rows,
@@ -602,15 +834,13 @@ extern "C" int tvb_attention_shared(const void* q, long long q_stride, const voi
         width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096)
         return TVB_BAD_ARGUMENT;
     const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
-    if (p.shared_items + p.own_items > 0x7fffffffLL || (long long)tokens * num_q > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
+    if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
     Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, scratch, nullptr, out, out_stride,
-             tokens, rows, width, p.shared_items > 0 ? groups : 0, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces,
-             (int)p.shared_items, p.own_tiles, scale * LOG2E};
-    a.part_ml = scratch + (long long)tokens * num_q * (p.shared_pieces + p.own_pieces) * head_dim;
+             tokens, rows, width, groups, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, scale * LOG2E};
+    a.part_ml = scratch + (long long)tokens * num_q * p.shared_pieces * head_dim;
     cudaStream_t s = (cudaStream_t)stream;
-    const long long items = p.shared_items + p.own_items;
-    if (head_dim == 64) return launch_all<64>(a, items, dtype, pdl, s);
-    if (head_dim == 128) return launch_all<128>(a, items, dtype, pdl, s);
-    if (head_dim == 256) return launch_all<256>(a, items, dtype, pdl, s);
+    if (head_dim == 64) return launch_all<64>(a, p, dtype, pdl, s);
+    if (head_dim == 128) return launch_all<128>(a, p, dtype, pdl, s);
+    if (head_dim == 256) return launch_all<256>(a, p, dtype, pdl, s);
     return TVB_BAD_ARGUMENT;
 }

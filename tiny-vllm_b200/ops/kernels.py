@@ -2181,7 +2181,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
               block_tables.shape[0], block_tables.shape[1], token_row.data_ptr(), positions.data_ptr(), group_starts.data_ptr(),
               shared_lens.data_ptr(), groups, scratch.data_ptr(), out.data_ptr(), out.stride(0), tokens, key_cache.shape[0],
               key_cache.shape[2], num_q, num_kv, head_dim, max_shared, max_own, scale, tag, _pdl("attention_shared"), _stream()),
-           "attention_shared", 2)
+           "attention_shared",
+           _fn("attention_shared", "tvb_attention_shared_launches", [c_int] * 7)(tokens, groups, num_q, num_kv, max_shared, max_own, tag))
     return out
 
 
