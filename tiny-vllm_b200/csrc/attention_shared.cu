@@ -51,8 +51,9 @@ struct Attend {
 
 struct Range { int first, end; };
 
-// piece c of n keys in up to `pieces`: whole tiles of 64
+// piece c of n keys in up to `pieces`: whole tiles of 64, of the shared keys whole blocks of 128
 __device__ __forceinline__ int piece_keys(int n, int pieces) { return max(KEYS, ((n + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS); }
+__device__ __forceinline__ int shared_piece_keys(int n, int pieces) { return max(2 * KEYS, ((n + pieces - 1) / pieces + 2 * KEYS - 1) / (2 * KEYS) * 2 * KEYS); }
 
 // (plain loads may be served by an L1 that a kernel before filled: attend_own starts without waiting)
 __device__ __forceinline__ int row_of(const Attend& a, int token) {
@@ -143,7 +144,7 @@ __device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows
         tile -= __shfl_sync(0xffffffffu, upto - count, at);
         start = __shfl_sync(0xffffffffu, start, at);
         const int end = min(max(__ldcg(a.group_starts + group + 1), start), a.tokens);
-        const int n = shared_of_group(a, group), per = piece_keys(n, a.shared_pieces);
+        const int n = shared_of_group(a, group), per = shared_piece_keys(n, a.shared_pieces);
         p.range = Range{piece * per, min(n, (piece + 1) * per)};
         if (p.range.first >= n) return false;
         // the table of the first token that reads all of the shared keys
@@ -256,7 +257,7 @@ __device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int
     } else {
         __syncthreads();
     }
-    const int used = shared > 0 ? (shared + piece_keys(shared, a.shared_pieces) - 1) / piece_keys(shared, a.shared_pieces) : 0;
+    const int per = shared > 0 ? shared_piece_keys(shared, a.shared_pieces) : 1, used = (shared + per - 1) / per;
     if (a.shared_pieces > 0) pdl_wait();        // the shared pieces are there
     const int parts = used + own;
     for (int i = tid; i < p.rows * parts; i += THREADS) {
@@ -763,27 +764,34 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
     join_pieces<float, D, OWN>(a, p, shared, e);
 }
 
+#include "attention_shared_tc.cuh"
+
 // ------------------------------------------------------------------ host side
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
 struct Plan {
     long long shared_items, own_items;
     int shared_pieces, own_pieces, own_tiles;
+    int tile_tokens;                            // tokens of a tile on the tensor cores of the fifth generation; 0: the other kernels
 };
 
-// Into how many pieces the keys are cut: enough for about three CTAs an SM, none shorter than MIN_KEYS.
-Plan plan_of(int tokens, int groups, int num_q, int num_kv, int max_shared, int max_own, int dtype) {
-    constexpr int MIN_KEYS = 128, CTAS = 3 * 148;
-    const int heads = num_q / num_kv, tile = dtype == TVB_F32 ? 16 : 64;
-    const long long tiles = groups > 0 && max_shared > 0 ? (long long)tokens * heads / tile + groups : 0;
-    auto pieces_of = [&](long long items, int keys, int most) {
-        const long long wanted = items > 0 ? ceil_div(CTAS, items) : 1;
+// Into how many pieces the keys are cut: the shared ones so that the CTAs have one round on the GPU, the tokens' own into about
+// three CTAs an SM; none shorter than MIN_KEYS.
+Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size, int max_shared, int max_own, int dtype) {
+    constexpr int MIN_KEYS = 128, SMS = 148;
+    const int heads = num_q / num_kv;
+    Plan p;
+    p.tile_tokens = dtype == TVB_BF16 && tc_takes(head_dim, heads, page_size) ? TC_ROWS / heads : 0;
+    long long tiles = 0;
+    if (groups > 0 && max_shared > 0)
+        tiles = groups + (p.tile_tokens > 0 ? tokens / p.tile_tokens : (long long)tokens * heads / (dtype == TVB_F32 ? 16 : 64));
+    auto pieces_of = [&](long long ctas, long long items, int keys, int most) {
+        const long long wanted = items > 0 ? max(1ll, ctas / items) : 1;
         return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1), MIN_KEYS)), (long long)most));
     };
-    Plan p;
     p.own_tiles = (int)ceil_div(heads, dtype == TVB_F32 ? 4 : 16);
-    p.shared_pieces = tiles > 0 ? pieces_of(tiles * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
-    p.own_pieces = pieces_of((long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
+    p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? SMS : 3 * SMS, tiles * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
+    p.own_pieces = pieces_of(4 * SMS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
     p.shared_items = tiles * num_kv * p.shared_pieces;
     p.own_items = (long long)tokens * num_kv * p.own_tiles * p.own_pieces;
     return p;
@@ -805,23 +813,34 @@ template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int p
         const int e = p.shared_items == 0 ? 0 : launch(attend_shared_f32_kernel<D>, p.shared_items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, 0, s, a);
         return e ? e : launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, cluster, s, a);
     }
-    const int e = p.shared_items == 0 ? 0 : launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
+    int e = 0;
+    if (p.shared_items > 0) {
+        if constexpr (D <= 128) {
+            if (p.tile_tokens > 0) e = launch_shared_tc<D>(a, p.shared_items, p.tile_tokens, pdl, s);
+            else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
+        } else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
+    }
     return e ? e : launch(attend_own_bf16_kernel<D>, p.own_items, Tiles<D>::bytes(16), pdl, cluster, s, a);
 }
 
 }  // namespace
 
-// float32 of scratch
-extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int num_q, int num_kv, int head_dim, int max_shared, int max_own,
-                                                  int dtype) {
+// float32 of scratch, and the launches that a call takes in `launches`
+extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size,
+                                                  int max_shared, int max_own, int dtype, int* launches) {
+    *launches = 0;
     if (tokens <= 0 || num_kv <= 0) return 0;
-    const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
+    const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
+    *launches = p.shared_items > 0 ? 2 : 1;
     return (long long)tokens * num_q * p.shared_pieces * (head_dim + 2);
 }
 
-// launches that a call takes
-extern "C" int tvb_attention_shared_launches(int tokens, int groups, int num_q, int num_kv, int max_shared, int max_own, int dtype) {
-    return tokens <= 0 || num_kv <= 0 ? 0 : plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype).shared_items > 0 ? 2 : 1;
+// 0, or which bounded wait gave up in some launch since the last call; reading clears it.  Synchronises.
+extern "C" int tvb_attention_shared_status() {
+    int value = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&value, tvb_attention_shared_status_word, sizeof(int)) != cudaSuccess) return -1;
+    if (value != 0) cudaMemcpyToSymbol(tvb_attention_shared_status_word, &zero, sizeof(int));
+    return value;
 }
 
 extern "C" int tvb_attention_shared(const void* q, long long q_stride, const void* keys, const void* values, const int* tables, int rows,
@@ -833,7 +852,7 @@ extern "C" int tvb_attention_shared(const void* q, long long q_stride, const voi
     if ((dtype != TVB_F32 && dtype != TVB_BF16) || num_kv <= 0 || num_q <= 0 || num_q % num_kv || page_size <= 0 || groups < 0 || rows < 0 ||
         width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096)
         return TVB_BAD_ARGUMENT;
-    const Plan p = plan_of(tokens, groups, num_q, num_kv, max_shared, max_own, dtype);
+    const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
     if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
     Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, scratch, nullptr, out, out_stride,
              tokens, rows, width, groups, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, scale * LOG2E};

@@ -9,6 +9,7 @@ library they raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
@@ -2121,6 +2122,26 @@ def adapters_expand(u: torch.Tensor, up: torch.Tensor, ids: torch.Tensor, y: tor
 
 
 # ------------------------------------------ attention over keys in common (paged)
+@functools.lru_cache(maxsize=4096)
+def _shared_plan(*sizes: int) -> tuple[int, int]:
+    """(float32 of scratch, launches) of an :func:`attention_shared` of these sizes."""
+    launches = ctypes.c_int(0)
+    floats = _fn("attention_shared", "tvb_attention_shared_scratch", [c_int] * 9 + [ctypes.POINTER(c_int)], c_longlong)(
+        *sizes, ctypes.byref(launches))
+    return floats, launches.value
+
+
+_attention_shared_unchecked = False
+
+
+def attention_shared_status() -> int:
+    """0, or which bounded wait of an :func:`attention_shared` launch gave up since the last call (the results of that launch are
+    not valid).  Synchronises the device; reading clears the record."""
+    global _attention_shared_unchecked
+    _attention_shared_unchecked = False
+    return _fn("attention_shared", "tvb_attention_shared_status", [])()
+
+
 def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tensor, value_cache: torch.Tensor,
                      block_tables: torch.Tensor, token_row: torch.Tensor, positions: torch.Tensor, *,
                      group_starts: torch.Tensor, shared_lens: torch.Tensor, num_q: int, num_kv: int, head_dim: int,
@@ -2171,8 +2192,7 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
     if tokens == 0:
         return out
-    need = _fn("attention_shared", "tvb_attention_shared_scratch", [c_int] * 8, c_longlong)(
-        tokens, groups, num_q, num_kv, head_dim, max_shared, max_own, tag)
+    need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, key_cache.shape[2], max_shared, max_own, tag)
     scratch = torch.empty(need, dtype=torch.float32, device=q.device)
     fn = _fn("attention_shared", "tvb_attention_shared",
              [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
@@ -2181,8 +2201,9 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
               block_tables.shape[0], block_tables.shape[1], token_row.data_ptr(), positions.data_ptr(), group_starts.data_ptr(),
               shared_lens.data_ptr(), groups, scratch.data_ptr(), out.data_ptr(), out.stride(0), tokens, key_cache.shape[0],
               key_cache.shape[2], num_q, num_kv, head_dim, max_shared, max_own, scale, tag, _pdl("attention_shared"), _stream()),
-           "attention_shared",
-           _fn("attention_shared", "tvb_attention_shared_launches", [c_int] * 7)(tokens, groups, num_q, num_kv, max_shared, max_own, tag))
+           "attention_shared", launches)
+    global _attention_shared_unchecked
+    _attention_shared_unchecked = _attention_shared_unchecked or launches > 1
     return out
 
 
@@ -2778,4 +2799,9 @@ def check_finished_launches() -> None:
         status = attention_prefill_tc_status()
         if status:
             raise KernelError(f"attention_prefill_tc: a wait inside the kernel ran out (code {status}); "
+                              "the results of this step are not valid")
+    if _attention_shared_unchecked:
+        status = attention_shared_status()
+        if status:
+            raise KernelError(f"attention_shared: a wait inside the kernel ran out (code {status}); "
                               "the results of this step are not valid")
