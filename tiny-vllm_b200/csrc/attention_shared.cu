@@ -24,10 +24,19 @@ namespace cg = cooperative_groups;
 
 namespace {
 
+#ifndef TVB_RING
+#define TVB_RING 3
+#endif
+#ifndef TVB_CTAS
+#define TVB_CTAS 592
+#endif
+#ifndef TVB_OWN
+#define TVB_OWN 8
+#endif
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int KEYS = 64;                        // keys of a bfloat16 tile
 constexpr int KEYS32 = 32;                      // keys of a float32 tile
-constexpr int MAX_SHARED_PIECES = 64, MAX_OWN_PIECES = 8;
+constexpr int MAX_SHARED_PIECES = 64, MAX_OWN_PIECES = TVB_OWN;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Attend {
@@ -50,6 +59,20 @@ struct Attend {
 };
 
 struct Range { int first, end; };
+
+// V neighbouring float32 (2, 4 or 8), from where another kernel may have written them
+template <int V> __device__ __forceinline__ void load_lane(const float* from, float (&v)[V]) {
+    if constexpr (V == 2) {
+        const float2 f = __ldcg(reinterpret_cast<const float2*>(from));
+        v[0] = f.x; v[1] = f.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(from + i));
+            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+        }
+    }
+}
 
 // piece c of n keys in up to `pieces`: whole tiles of 64, of the shared keys whole blocks of 128
 __device__ __forceinline__ int piece_keys(int n, int pieces) { return max(KEYS, ((n + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS); }
@@ -98,14 +121,16 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) {
+__device__ __forceinline__ void ldmatrix_x4_at(uint32_t* r, uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, const bf16* p) {
+__device__ __forceinline__ void ldmatrix_x4_trans_at(uint32_t* r, uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
+__device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) { ldmatrix_x4_at(r, smem_address(p)); }
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, const bf16* p) { ldmatrix_x4_trans_at(r, smem_address(p)); }
 
 // One piece: ROWS query rows (token, head) of one kv head over the keys [range.first, range.end) of the request with this
 // block table.
@@ -199,58 +224,32 @@ __device__ __forceinline__ bool takes_part(const Attend& a, const Piece& p, int 
     const int row = __ldcg(a.token_row + token), position = __ldcg(a.positions + token);
     return (unsigned)row < (unsigned)a.rows && position >= p.keys - 1;          // (no table is shorter than the shared keys)
 }
-// place of a key's row in the cache, in rows of D; -1: no such page
-__device__ __forceinline__ int64_t row_in(const Attend& a, const Piece& p, int page, int key) {
-    return (unsigned)page < (unsigned)a.pages ? ((int64_t)page * a.num_kv + p.kv_head) * a.page_size + key % a.page_size : -1;
+// place of a key's row in the cache, in rows of D (of which there are less than 2^31); -1: no such page
+__device__ __forceinline__ int row_in(const Attend& a, const Piece& p, int page, int key) {
+    return (unsigned)page < (unsigned)a.pages ? (page * a.num_kv + p.kv_head) * a.page_size + key % a.page_size : -1;
 }
-__device__ __forceinline__ int64_t cache_row(const Attend& a, const Piece& p, int key) {
+__device__ __forceinline__ int cache_row(const Attend& a, const Piece& p, int key) {
     return row_in(a, p, __ldcg(p.table + key / a.page_size), key);
 }
 
 // ----------------------------------------------------------- joining the pieces
-// What a CTA of attend_own ends with, in shared memory: rows' O [OWN][D] and (m, l) of its piece.
+// What the warps of an attend_own CTA end with, in shared memory: their rows' O [WARPS][OWN][D] and (m, l) [WARPS][OWN][2].
 template <int D, int OWN> struct Ends {
-    static constexpr int PARTS = MAX_SHARED_PIECES + MAX_OWN_PIECES;
-    static constexpr int WARP_PITCH = D + 4;
-    static constexpr int FLOATS = WARPS * OWN * (WARP_PITCH + 2) + OWN * (D + 2) + 2 * OWN * PARTS;
-    float* warp_o;                              // [WARPS][OWN][WARP_PITCH], the warps' shares
-    float* warp_ml;                             // [WARPS][OWN][2]
-    float* o;                                   // [OWN][D], the CTA's
-    float* ml;                                  // [OWN][2]
-    float* weights;                             // [OWN][PARTS][2]: every part's m and l, then its factor in the first place
-    __device__ __forceinline__ explicit Ends(float* at) {
-        warp_o = at;
-        warp_ml = warp_o + WARPS * OWN * WARP_PITCH;
-        o = warp_ml + WARPS * OWN * 2;
-        ml = o + OWN * D;
-        weights = ml + OWN * 2;
-    }
+    static constexpr int PITCH = D + 4, FLOATS = WARPS * OWN * (PITCH + 2);
+    float* o;
+    float* ml;
+    __device__ __forceinline__ explicit Ends(float* at) : o(at), ml(at + WARPS * OWN * PITCH) {}
 };
 
-// Every warp has stored its share (behind a barrier): the CTA's own, the cluster's, the shared pieces', the result.
+// Every warp has stored its share: the result of the token's rows from the shares of the cluster's warps and the shared pieces, a
+// warp a row, the rows dealt over the cluster.
 template <typename T, int D, int OWN>
-__device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int shared, const Ends<D, OWN>& e) {
+__device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int shared, const Ends<D, OWN>& ends) {
     using E = Ends<D, OWN>;
+    constexpr int V = D / 32, EACH = (MAX_SHARED_PIECES + MAX_OWN_PIECES * WARPS + 31) / 32;     // values, parts of a lane
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, own = a.own_pieces, rank = own > 1 ? (int)cluster.block_rank() : 0;
-    for (int i = tid; i < p.rows * (D / 4); i += THREADS) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, e.warp_ml[2 * (w * OWN + r)]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-        float4 sum = make_float4(0, 0, 0, 0);
-        float total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float f = exp2f(e.warp_ml[2 * (w * OWN + r)] - ref);
-            const float4 v = *reinterpret_cast<const float4*>(e.warp_o + (w * OWN + r) * E::WARP_PITCH + d);
-            sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
-            total += f * e.warp_ml[2 * (w * OWN + r) + 1];
-        }
-        *reinterpret_cast<float4*>(e.o + r * D + d) = sum;
-        if (d == 0) { e.ml[2 * r] = top; e.ml[2 * r + 1] = total; }
-    }
+    const int own = a.own_pieces, rank = own > 1 ? (int)cluster.block_rank() : 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (own > 1) {
         cluster_arrive();
         cluster_wait();
@@ -258,67 +257,78 @@ __device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int
         __syncthreads();
     }
     const int per = shared > 0 ? shared_piece_keys(shared, a.shared_pieces) : 1, used = (shared + per - 1) / per;
+    const int parts = used + own * WARPS;       // the shared pieces, then warp w of the cluster's CTA c at used + c * WARPS + w
     if (a.shared_pieces > 0) pdl_wait();        // the shared pieces are there
-    const int parts = used + own;
-    for (int i = tid; i < p.rows * parts; i += THREADS) {
-        const int r = i / parts, part = i % parts;
-        float2 v;
-        if (part < used) {
-            int head;
-            const int token = token_of(a, p, r, head);
-            v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + part_of(a, token, head, part));
-        } else {
-            const float* ml = own > 1 ? cluster.map_shared_rank(e.ml, part - used) : e.ml;
-            v = make_float2(ml[2 * r], ml[2 * r + 1]);
+    for (int r = rank * WARPS + warp; warp < WARPS && r < p.rows; r += WARPS * own) {
+        int head;
+        const int token = token_of(a, p, r, head);
+        const int64_t first = part_of(a, token, head, 0);
+        float m[EACH], weight[EACH], top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int part = lane + 32 * i;
+            m[i] = -INFINITY;
+            weight[i] = 0.0f;
+            if (part < used) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first + part);
+                m[i] = v.x; weight[i] = v.y;
+            } else if (part < parts) {
+                const int c = (part - used) / WARPS, w = (part - used) % WARPS;
+                const float* ml = (own > 1 ? cluster.map_shared_rank(ends.ml, c) : ends.ml) + 2 * (w * OWN + r);
+                m[i] = ml[0]; weight[i] = ml[1];
+            }
+            top = fmaxf(top, m[i]);
         }
-        e.weights[2 * (r * E::PARTS + part)] = v.x;
-        e.weights[2 * (r * E::PARTS + part) + 1] = v.y;
-    }
-    __syncthreads();
-    for (int r = tid >> 5; r < p.rows; r += WARPS) {                            // a warp a row
-        const int lane = tid & 31;
-        float top = -INFINITY;
-        for (int part = lane; part < parts; part += 32) top = fmaxf(top, e.weights[2 * (r * E::PARTS + part)]);
         top = warp_max(top);
         const float ref = top == -INFINITY ? 0.0f : top;
-        float total = 0.0f;
-        for (int part = lane; part < parts; part += 32) {
-            float* at = e.weights + 2 * (r * E::PARTS + part);
-            at[0] = exp2f(at[0] - ref);
-            total = fmaf(at[0], at[1], total);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            m[i] = exp2f(m[i] - ref);
+            total = fmaf(m[i], weight[i], total);
         }
         total = warp_sum(total);
         const float inverse = total == 0.0f ? 0.0f : 1.0f / total;              // no key is seen: zeros
-        for (int part = lane; part < parts; part += 32) e.weights[2 * (r * E::PARTS + part)] *= inverse;
-    }
-    __syncthreads();
-    for (int i = tid + THREADS * rank; i < p.rows * (D / 4); i += THREADS * own) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        int head;
-        const int token = token_of(a, p, r, head);
-        const float* from = a.part_o + part_of(a, token, head, 0) * D + d;
-        const float* weight = e.weights + 2 * r * E::PARTS;
-        float4 sum = make_float4(0, 0, 0, 0);
-        auto add = [&](float w, const float4& v) {
-            sum.x = fmaf(w, v.x, sum.x); sum.y = fmaf(w, v.y, sum.y); sum.z = fmaf(w, v.z, sum.z); sum.w = fmaf(w, v.w, sum.w);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) weight[i] = m[i] * inverse;
+        float sum[V] = {};
+        auto weight_of = [&](int part) {
+            float w = __shfl_sync(0xffffffffu, weight[0], part & 31);
+#pragma unroll
+            for (int i = 1; i < EACH; ++i) {
+                const float other = __shfl_sync(0xffffffffu, weight[i], part & 31);
+                if (part >> 5 == i) w = other;
+            }
+            return w;
         };
-        int part = 0;
-        for (; part + 4 <= used; part += 4) {
-            float4 v[4];
+        const float* from = a.part_o + first * D + lane * V;
+        constexpr int AHEAD = 8;
+        for (int part = 0; part < used; part += AHEAD) {
+            float v[AHEAD][V];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = __ldcg(reinterpret_cast<const float4*>(from + (int64_t)(part + j) * D));
+            for (int j = 0; j < AHEAD; ++j) {
+                if (part + j >= used) break;
+                load_lane<V>(from + (int64_t)(part + j) * D, v[j]);
+            }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) add(weight[2 * (part + j)], v[j]);
+            for (int j = 0; j < AHEAD; ++j) {
+                if (part + j >= used) break;
+                const float w = weight_of(part + j);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] = fmaf(w, v[j][e], sum[e]);
+            }
         }
-        for (; part < used; ++part) add(weight[2 * part], __ldcg(reinterpret_cast<const float4*>(from + (int64_t)part * D)));
         for (int c = 0; c < own; ++c) {
-            const float* o = own > 1 ? cluster.map_shared_rank(e.o, c) : e.o;
-            add(weight[2 * (used + c)], *reinterpret_cast<const float4*>(o + r * D + d));
-        }
-        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + d;
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+            const float* o = (own > 1 ? cluster.map_shared_rank(ends.o, c) : ends.o) + r * E::PITCH + lane * V;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) out[j] = from_float<T>(v[j]);
+            for (int w = 0; w < WARPS; ++w) {
+                const float f = weight_of(used + c * WARPS + w);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] = fmaf(f, o[w * OWN * E::PITCH + e], sum[e]);
+            }
+        }
+        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + lane * V;
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = from_float<T>(sum[e]);
     }
     if (own > 1) {                              // the others' shared memory is read until here
         cluster_arrive();
@@ -329,7 +339,7 @@ __device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int
 // a token that is none: zeros
 template <typename T, int D> __device__ __forceinline__ void store_zeros(const Attend& a, const Piece& p) {
     if (blockIdx.x % a.own_pieces != 0) return;
-    for (int i = threadIdx.x; i < p.rows * D; i += THREADS) {
+    for (int i = threadIdx.x; i < p.rows * D; i += blockDim.x) {
         int head;
         const int token = token_of(a, p, i / D, head);
         reinterpret_cast<T*>(a.out)[token * a.out_stride + head * D + i % D] = from_float<T>(0.0f);
@@ -347,21 +357,19 @@ __device__ __forceinline__ void start_own(const Attend& a) {
 template <int D> struct Tiles {
     static constexpr int PITCH = D + 8;
     static constexpr int TILE = KEYS * PITCH;                                   // elements of a K or V tile
-    static constexpr int bytes(int rows) { return (rows + 4 * KEYS) * PITCH * 2 + 3 * KEYS * 8 + 3 * 2 * 4 + 64; }
+    static constexpr int bytes(int rows) { return (rows + 4 * KEYS) * PITCH * 2 + 3 * KEYS * 4 + 3 * 2 * 4 + 64; }
 };
 
-// SHARED: the tile's 64 query rows, 16 a warp, every warp over every key.  Else: up to 16 query rows, a warp over 16 keys of
-// every tile, the warps' results joined at the end.
-template <int D, bool SHARED>
-__device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, int shared, unsigned char* raw) {
-    constexpr int PITCH = Tiles<D>::PITCH, ROWS = SHARED ? 64 : 16;
-    constexpr int NK = SHARED ? KEYS : KEYS / WARPS;                            // keys of a tile that a warp has
+// A piece of the shared keys, 64 query rows, 16 a warp: for what the kernel of attention_shared_tc.cuh does not take.
+template <int D>
+__device__ __forceinline__ void attend_shared_piece(const Attend& a, const Piece& p, unsigned char* raw) {
+    constexpr int PITCH = Tiles<D>::PITCH, ROWS = 64, NK = KEYS;
     bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [ROWS][PITCH]
     bf16* k_s = q_s + ROWS * PITCH;                                              // [2][KEYS][PITCH]
     bf16* v_s = k_s + 2 * Tiles<D>::TILE;
     // of a tile's keys: the place of their rows (-1: none), and which there are.  Three tiles of them: one warp may look up
     // those of a tile while another still reads the bits of the one two before.
-    int64_t* at_s = reinterpret_cast<int64_t*>(v_s + 2 * Tiles<D>::TILE);       // [3][KEYS]
+    int* at_s = reinterpret_cast<int*>(v_s + 2 * Tiles<D>::TILE);               // [3][KEYS]
     uint32_t* there_s = reinterpret_cast<uint32_t*>(at_s + 3 * KEYS);           // [3][2]
     bool* takes_s = reinterpret_cast<bool*>(there_s + 6);                       // [ROWS] tokens that take part
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -378,7 +386,7 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
         const int slot = tile % 3;
         if (tid < KEYS) {
             const int key = p.range.first + tile * KEYS + tid;
-            const int64_t at = key < p.range.end ? row_in(a, p, page, key) : -1;
+            const int at = key < p.range.end ? row_in(a, p, page, key) : -1;
             at_s[slot * KEYS + tid] = at;
             const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
             if (lane == 0) there_s[slot * 2 + warp] = there;
@@ -390,8 +398,8 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
 #pragma unroll 4
         for (int i = tid; i < KEYS * WORDS; i += THREADS) {
             const int key = i / WORDS, word = i % WORDS;
-            const int64_t at = at_s[slot * KEYS + key];
-            const int64_t from = (at < 0 ? 0 : at) * D + word * 8;
+            const int at = at_s[slot * KEYS + key];
+            const int64_t from = (int64_t)max(at, 0) * D + word * 8;
             cp_async_16(k_s + buffer * Tiles<D>::TILE + key * PITCH + word * 8, keys + from, at >= 0);
             cp_async_16(v_s + buffer * Tiles<D>::TILE + key * PITCH + word * 8, values + from, at >= 0);
         }
@@ -399,11 +407,9 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
     };
     const int first_page = page_of(0);
     int next_page = page_of(1);
-    if constexpr (SHARED) {
-        if (tid < ROWS) {
-            int head;
-            takes_s[tid] = tid < p.rows && takes_part(a, p, token_of(a, p, tid, head));
-        }
+    if (tid < ROWS) {
+        int head;
+        takes_s[tid] = tid < p.rows && takes_part(a, p, token_of(a, p, tid, head));
     }
 #pragma unroll 4
     for (int i = tid; i < ROWS * (D / 8); i += THREADS) {
@@ -419,7 +425,7 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
     place(0, first_page);
     __syncthreads();
     if (tiles > 0) load(0);
-    const bf16* q_rows = q_s + (SHARED ? warp * 16 : 0) * PITCH + (lane & 15) * PITCH + (lane >> 4) * 8;
+    const bf16* q_rows = q_s + warp * 16 * PITCH + (lane & 15) * PITCH + (lane >> 4) * 8;
     uint32_t q_frag[D <= 128 ? D / 16 : 1][4];
     if constexpr (D <= 128)
 #pragma unroll
@@ -431,7 +437,6 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const int key_at = SHARED ? 0 : warp * NK;
 
     for (int tile = 0; tile < tiles; ++tile) {
         const int buffer = tile & 1;
@@ -442,8 +447,8 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
         cp_async_wait<0>();
         __syncthreads();                                                        // the tile is there; places of the next too
         if (tile + 1 < tiles) load(tile + 1);
-        const bf16* k_tile = k_s + buffer * Tiles<D>::TILE + key_at * PITCH;
-        const bf16* v_tile = v_s + buffer * Tiles<D>::TILE + key_at * PITCH;
+        const bf16* k_tile = k_s + buffer * Tiles<D>::TILE;
+        const bf16* v_tile = v_s + buffer * Tiles<D>::TILE;
         float s[NK / 8][4];
 #pragma unroll
         for (int n = 0; n < NK / 8; ++n)
@@ -470,7 +475,7 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 s[n][i] *= a.scale_log2;
-                if (~there != 0 && !(there >> (key_at + n * 8 + 2 * t4 + (i & 1)) & 1)) s[n][i] = -INFINITY;
+                if (~there != 0 && !(there >> (n * 8 + 2 * t4 + (i & 1)) & 1)) s[n][i] = -INFINITY;
                 most[i >> 1] = fmaxf(most[i >> 1], s[n][i]);
             }
         float subtract[2];
@@ -519,35 +524,17 @@ __device__ __forceinline__ void attend_piece(const Attend& a, const Piece& p, in
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    if constexpr (SHARED) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = warp * 16 + g + 8 * h;
-            if (r >= p.rows || !takes_s[r]) continue;
-            int head;
-            const int token = token_of(a, p, r, head);
-            const int64_t part = part_of(a, token, head, p.slot);
+    for (int h = 0; h < 2; ++h) {
+        const int r = warp * 16 + g + 8 * h;
+        if (r >= p.rows || !takes_s[r]) continue;
+        int head;
+        const int token = token_of(a, p, r, head);
+        const int64_t part = part_of(a, token, head, p.slot);
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(a.part_o + part * D + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-            if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[h], l[h]);
-        }
-    } else {
-        // the warps' shares lie over the tiles
-        using E = Ends<D, 16>;
-        static_assert(E::FLOATS * 4 <= 4 * Tiles<D>::TILE * 2, "room for what the CTA ends with");
-        const E e(reinterpret_cast<float*>(k_s));
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = warp * 16 + g + 8 * h;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n)
-                *reinterpret_cast<float2*>(e.warp_o + r * E::WARP_PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-            if (t4 == 0) { e.warp_ml[2 * r] = m[h]; e.warp_ml[2 * r + 1] = l[h]; }
-        }
-        __syncthreads();
-        join_pieces<bf16, D, 16>(a, p, shared, e);
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(a.part_o + part * D + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (t4 == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m[h], l[h]);
     }
 }
 
@@ -556,19 +543,183 @@ template <int D> __global__ void __launch_bounds__(THREADS) attend_shared_bf16_k
     pdl_wait();
     pdl_launch_dependents();
     Piece p;
-    if (find_shared_piece(a, 64, p)) attend_piece<D, true>(a, p, 0, raw);
+    if (find_shared_piece(a, 64, p)) attend_shared_piece<D>(a, p, raw);
 }
 
-template <int D> __global__ void __launch_bounds__(THREADS) attend_own_bf16_kernel(Attend a) {
+// A token's own keys: up to 16 of its query heads (one tile of the instruction), tiles of 32 keys, eight a warp, in a ring of three.
+template <int D> struct OwnTiles {
+    static constexpr int KEYS = 32, RING = TVB_RING, PITCH = D + 8, TILE = KEYS * PITCH;
+    static constexpr int RING_BYTES = (16 + 2 * RING * KEYS) * PITCH * 2, END_BYTES = Ends<D, 16>::FLOATS * 4;
+    static constexpr int BYTES = (RING_BYTES > END_BYTES ? RING_BYTES : END_BYTES) + 8 * KEYS * 4 + 8 * 4;
+    static constexpr int CTAS = D == 64 ? 6 : D == 128 ? 4 : 2;                 // on an SM
+};
+__device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
+}
+
+template <int D> __global__ void __launch_bounds__(THREADS, TVB_RING == 3 ? OwnTiles<D>::CTAS : 1) attend_own_bf16_kernel(Attend a) {
+    using S = OwnTiles<D>;
+    constexpr int PITCH = S::PITCH, WORDS = D / 8;
     extern __shared__ __align__(16) unsigned char raw[];
     start_own(a);
     Piece p;
     int shared = 0;
-    if (find_own_piece(a, 16, p, shared)) attend_piece<D, false>(a, p, shared, raw);
-    else {
+    if (!find_own_piece(a, 16, p, shared)) {
         store_zeros<bf16, D>(a, p);
         if (a.shared_pieces > 0) pdl_wait();
+        return;
     }
+    bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [16][PITCH]
+    bf16* k_s = q_s + 16 * PITCH;                                               // [RING][KEYS][PITCH]
+    bf16* v_s = k_s + S::RING * S::TILE;
+    // of a tile's keys: the place of their rows (-1: none), and which there are; four tiles of them, the last being looked up while
+    // a slow warp is still at the first
+    int* at_s = reinterpret_cast<int*>(raw + S::BYTES - 8 * S::KEYS * 4 - 8 * 4);                // [8][KEYS]
+    uint32_t* there_s = reinterpret_cast<uint32_t*>(at_s + 8 * S::KEYS);        // [8]
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const bf16* keys = reinterpret_cast<const bf16*>(a.keys);
+    const bf16* values = reinterpret_cast<const bf16*>(a.values);
+    const int tiles = (p.range.end - p.range.first + S::KEYS - 1) / S::KEYS;
+    // the first warp; a page's number is asked for a tile before it is looked at
+    auto page_of = [&](int tile) -> int {
+        const int key = p.range.first + tile * S::KEYS + lane;
+        return warp == 0 && key < p.range.end ? __ldcg(p.table + key / a.page_size) : -1;
+    };
+    auto place = [&](int tile, int page) {
+        if (warp != 0) return;
+        const int key = p.range.first + tile * S::KEYS + lane;
+        const int at = key < p.range.end ? row_in(a, p, page, key) : -1;
+        at_s[(tile & 7) * S::KEYS + lane] = at;
+        const uint32_t there = __ballot_sync(0xffffffffu, at >= 0);
+        if (lane == 0) there_s[tile & 7] = there;
+    };
+    auto load = [&](int tile) {
+        if (tile < tiles) {
+            bf16* k_to = k_s + tile % S::RING * S::TILE;
+            bf16* v_to = v_s + tile % S::RING * S::TILE;
+#pragma unroll 4
+            for (int i = tid; i < S::KEYS * WORDS; i += THREADS) {
+                const int key = i / WORDS, word = i % WORDS;
+                const int at = at_s[(tile & 7) * S::KEYS + key];
+                const int64_t from = (int64_t)max(at, 0) * D + word * 8;
+                cp_async_16(k_to + key * PITCH + word * 8, keys + from, at >= 0);
+                cp_async_16(v_to + key * PITCH + word * 8, values + from, at >= 0);
+            }
+        }
+        cp_async_commit();
+    };
+    {
+        int pages[S::RING - 1];
+#pragma unroll
+        for (int i = 0; i < S::RING - 1; ++i) pages[i] = page_of(i);
+        for (int i = tid; i < 16 * WORDS; i += THREADS) {
+            const int r = i / WORDS, word = i % WORDS;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (r < p.rows) {
+                int head;
+                const int token = token_of(a, p, r, head);
+                v = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(a.q) + token * a.q_stride + head * D + word * 8));
+            }
+            *reinterpret_cast<uint4*>(q_s + r * PITCH + word * 8) = v;
+        }
+#pragma unroll
+        for (int i = 0; i < S::RING - 1; ++i) place(i, pages[i]);
+    }
+    int next_page = page_of(S::RING - 1);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::RING - 1; ++i) load(i);
+    const bf16* q_rows = q_s + (lane & 15) * PITCH + (lane >> 4) * 8;
+    uint32_t q_frag[D <= 128 ? D / 16 : 1][4];
+    if constexpr (D <= 128)
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) ldmatrix_x4(q_frag[ks], q_rows + ks * 16);
+    float o[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[n][i] = 0.0f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+    for (int tile = 0; tile < tiles; ++tile) {
+        place(tile + S::RING - 1, next_page);
+        next_page = page_of(tile + S::RING);
+        cp_async_wait<S::RING - 2>();
+        __syncthreads();                        // the tile is there, the places of the one after next too, the one before is through
+        load(tile + S::RING - 1);
+        const int at = (warp * 8 + (lane & 7)) * PITCH + (lane >> 3) * 8;       // of this warp's keys, 32 values at a time
+        const bf16* k_tile = k_s + tile % S::RING * S::TILE + at;
+        const bf16* v_tile = v_s + tile % S::RING * S::TILE + at;
+        float s[2][4] = {};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+            uint32_t b[4];
+            ldmatrix_x4(b, k_tile + ks * 32);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t q_now[4];
+                if constexpr (D > 128) ldmatrix_x4(q_now, q_rows + (2 * ks + half) * 16);
+                const uint32_t (&q4)[4] = D <= 128 ? q_frag[D <= 128 ? 2 * ks + half : 0] : q_now;
+                mma_16816(s[half], q4, b[2 * half], b[2 * half + 1]);
+            }
+        }
+        const uint32_t there = there_s[tile & 7] >> (warp * 8);
+        float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[0][i] = there >> (2 * t4 + (i & 1)) & 1 ? (s[0][i] + s[1][i]) * a.scale_log2 : -INFINITY;
+            most[i >> 1] = fmaxf(most[i >> 1], s[0][i]);
+        }
+        float subtract[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+            most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+            const float now = fmaxf(m[h], most[h]);
+            subtract[h] = now == -INFINITY ? 0.0f : now;                        // no inf - inf where no key was seen yet
+            most[h] = exp2_unit(m[h] - subtract[h]);
+            m[h] = now;
+            l[h] *= most[h];
+        }
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = exp2_unit(s[0][i] - subtract[i >> 1]);
+            l[i >> 1] += w[i];
+        }
+        const uint32_t w_lo = pack_bf16x2(w[0], w[1]), w_hi = pack_bf16x2(w[2], w[3]);
+        if (__any_sync(0xffffffffu, most[0] != 1.0f || most[1] != 1.0f))
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][i] *= most[i >> 1];
+#pragma unroll
+        for (int dp = 0; dp < D / 32; ++dp) {
+            uint32_t b[4];
+            ldmatrix_x4_trans(b, v_tile + dp * 32);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_1688(o[4 * dp + j], w_lo, w_hi, b[j]);
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    const Ends<D, 16> ends(reinterpret_cast<float*>(raw));                      // over the tiles
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h, at = warp * 16 + r;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(ends.o + at * Ends<D, 16>::PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+        if (t4 == 0) *reinterpret_cast<float2*>(ends.ml + 2 * at) = make_float2(m[h], l[h]);
+    }
+    join_pieces<bf16, D, 16>(a, p, shared, ends);
 }
 
 // ------------------------------------------------------------------- float32
@@ -691,18 +842,6 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float* keys = reinterpret_cast<const float*>(a.keys);
     const float* values = reinterpret_cast<const float*>(a.values);
-    auto load = [&](const float* from, float (&v)[V]) {
-        if constexpr (V == 2) {
-            const float2 f = __ldcg(reinterpret_cast<const float2*>(from + lane * V));
-            v[0] = f.x; v[1] = f.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                const float4 f = __ldcg(reinterpret_cast<const float4*>(from + lane * V + i));
-                v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
-            }
-        }
-    };
     float q[OWN][V] = {}, o[OWN][V] = {}, m[OWN], l[OWN] = {};
 #pragma unroll
     for (int r = 0; r < OWN; ++r) {
@@ -710,7 +849,7 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
         if (r >= p.rows) continue;
         int head;
         const int token = token_of(a, p, r, head);
-        load(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D, q[r]);
+        load_lane<V>(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D + lane * V, q[r]);
     }
     for (int key0 = p.range.first + warp; key0 < p.range.end; key0 += AHEAD * WARPS) {
         float k[AHEAD][V] = {}, v[AHEAD][V] = {};
@@ -721,8 +860,8 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
             const int64_t at = key < p.range.end ? cache_row(a, p, key) : -1;
             there[i] = at >= 0;
             if (there[i]) {
-                load(keys + at * D, k[i]);
-                load(values + at * D, v[i]);
+                load_lane<V>(keys + at * D + lane * V, k[i]);
+                load_lane<V>(values + at * D + lane * V, v[i]);
             }
         }
 #pragma unroll
@@ -752,19 +891,19 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
             }
         }
     }
-    const E e(reinterpret_cast<float*>(raw));
+    const E ends(reinterpret_cast<float*>(raw));
 #pragma unroll
     for (int r = 0; r < OWN; ++r) {
         const int at = warp * OWN + r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) e.warp_o[at * E::WARP_PITCH + lane * V + i] = o[r][i];
-        if (lane == 0) { e.warp_ml[2 * at] = m[r]; e.warp_ml[2 * at + 1] = l[r]; }
+        for (int i = 0; i < V; ++i) ends.o[at * E::PITCH + lane * V + i] = o[r][i];
+        if (lane == 0) { ends.ml[2 * at] = m[r]; ends.ml[2 * at + 1] = l[r]; }
     }
-    __syncthreads();
-    join_pieces<float, D, OWN>(a, p, shared, e);
+    join_pieces<float, D, OWN>(a, p, shared, ends);
 }
 
 #include "attention_shared_tc.cuh"
+#include "attention_own_tma.cuh"
 
 // ------------------------------------------------------------------ host side
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
@@ -791,7 +930,7 @@ Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pa
     };
     p.own_tiles = (int)ceil_div(heads, dtype == TVB_F32 ? 4 : 16);
     p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? SMS : 3 * SMS, tiles * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
-    p.own_pieces = pieces_of(4 * SMS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
+    p.own_pieces = pieces_of(TVB_CTAS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
     p.shared_items = tiles * num_kv * p.shared_pieces;
     p.own_items = (long long)tokens * num_kv * p.own_tiles * p.own_pieces;
     return p;
@@ -820,7 +959,9 @@ template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int p
             else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
         } else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
     }
-    return e ? e : launch(attend_own_bf16_kernel<D>, p.own_items, Tiles<D>::bytes(16), pdl, cluster, s, a);
+    if (e) return e;
+    if (own_tma_takes(a.page_size)) return launch_own_tma<D>(a, p.own_items, cluster, pdl, s);
+    return launch(attend_own_bf16_kernel<D>, p.own_items, OwnTiles<D>::BYTES, pdl, cluster, s, a);
 }
 
 }  // namespace
@@ -850,7 +991,8 @@ extern "C" int tvb_attention_shared(const void* q, long long q_stride, const voi
                                     void* stream) {
     if (tokens <= 0) return 0;
     if ((dtype != TVB_F32 && dtype != TVB_BF16) || num_kv <= 0 || num_q <= 0 || num_q % num_kv || page_size <= 0 || groups < 0 || rows < 0 ||
-        width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096)
+        width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096 ||
+        (long long)pages * num_kv * page_size > 0x7fffffffLL)
         return TVB_BAD_ARGUMENT;
     const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
     if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL) return TVB_BAD_ARGUMENT;

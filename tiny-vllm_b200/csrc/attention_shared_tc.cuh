@@ -9,26 +9,26 @@
 // maximum has grown by more than 2^8 since the reference that its exponentials use was set.  No key of a piece is hidden from
 // one row and seen by another, so the only masks are the end of the keys and pages that are none.
 //
-// Roles: warp 0 issues the copies (lane p the page p of a block), a thread of warp 1 the products Q K^T, warps 2 to 5 and 6 to 9
+// Roles: warps 0 and 11 issue the copies of keys and of values (lane p the page p of a block), a thread of warp 1 the products Q K^T, warps 2 to 5 and 6 to 9
 // are the softmax groups, warp 10 issues P V (and zeroes rows of V behind the last shared key: what a page holds there is of no
 // account).  Every wait is bounded (tc5.cuh).
 #pragma once
 
 #include "tc5.cuh"
 
-constexpr int TC_THREADS = 352, TC_ROWS = 128, TC_KEYS = 128, TC_GROUP_WARPS = 4;
+constexpr int TC_THREADS = 384, TC_ROWS = 128, TC_KEYS = 128, TC_GROUP_WARPS = 4;
 constexpr int TC_HALF = 128 * 64 * 2;           // [128 rows, 64 values] bfloat16: one swizzled sub-tile
 constexpr float TC_RESCALE = 8.0f;              // log2 of the growth of a row's maximum that moves its reference
 constexpr uint32_t TC_COLUMNS = 512;
 
 template <int HD> struct TcShared {
     static constexpr int TILE = HD / 64 * TC_HALF;                              // a Q, K or V tile
-    // The ring is small enough to leave room for a CTA of attend_own on the same SM.
-    static constexpr int RING = HD == 128 ? 3 : 5;
-    static constexpr int EXCHANGE = TC_ROWS * 2 * 4;                            // [row][reference, denominator] of the second group
-    static constexpr int Q_FULL = 0, KV_FULL = 1, KV_EMPTY = KV_FULL + RING, S_FULL = KV_EMPTY + RING, P_FULL = S_FULL + 2,
+    static constexpr int K_RING = 2, V_RING = 2;                                 // (leaves room for a CTA of attend_own beside)
+    static constexpr int EXCHANGE = TC_ROWS * 2 * 4 + TC_ROWS * 8;              // [row][reference, denominator] of the second group; [row] place of the result
+    static constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + K_RING, V_FULL = K_EMPTY + K_RING, V_EMPTY = V_FULL + V_RING,
+                         S_FULL = V_EMPTY + V_RING, P_FULL = S_FULL + 2,
                          P_READ = P_FULL + 2, O_LAST = P_READ + 2, SECOND_DONE = O_LAST + 2, BARRIERS = SECOND_DONE + 1;
-    static constexpr int BYTES = TILE * (1 + RING) + EXCHANGE + BARRIERS * 8 + 16 + 1024;
+    static constexpr int BYTES = TILE * (1 + K_RING + V_RING) + EXCHANGE + BARRIERS * 8 + 16 + 1024;
 };
 
 __device__ int tvb_attention_shared_status_word = 0;
@@ -39,79 +39,78 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                         const __grid_constant__ CUtensorMap map_v, Attend a, int tile_tokens) {
     using T = TcShared<HD>;
     extern __shared__ uint8_t raw_tc[];
-    pdl_wait();
-    pdl_launch_dependents();
-    Piece p;
     const int heads = a.num_q / a.num_kv;
-    if (!find_shared_piece(a, tile_tokens * heads, p)) return;                  // the whole CTA
     const uint32_t base = (smem_address(raw_tc) + 1023u) & ~1023u;
     uint8_t* aligned = raw_tc + (base - smem_address(raw_tc));
     const uint32_t q_at = base, kv_at = base + T::TILE;
-    float* exchange = reinterpret_cast<float*>(aligned + T::TILE * (1 + T::RING));
-    const uint32_t bars = base + T::TILE * (1 + T::RING) + T::EXCHANGE;
+    float* exchange = reinterpret_cast<float*>(aligned + T::TILE * (1 + T::K_RING + T::V_RING));
+    const uint32_t bars = base + T::TILE * (1 + T::K_RING + T::V_RING) + T::EXCHANGE;
     auto bar = [&](int i) { return bars + 8u * i; };
-    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + T::TILE * (1 + T::RING) + T::EXCHANGE + T::BARRIERS * 8);
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + T::TILE * (1 + T::K_RING + T::V_RING) + T::EXCHANGE + T::BARRIERS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
     int* status = &tvb_attention_shared_status_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int blocks = (p.range.end - p.range.first + TC_KEYS - 1) / TC_KEYS, pages_per_block = TC_KEYS / a.page_size;
-
+    // what needs nothing of the kernel before, while that ends
     if (threadIdx.x == 0) {
         for (int i = 0; i < T::BARRIERS; ++i)
             mbar_init(bar(i), (i >= T::P_FULL && i < T::P_FULL + 2) || i == T::SECOND_DONE ? TC_GROUP_WARPS : 1);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        prefetch_tensormap(&map_q);
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
     }
     if (warp == 1) tmem_alloc(smem_address(tmem_base_slot), TC_COLUMNS);
+    pdl_wait();
+    pdl_launch_dependents();
+    Piece p;
+    const bool found = find_shared_piece(a, tile_tokens * heads, p);            // the same for the whole CTA
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem_base = *tmem_base_slot;
-    // The tiles come through the ring in the order K0, K1, V0, K2, V1, ..: K of block j is tile 2 j - 1 (0 for j = 0), V of block j
-    // tile 2 j + 2 (2 n - 1 for the last of n).
-    auto k_tile_of = [&](int j) -> uint32_t { return j == 0 ? 0 : 2 * j - 1; };
-    auto v_tile_of = [&](int j) -> uint32_t { return j + 1 < blocks ? 2 * j + 2 : 2 * blocks - 1; };
-    // page of this lane in block j; -1 (a coordinate that reads zeros): past the keys, or no page
+    if (!found) {
+        if (warp == 1) tmem_free(tmem_base, TC_COLUMNS);
+        return;
+    }
+    const int blocks = (p.range.end - p.range.first + TC_KEYS - 1) / TC_KEYS, pages_per_block = TC_KEYS / a.page_size;
+    // Two rings, of keys and of values: block j is in slot j % its length.
+    // page of this lane in block j as it stands in the table, -1 past the keys; whether it is one is asked where it is used, since the
+    // warp would wait for the load there and then
     auto page_of = [&](int j) -> int {
         const int index = p.range.first / a.page_size + j * pages_per_block + lane;
-        if (lane >= pages_per_block || j >= blocks || (int64_t)index * a.page_size >= p.range.end) return -1;
-        const int page = __ldcg(p.table + index);
-        return (unsigned)page < (unsigned)a.pages ? page : -1;
+        return lane < pages_per_block && j < blocks && (int64_t)index * a.page_size < p.range.end ? __ldcg(p.table + index) : -1;
     };
+    const uint32_t k_at = kv_at, v_at = kv_at + T::K_RING * T::TILE;
 
-    if (warp == 0) {
+    if (warp == 0 || warp == 11) {
         // ---- copies
-        uint32_t ring = 0;
-        bool alive = true;
-        auto load_tile = [&](const CUtensorMap* map, int page) -> bool {
-            const int slot = ring % T::RING;
-            int ready = lane == 0 ? (int)mbar_wait(bar(T::KV_EMPTY + slot), ((ring / T::RING) & 1u) ^ 1u, abort_flag, status, 1) : 1;
-            if (__shfl_sync(0xffffffffu, ready, 0) == 0) return false;
-            if (lane == 0) mbar_arrive_expect(bar(T::KV_FULL + slot), T::TILE);
-            __syncwarp();
-            if (lane < pages_per_block)
-#pragma unroll
-                for (int h = 0; h < HD / 64; ++h)
-                    tma_load_4d(kv_at + slot * T::TILE + h * TC_HALF + (uint32_t)(lane * a.page_size * 128), map, 64 * h, 0, p.kv_head,
-                                page, bar(T::KV_FULL + slot));
-            ++ring;
-            return true;
-        };
-        int page_v = page_of(0), page_k = page_of(1);
-        if (lane == 0) {
+        const bool of_k = warp == 0;
+        const int ring = of_k ? T::K_RING : T::V_RING, first_full = of_k ? T::K_FULL : T::V_FULL, first_empty = of_k ? T::K_EMPTY : T::V_EMPTY;
+        const CUtensorMap* map = of_k ? &map_k : &map_v;
+        int page = page_of(0), next_page = page_of(1);
+        if (of_k && lane == 0) {
             mbar_arrive_expect(bar(T::Q_FULL), (uint32_t)(tile_tokens * heads * HD * 2));
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h)
                 tma_load_3d(q_at + h * TC_HALF, &map_q, 64 * h, p.kv_head * heads, p.token0 + p.row0 / heads, bar(T::Q_FULL));
         }
         __syncwarp();
-        alive = load_tile(&map_k, page_v);
-        for (int j = 0; j < blocks && alive; ++j) {
-            const int page_after = page_of(j + 2);
-            if (j + 1 < blocks) alive = load_tile(&map_k, page_k);
-            if (alive) alive = load_tile(&map_v, page_v);
-            page_v = page_k;
-            page_k = page_after;
+        for (int j = 0; j < blocks; ++j) {
+            const int slot = j % ring, after = page_of(j + 2);
+            if (j >= ring) {
+                const int ready = lane == 0 ? (int)mbar_wait(bar(first_empty + slot), (j / ring - 1) & 1u, abort_flag, status, 1) : 1;
+                if (__shfl_sync(0xffffffffu, ready, 0) == 0) break;
+            }
+            if (lane == 0) mbar_arrive_expect(bar(first_full + slot), T::TILE);
+            __syncwarp();
+            if (lane < pages_per_block)         // a page that is none: a coordinate that reads zeros
+#pragma unroll
+                for (int h = 0; h < HD / 64; ++h)
+                    tma_load_4d((of_k ? k_at : v_at) + slot * T::TILE + h * TC_HALF + (uint32_t)(lane * a.page_size * 128), map, 64 * h, 0,
+                                p.kv_head, (unsigned)page < (unsigned)a.pages ? page : -1, bar(first_full + slot));
+            page = next_page;
+            next_page = after;
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -119,8 +118,8 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         if (lane == 0 && mbar_wait(bar(T::Q_FULL), 0, abort_flag, status, 8)) {
             constexpr uint32_t idesc = instruction_descriptor_bf16(TC_ROWS, TC_KEYS, false);
             for (int j = 0; j < blocks; ++j) {
-                const uint32_t b = j & 1u, n = j / 2, tile = k_tile_of(j), slot = tile % T::RING;
-                if (!mbar_wait(bar(T::KV_FULL + slot), (tile / T::RING) & 1u, abort_flag, status, 3)) break;
+                const uint32_t b = j & 1u, n = j / 2, slot = j % T::K_RING;
+                if (!mbar_wait(bar(T::K_FULL + slot), (j / T::K_RING) & 1u, abort_flag, status, 3)) break;
                 // S of the group is also where its P lies: the product that read P of the block before must have finished
                 if (n > 0 && !mbar_wait(bar(T::P_READ + b), (n - 1) & 1u, abort_flag, status, 4)) break;
                 tc_fence_after_sync();
@@ -128,9 +127,9 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t half = (kk / 4) * TC_HALF, step = 2u * (kk % 4);
                     tc_mma(tmem_base + b * TC_KEYS, tile_descriptor(q_at + half) + step,
-                           tile_descriptor(kv_at + slot * T::TILE + half) + step, idesc, kk != 0);
+                           tile_descriptor(k_at + slot * T::TILE + half) + step, idesc, kk != 0);
                 }
-                tc_commit(bar(T::KV_EMPTY + slot));
+                tc_commit(bar(T::K_EMPTY + slot));
                 tc_commit(bar(T::S_FULL + b));
             }
         }
@@ -142,9 +141,9 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             return __all_sync(0xffffffffu, mbar_wait(bar(barrier), parity, abort_flag, status, code));
         };
         for (int j = 0; j < blocks; ++j) {
-            const uint32_t b = j & 1u, n = j / 2, tile = v_tile_of(j), slot = tile % T::RING;
-            if (!all_wait(T::KV_FULL + slot, (tile / T::RING) & 1u, 5)) break;
-            const uint32_t v_tile = kv_at + slot * T::TILE;
+            const uint32_t b = j & 1u, n = j / 2, slot = j % T::V_RING;
+            if (!all_wait(T::V_FULL + slot, (j / T::V_RING) & 1u, 5)) break;
+            const uint32_t v_tile = v_at + slot * T::TILE;
             const int have = p.range.end - p.range.first - j * TC_KEYS;         // keys of this block that are shared
             if (have < TC_KEYS) {
                 const int end = min(TC_KEYS, (have + a.page_size - 1) / a.page_size * a.page_size);
@@ -164,7 +163,7 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     // 16 keys: 8 columns of P (two bfloat16 a column), two 1024-byte atoms of V
                     tc_mma_a_in_tmem(tmem_base + 2 * TC_KEYS + b * HD, tmem_base + b * TC_KEYS + kk * 8,
                                      tile_descriptor_mn_major(v_tile + kk * 2048, TC_HALF), idesc, !(j < 2 && kk == 0));
-                tc_commit(bar(T::KV_EMPTY + slot));
+                tc_commit(bar(T::V_EMPTY + slot));
                 tc_commit(bar(T::P_READ + b));
                 if (j + 2 >= blocks) tc_commit(bar(T::O_LAST + b));
             }
@@ -185,9 +184,11 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         };
         float reference = -INFINITY, l = 0.0f;  // what the exponentials of this row subtract (log2); the group's denominator
         bool alive = true;
+        int next_page = page_of(group);
         for (int j = group; j < blocks && alive; j += 2) {
             const int have = p.range.end - p.range.first - j * TC_KEYS;
-            const uint32_t pages = __ballot_sync(0xffffffffu, page_of(j) >= 0);
+            const uint32_t pages = __ballot_sync(0xffffffffu, (unsigned)next_page < (unsigned)a.pages);
+            next_page = page_of(j + 2);
             const bool full = have >= TC_KEYS && __popc(pages) == pages_per_block;
             // which of the 32 keys from c on are there
             auto seen_of = [&](int c) -> uint32_t {
@@ -201,24 +202,24 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             };
             if (!warp_wait(T::S_FULL + group, (j / 2) & 1u, 10)) { alive = false; break; }
             tc_fence_after_sync();
-            // ---- the block's maximum of this row
-            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-            for (int c = 0; c < TC_KEYS; c += 32) {
-                uint32_t v[32];
-                tmem_load_32(s_address + c, v);
-                tmem_load_wait();
-                if (full) {
+            // the row's 128 scores, once: the maximum, then the exponentials
+            uint32_t v[TC_KEYS];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(v[e]) * a.scale_log2);
-                } else {
+            for (int c = 0; c < TC_KEYS; c += 32) tmem_load_32(s_address + c, v + c);
+            tmem_load_wait();
+            if (!full)
+#pragma unroll
+                for (int c = 0; c < TC_KEYS; c += 32) {
                     const uint32_t seen = seen_of(c);
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        part[e & 3] = fmaxf(part[e & 3], seen >> e & 1u ? __uint_as_float(v[e]) * a.scale_log2 : -INFINITY);
+                        if (!(seen >> e & 1u)) v[c + e] = 0xff800000u;          // -inf: its exponential is 0
                 }
-            }
-            const float block_max = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+            float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < TC_KEYS; ++e) part[e & 3] = fmaxf(part[e & 3], __uint_as_float(v[e]));
+            // (the scale is positive)
+            const float block_max = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * a.scale_log2;
             const bool moves = block_max > reference + TC_RESCALE || (reference == -INFINITY && block_max > -INFINITY);
             float factor = 1.0f;
             if (moves) {
@@ -226,6 +227,22 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 reference = block_max;
                 l *= factor;
             }
+            const float subtract = reference == -INFINITY ? 0.0f : reference;
+            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < TC_KEYS; c += 32) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float w0 = exp2_unit(fmaf(__uint_as_float(v[c + e]), a.scale_log2, -subtract));
+                    const float w1 = exp2_unit(fmaf(__uint_as_float(v[c + e + 1]), a.scale_log2, -subtract));
+                    sums[e & 3] += w0;
+                    sums[(e & 3) + 1] += w1;
+                    packed[e / 2] = pack_bf16x2(w0, w1);
+                }
+                tmem_store_16(s_address + c / 2, packed);                       // P over the columns of S
+            }
+            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             // S of this block is there, so the product into this group's O before it has finished: O may be scaled
             if (j >= 2 && __any_sync(0xffffffffu, moves)) {
 #pragma unroll 1
@@ -238,41 +255,23 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                     tmem_store_32(o_address + c, o);
                 }
             }
-            // ---- exponentials; P over the columns of S just read
-            const float subtract = reference == -INFINITY ? 0.0f : reference;
-            float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 1
-            for (int c = 0; c < TC_KEYS; c += 32) {
-                uint32_t v[32], packed[16];
-                tmem_load_32(s_address + c, v);
-                tmem_load_wait();
-                const uint32_t seen = full ? ~0u : seen_of(c);
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float w[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        w[i] = exp2_unit(fmaf(__uint_as_float(v[e + i]), a.scale_log2, -subtract));
-                        if (!full && !(seen >> (e + i) & 1u)) w[i] = 0.0f;
-                        sums[(e + i) & 3] += w[i];
-                    }
-                    packed[e / 2] = pack_bf16x2(w[0], w[1]);
-                }
-                tmem_store_16(s_address + c / 2, packed);
-            }
-            l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             tmem_store_wait();
             tc_fence_before_sync();
             warp_arrive(T::P_FULL + group);
         }
         const bool second = blocks > 1;         // else the second group had no block, and its O holds nothing
         if (alive && (group == 0 || second)) alive = warp_wait(T::O_LAST + group, 0, 13);
+        int64_t* places = reinterpret_cast<int64_t*>(exchange + TC_ROWS * 2);
+        // The rows' O goes out through shared memory (that of the tiles, which are all consumed), so that a warp stores whole rows;
+        // 16-byte word w of row r lies in place w ^ (r % 32, or % 16 for 64 values).
+        constexpr int WORDS = HD / 4;
+        uint4* staged = reinterpret_cast<uint4*>(aligned + T::TILE);
         if (alive && group == 1) {
             exchange[row * 2] = reference;
             exchange[row * 2 + 1] = l;
             tc_fence_before_sync();
             warp_arrive(T::SECOND_DONE);
-        } else if (alive && warp_wait(T::SECOND_DONE, 0, 17)) {
+        } else if (alive && (alive = warp_wait(T::SECOND_DONE, 0, 17))) {
             tc_fence_after_sync();
             const float other = exchange[row * 2], other_l = exchange[row * 2 + 1], top = fmaxf(reference, other);
             const float mine = reference == -INFINITY ? 0.0f : exp2_unit(reference - top);
@@ -280,7 +279,8 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             int head = 0;
             const int token = row < p.rows ? token_of(a, p, row, head) : 0;
             const bool takes = row < p.rows && takes_part(a, p, token);
-            const int64_t at = takes ? part_of(a, token, head, p.slot) : 0;
+            const int64_t at = takes ? part_of(a, token, head, p.slot) : -1;
+            places[row] = at;
             if (takes) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, l * mine + other_l * theirs);
 #pragma unroll 1
             for (int c = 0; c < HD; c += 32) {
@@ -288,18 +288,24 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 tmem_load_32(lane_address + 2 * TC_KEYS + c, x);
                 if (second) tmem_load_32(lane_address + 2 * TC_KEYS + HD + c, y);
                 tmem_load_wait();
-                if (!takes) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) {
-                    float f[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        f[i] = __uint_as_float(x[e + i]) * mine;
-                        if (second) f[i] = fmaf(__uint_as_float(y[e + i]), theirs, f[i]);
-                    }
-                    *reinterpret_cast<float4*>(a.part_o + at * HD + c + e) = make_float4(f[0], f[1], f[2], f[3]);
+                for (int e = 0; e < 32; ++e) {
+                    float f = __uint_as_float(x[e]) * mine;
+                    if (second) f = fmaf(__uint_as_float(y[e]), theirs, f);
+                    x[e] = __float_as_uint(f);
                 }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    staged[row * WORDS + (((c + e) / 4) ^ (row % WORDS))] = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
             }
+        } else if (group == 0) {
+            places[row] = -1;                   // a wait ran out
+        }
+        asm volatile("bar.sync 1, 256;\n" ::: "memory");                        // the softmax warps
+        const int w8 = warp - 2;
+        for (int r = w8; r < TC_ROWS; r += 8) {
+            const int64_t at = places[r];
+            if (at >= 0 && lane < WORDS) *reinterpret_cast<uint4*>(a.part_o + at * HD + lane * 4) = staged[r * WORDS + (lane ^ (r % WORDS))];
         }
     }
     tc_fence_before_sync();

@@ -2183,6 +2183,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     max_own = held if max_own is None else min(max_own, held)
     if max_shared < 0 or max_own < 0:
         raise KernelError("attention_shared: max_shared and max_own are not negative")
+    if not 0.0 < scale < float("inf"):
+        raise KernelError("attention_shared: the scale is positive and finite")
     if out is None:
         _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
         out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
