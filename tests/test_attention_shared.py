@@ -37,7 +37,7 @@ def test_a_good_call_gets_as_far_as_the_device(changed):
     dict(block_tables=torch.zeros(6, dtype=I32)), dict(block_tables=torch.zeros(3, 2)), dict(block_tables=torch.zeros(2, 3, dtype=I32).t()),
     dict(group_starts=torch.zeros(3, dtype=I32)), dict(shared_lens=torch.zeros(1)), dict(shared_lens=torch.zeros(1, 1, dtype=I32)),
     dict(q_token_stride=128), dict(q_token_stride=260), dict(q_token_stride=264), dict(q=torch.zeros(3, 512, dtype=BF16)[:, ::2]),
-    dict(q=torch.zeros(3 * 256 + 8, dtype=BF16)[1:769].view(3, 256)), dict(max_shared=-1), dict(max_own=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
+    dict(q=torch.zeros(3 * 256 + 8, dtype=BF16)[1:769].view(3, 256)), dict(max_shared=-1), dict(max_own=-1), dict(max_shared=2**31), dict(max_own=2**31), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(out=torch.zeros(3, 256)), dict(out=torch.zeros(3, 255, dtype=BF16)), dict(out=torch.zeros(256, 3, dtype=BF16).t()),
     dict(out=torch.zeros(1, 256, dtype=BF16).expand(3, 256)),
 ])

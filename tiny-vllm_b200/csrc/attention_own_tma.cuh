@@ -45,14 +45,13 @@ attend_own_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     start_own(a);
     Piece p;
-    int shared = 0;
-    if (!find_own_piece(a, 16, p, shared)) {
+    if (!find_own_piece(a, 16, p)) {
         store_zeros<bf16, D>(a, p);
-        if (a.shared_pieces > 0) pdl_wait();
+        end_own(a);
         return;
     }
     const int key0 = p.range.first / S::KEYS * S::KEYS;                          // of the first tile
-    const int tiles = p.range.end > p.range.first ? (p.range.end - key0 + S::KEYS - 1) / S::KEYS : 0;
+    const int tiles = (p.range.end - key0 + S::KEYS - 1) / S::KEYS;
     const int box = min(a.page_size, S::KEYS), boxes = S::KEYS / box;            // keys of a copy; copies of a tile of 64 values
     const int shift = 31 - __clz(a.page_size);
     // a page's number as it stands in the table (-1 past the piece); whether it is one is asked where it is used, since the warp
@@ -195,12 +194,13 @@ attend_own_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             *reinterpret_cast<float2*>(ends.o + row * Ends<D, 16>::PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         if (t4 == 0) *reinterpret_cast<float2*>(ends.ml + 2 * row) = make_float2(m[h], l[h]);
     }
-    join_pieces<bf16, D, 16>(a, p, shared, ends);
+    finish_own<bf16, D, 16>(a, p, ends);
+    end_own(a);
 }
 
 inline bool own_tma_takes(int page_size) { return page_size >= 8 && page_size <= 128 && (page_size & (page_size - 1)) == 0; }
 
-template <int D> int launch_own_tma(const Attend& a, long long items, int cluster, int pdl, cudaStream_t stream) {
+template <int D> int launch_own_tma(const Attend& a, long long items, int pdl, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.page_size, (cuuint64_t)a.num_kv, (cuuint64_t)a.pages};
     const cuuint64_t strides[3] = {D * 2, (cuuint64_t)a.page_size * D * 2, (cuuint64_t)a.num_kv * a.page_size * D * 2};
@@ -210,7 +210,7 @@ template <int D> int launch_own_tma(const Attend& a, long long items, int cluste
     auto kernel = attend_own_tma_kernel<D>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnTma<D>::BYTES);
     if (e != cudaSuccess) return (int)e;
-    TvbLaunch at(dim3((unsigned)items), dim3(OwnTma<D>::THREADS_ALL), OwnTma<D>::BYTES, stream, pdl, cluster);
+    TvbLaunch at(dim3((unsigned)items), dim3(OwnTma<D>::THREADS_ALL), OwnTma<D>::BYTES, stream, pdl);
     const cudaError_t launched = cudaLaunchKernelEx(&at.config, kernel, map_k, map_v, a);
     return launched == cudaSuccess ? tvb_last_error() : (int)launched;
 }

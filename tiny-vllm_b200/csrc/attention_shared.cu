@@ -4,39 +4,27 @@
 // head) instead of once a token.
 //
 // Softmax over a union of key ranges from the ranges' own results: a range gives its maximum m, l = sum exp(s - m) and
-// O = sum exp(s - m) v, and ranges join as l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).  Two launches:
+// O = sum exp(s - m) v, and ranges join as l = sum l_i exp(m_i - m), O = sum O_i exp(m_i - m).  The launches:
 //   attend_shared   pieces of the shared keys, a tile of query rows each; m, l and O go to float32 scratch;
-//   attend_own      what every token has behind them, a token's query heads of one kv head a cluster of CTAs that have a piece
-//                   of the keys each; they meet in distributed shared memory, join the shared pieces and store the result.
-// The second does not need the first before its end: launched programmatically it runs beside it (every CTA of the first
-// waits for the kernel before, so what that wrote is there for both) and waits for it before it reads the scratch.
+//   attend_own      what every token has behind them, a CTA a token, kv head and piece; to the scratch too;
+//   join            every row's pieces in their order, and the result.
+// The second does not need the first: launched programmatically it runs beside it (every CTA of the first waits for the kernel before,
+// so what that wrote is there for both), and one of its CTAs waits for the first's end, so that the third has both behind it.  Where
+// no keys are shared and no token's are cut, attend_own is all there is and stores the result itself.
 //
 // bfloat16: mma.sync m16n8k16 over tiles of 64 keys that cp.async brings two deep; a warp of a shared piece has 16 query
 // rows and every key, the warps of a token's own piece share the keys of a tile among them.  P is rounded to bfloat16 for
 // the second product, the denominator sums what was not rounded.  float32: the float32 cores.
 //
 // Bound by reading keys and values while a group has few query rows, by the tensor cores once it has many.
-#include <cooperative_groups.h>
-
 #include "common.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace {
 
-#ifndef TVB_RING
-#define TVB_RING 3
-#endif
-#ifndef TVB_CTAS
-#define TVB_CTAS 592
-#endif
-#ifndef TVB_OWN
-#define TVB_OWN 8
-#endif
 constexpr int THREADS = 128, WARPS = 4;
 constexpr int KEYS = 64;                        // keys of a bfloat16 tile
 constexpr int KEYS32 = 32;                      // keys of a float32 tile
-constexpr int MAX_SHARED_PIECES = 64, MAX_OWN_PIECES = TVB_OWN;
+constexpr int MAX_SHARED_PIECES = 64, MAX_OWN_PIECES = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Attend {
@@ -49,8 +37,8 @@ struct Attend {
     const int* positions;                       // [tokens]
     const int* group_starts;                    // [groups + 1]
     const int* shared_lens;                     // [groups]
-    float* part_o;                              // [tokens, q heads, shared pieces, D]
-    float* part_ml;                             // [tokens, q heads, shared pieces, 2]
+    float* part_o;                              // [tokens, q heads, shared and own pieces, D]; null: attend_own stores the result
+    float* part_ml;                             // [tokens, q heads, shared and own pieces, 2]
     void* out;
     int64_t out_stride;
     int tokens, rows, width, groups, pages, page_size, num_q, num_kv;
@@ -78,15 +66,7 @@ template <int V> __device__ __forceinline__ void load_lane(const float* from, fl
 __device__ __forceinline__ int piece_keys(int n, int pieces) { return max(KEYS, ((n + pieces - 1) / pieces + KEYS - 1) / KEYS * KEYS); }
 __device__ __forceinline__ int shared_piece_keys(int n, int pieces) { return max(2 * KEYS, ((n + pieces - 1) / pieces + 2 * KEYS - 1) / (2 * KEYS) * 2 * KEYS); }
 
-// (plain loads may be served by an L1 that a kernel before filled: attend_own starts without waiting)
-__device__ __forceinline__ int row_of(const Attend& a, int token) {
-    const int row = __ldcg(a.token_row + token);
-    return (unsigned)row < (unsigned)a.rows && __ldcg(a.positions + token) >= 0 ? row : -1;
-}
-// keys a token reads: its position's and those before it, as far as its table goes
-__device__ __forceinline__ int keys_of(const Attend& a, int token) {
-    return (int)min((int64_t)__ldcg(a.positions + token) + 1, (int64_t)a.width * a.page_size);
-}
+// (__ldcg: plain loads may be served by an L1 that a kernel before filled, and attend_own starts without waiting)
 __device__ __forceinline__ int shared_of_group(const Attend& a, int group) {
     return (int)min((int64_t)max(__ldcg(a.shared_lens + group), 0), (int64_t)a.width * a.page_size);
 }
@@ -151,12 +131,15 @@ __device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows
     int tile = item / a.num_kv;
     // the group that has the tile: 32 groups at a time
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
-        int start = 0, count = 0;
+        int start = 0, end = 0, shared = 0;
         if (g0 + lane < a.groups) {
-            start = min(max(__ldcg(a.group_starts + g0 + lane), 0), a.tokens);
-            const int end = min(max(__ldcg(a.group_starts + g0 + lane + 1), start), a.tokens);
-            count = shared_of_group(a, g0 + lane) > 0 ? ((end - start) * heads + tile_rows - 1) / tile_rows : 0;
+            start = __ldcg(a.group_starts + g0 + lane);
+            end = __ldcg(a.group_starts + g0 + lane + 1);
+            shared = shared_of_group(a, g0 + lane);
+            start = min(max(start, 0), a.tokens);
+            end = min(max(end, start), a.tokens);
         }
+        const int count = shared > 0 ? ((end - start) * heads + tile_rows - 1) / tile_rows : 0;
         int upto = count;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -165,18 +148,22 @@ __device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows
         }
         const uint32_t past = __ballot_sync(0xffffffffu, upto > tile);
         if (past == 0) { tile -= __shfl_sync(0xffffffffu, upto, 31); continue; }
-        const int at = __ffs(past) - 1, group = g0 + at;
+        const int at = __ffs(past) - 1;
         tile -= __shfl_sync(0xffffffffu, upto - count, at);
         start = __shfl_sync(0xffffffffu, start, at);
-        const int end = min(max(__ldcg(a.group_starts + group + 1), start), a.tokens);
-        const int n = shared_of_group(a, group), per = shared_piece_keys(n, a.shared_pieces);
+        end = __shfl_sync(0xffffffffu, end, at);
+        const int n = __shfl_sync(0xffffffffu, shared, at), per = shared_piece_keys(n, a.shared_pieces);
         p.range = Range{piece * per, min(n, (piece + 1) * per)};
         if (p.range.first >= n) return false;
         // the table of the first token that reads all of the shared keys
         int row = -1;
         for (int token = start; token < end && row < 0; token += 32) {
-            const int mine = token + lane < end ? row_of(a, token + lane) : -1;
-            const uint32_t reads = __ballot_sync(0xffffffffu, mine >= 0 && keys_of(a, token + lane) >= n);
+            int mine = -1, position = -1;
+            if (token + lane < end) {
+                mine = __ldcg(a.token_row + token + lane);
+                position = __ldcg(a.positions + token + lane);
+            }
+            const uint32_t reads = __ballot_sync(0xffffffffu, (unsigned)mine < (unsigned)a.rows && position >= n - 1);
             if (reads) row = __shfl_sync(0xffffffffu, mine, __ffs(reads) - 1);
         }
         if (row < 0) return false;
@@ -191,9 +178,9 @@ __device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows
     return false;
 }
 
-// The piece of a token's own keys that this CTA of its cluster has (it may be empty), up to `tile` of its query heads, and
-// how many keys the token reads with its group; false: the token is padding.
-__device__ __forceinline__ bool find_own_piece(const Attend& a, int tile_rows, Piece& p, int& shared) {
+// The piece of a token's own keys that this CTA has, up to `tile` of its query heads; false: none (p.rows rows of the token are
+// there, though, for the first of its pieces: the token is padding, or has no keys but shared ones).
+__device__ __forceinline__ bool find_own_piece(const Attend& a, int tile_rows, Piece& p) {
     int item = blockIdx.x;
     const int piece = item % a.own_pieces;
     item /= a.own_pieces;
@@ -203,13 +190,13 @@ __device__ __forceinline__ bool find_own_piece(const Attend& a, int tile_rows, P
     p.token0 = item / a.num_kv;
     p.row0 = tile * tile_rows;
     p.rows = min(tile_rows, a.num_q / a.num_kv - p.row0);
+    p.slot = a.shared_pieces + piece;
     const Facts f = facts_of(a, p.token0);
     if (f.row < 0) return false;
-    shared = f.shared;
-    const int n = f.keys - shared, per = piece_keys(n, a.own_pieces);
-    p.range = Range{shared + min(n, piece * per), shared + min(n, (piece + 1) * per)};
+    const int n = f.keys - f.shared, per = piece_keys(n, a.own_pieces);
+    p.range = Range{f.shared + min(n, piece * per), f.shared + min(n, (piece + 1) * per)};
     p.table = a.tables + (int64_t)f.row * a.width;
-    return true;
+    return p.range.first < p.range.end;
 }
 __device__ __forceinline__ int token_of(const Attend& a, const Piece& p, int r, int& head) {
     const int heads = a.num_q / a.num_kv, at = p.row0 + r;
@@ -217,7 +204,7 @@ __device__ __forceinline__ int token_of(const Attend& a, const Piece& p, int r, 
     return p.token0 + at / heads;
 }
 __device__ __forceinline__ int64_t part_of(const Attend& a, int token, int head, int slot) {
-    return ((int64_t)token * a.num_q + head) * a.shared_pieces + slot;
+    return ((int64_t)token * a.num_q + head) * (a.shared_pieces + a.own_pieces) + slot;
 }
 // a token that takes part in its group's pieces: it is one, and reads all of the shared keys
 __device__ __forceinline__ bool takes_part(const Attend& a, const Piece& p, int token) {
@@ -241,104 +228,56 @@ template <int D, int OWN> struct Ends {
     __device__ __forceinline__ explicit Ends(float* at) : o(at), ml(at + WARPS * OWN * PITCH) {}
 };
 
-// Every warp has stored its share: the result of the token's rows from the shares of the cluster's warps and the shared pieces, a
-// warp a row, the rows dealt over the cluster.
-template <typename T, int D, int OWN>
-__device__ __forceinline__ void join_pieces(const Attend& a, const Piece& p, int shared, const Ends<D, OWN>& ends) {
-    using E = Ends<D, OWN>;
-    constexpr int V = D / 32, EACH = (MAX_SHARED_PIECES + MAX_OWN_PIECES * WARPS + 31) / 32;     // values, parts of a lane
-    cg::cluster_group cluster = cg::this_cluster();
-    const int own = a.own_pieces, rank = own > 1 ? (int)cluster.block_rank() : 0;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (own > 1) {
-        cluster_arrive();
-        cluster_wait();
-    } else {
-        __syncthreads();
-    }
-    const int per = shared > 0 ? shared_piece_keys(shared, a.shared_pieces) : 1, used = (shared + per - 1) / per;
-    const int parts = used + own * WARPS;       // the shared pieces, then warp w of the cluster's CTA c at used + c * WARPS + w
-    if (a.shared_pieces > 0) pdl_wait();        // the shared pieces are there
-    for (int r = rank * WARPS + warp; warp < WARPS && r < p.rows; r += WARPS * own) {
-        int head;
-        const int token = token_of(a, p, r, head);
-        const int64_t first = part_of(a, token, head, 0);
-        float m[EACH], weight[EACH], top = -INFINITY, total = 0.0f;
+template <typename T, int V> __device__ __forceinline__ void store_lane(T* to, const float (&v)[V]) {
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int part = lane + 32 * i;
-            m[i] = -INFINITY;
-            weight[i] = 0.0f;
-            if (part < used) {
-                const float2 v = __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first + part);
-                m[i] = v.x; weight[i] = v.y;
-            } else if (part < parts) {
-                const int c = (part - used) / WARPS, w = (part - used) % WARPS;
-                const float* ml = (own > 1 ? cluster.map_shared_rank(ends.ml, c) : ends.ml) + 2 * (w * OWN + r);
-                m[i] = ml[0]; weight[i] = ml[1];
-            }
-            top = fmaxf(top, m[i]);
-        }
-        top = warp_max(top);
+    for (int e = 0; e < V; ++e) to[e] = from_float<T>(v[e]);
+}
+
+// Every warp has stored its share (the barrier is here): a warp a row, the warps' shares as one piece, or as the result.
+template <typename T, int D, int OWN>
+__device__ __forceinline__ void finish_own(const Attend& a, const Piece& p, const Ends<D, OWN>& ends) {
+    using E = Ends<D, OWN>;
+    constexpr int V = D / 32;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __syncthreads();
+    for (int r = warp; warp < WARPS && r < p.rows; r += WARPS) {
+        float top = -INFINITY, total = 0.0f, sum[V] = {};
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ends.ml[2 * (w * OWN + r)]);
         const float ref = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            m[i] = exp2f(m[i] - ref);
-            total = fmaf(m[i], weight[i], total);
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = exp2f(ends.ml[2 * (w * OWN + r)] - ref);
+            total = fmaf(f, ends.ml[2 * (w * OWN + r) + 1], total);
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[e] = fmaf(f, ends.o[(w * OWN + r) * E::PITCH + lane * V + e], sum[e]);
         }
-        total = warp_sum(total);
-        const float inverse = total == 0.0f ? 0.0f : 1.0f / total;              // no key is seen: zeros
+        int head;
+        const int token = token_of(a, p, r, head);
+        if (a.part_o) {
+            const int64_t part = part_of(a, token, head, p.slot);
+            store_lane(a.part_o + part * D + lane * V, sum);
+            if (lane == 0) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(top, total);
+        } else {
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;          // no key is seen: zeros
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) weight[i] = m[i] * inverse;
-        float sum[V] = {};
-        auto weight_of = [&](int part) {
-            float w = __shfl_sync(0xffffffffu, weight[0], part & 31);
-#pragma unroll
-            for (int i = 1; i < EACH; ++i) {
-                const float other = __shfl_sync(0xffffffffu, weight[i], part & 31);
-                if (part >> 5 == i) w = other;
-            }
-            return w;
-        };
-        const float* from = a.part_o + first * D + lane * V;
-        constexpr int AHEAD = 8;
-        for (int part = 0; part < used; part += AHEAD) {
-            float v[AHEAD][V];
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (part + j >= used) break;
-                load_lane<V>(from + (int64_t)(part + j) * D, v[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                if (part + j >= used) break;
-                const float w = weight_of(part + j);
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum[e] = fmaf(w, v[j][e], sum[e]);
-            }
+            for (int e = 0; e < V; ++e) sum[e] *= inverse;
+            store_lane(reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + lane * V, sum);
         }
-        for (int c = 0; c < own; ++c) {
-            const float* o = (own > 1 ? cluster.map_shared_rank(ends.o, c) : ends.o) + r * E::PITCH + lane * V;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float f = weight_of(used + c * WARPS + w);
-#pragma unroll
-                for (int e = 0; e < V; ++e) sum[e] = fmaf(f, o[w * OWN * E::PITCH + e], sum[e]);
-            }
-        }
-        T* out = reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + lane * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) out[e] = from_float<T>(sum[e]);
-    }
-    if (own > 1) {                              // the others' shared memory is read until here
-        cluster_arrive();
-        cluster_wait();
     }
 }
 
-// a token that is none: zeros
+// The kernels' waits (see the top).
+__device__ __forceinline__ void start_own(const Attend& a) {
+    if (a.shared_pieces == 0) pdl_wait();
+    pdl_launch_dependents();
+}
+__device__ __forceinline__ void end_own(const Attend& a) {
+    if (a.shared_pieces > 0 && blockIdx.x + 1 == gridDim.x) pdl_wait();
+}
+// The rows of a CTA without keys, where nobody joins pieces: zeros.
 template <typename T, int D> __device__ __forceinline__ void store_zeros(const Attend& a, const Piece& p) {
-    if (blockIdx.x % a.own_pieces != 0) return;
+    if (a.part_o) return;
     for (int i = threadIdx.x; i < p.rows * D; i += blockDim.x) {
         int head;
         const int token = token_of(a, p, i / D, head);
@@ -346,11 +285,73 @@ template <typename T, int D> __device__ __forceinline__ void store_zeros(const A
     }
 }
 
-// The kernels' waits (see the top).  attend_own waits at its start where there is no attend_shared before it, else before it
-// reads the shared pieces or ends.
-__device__ __forceinline__ void start_own(const Attend& a) {
-    if (a.shared_pieces == 0) pdl_wait();
+// a warp a row: a token's query head
+template <typename T, int D> __global__ void __launch_bounds__(THREADS) join_kernel(Attend a) {
+    constexpr int V = D / 32, EACH = (MAX_SHARED_PIECES + MAX_OWN_PIECES) / 32, AHEAD = 8;      // values, parts of a lane; pieces in flight
+    const int lane = threadIdx.x & 31;
+    const int64_t at = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
+    const int token = (int)(at / a.num_q), head = (int)(at % a.num_q), slots = a.shared_pieces + a.own_pieces;
+    pdl_wait();
     pdl_launch_dependents();
+    if (token >= a.tokens) return;
+    const int64_t first = part_of(a, token, head, 0);
+    // all slots' m and l, whether they have been written or not, beside what says so
+    float m[EACH], weight[EACH], top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const float2 v = lane + 32 * i < slots ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first + lane + 32 * i) : make_float2(0, 0);
+        m[i] = v.x; weight[i] = v.y;
+    }
+    const Facts f = facts_of(a, token);
+    int shared_used = 0, own_used = 0;
+    if (f.row >= 0) {
+        const int own = f.keys - f.shared;
+        if (f.shared > 0) shared_used = (f.shared - 1) / shared_piece_keys(f.shared, a.shared_pieces) + 1;
+        if (own > 0) own_used = (own - 1) / piece_keys(own, a.own_pieces) + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int slot = lane + 32 * i;
+        const bool used = slot < shared_used || (slot >= a.shared_pieces && slot < a.shared_pieces + own_used);
+        if (!used) { m[i] = -INFINITY; weight[i] = 0.0f; }
+        top = fmaxf(top, m[i]);
+    }
+    top = warp_max(top);
+    const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        m[i] = exp2f(m[i] - ref);
+        total = fmaf(m[i], weight[i], total);
+    }
+    total = warp_sum(total);
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;                  // a token that is none, or sees no key: zeros
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) m[i] *= inverse;
+    float sum[V] = {};
+    const float* from = a.part_o + first * D + lane * V;
+    const int parts = shared_used + own_used, gap = a.shared_pieces - shared_used;
+    for (int part = 0; part < parts; part += AHEAD) {
+        float v[AHEAD][V];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int slot = part + j < shared_used ? part + j : part + j + gap;
+            if (part + j < parts) load_lane<V>(from + (int64_t)slot * D, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int slot = part + j < shared_used ? part + j : part + j + gap;
+            float w = __shfl_sync(0xffffffffu, m[0], slot & 31);
+#pragma unroll
+            for (int i = 1; i < EACH; ++i) {
+                const float other = __shfl_sync(0xffffffffu, m[i], slot & 31);
+                if (slot >> 5 == i) w = other;
+            }
+            if (part + j < parts)
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] = fmaf(w, v[j][e], sum[e]);
+        }
+    }
+    store_lane(reinterpret_cast<T*>(a.out) + token * a.out_stride + head * D + lane * V, sum);
 }
 
 // ------------------------------------------------------------------ bfloat16
@@ -548,7 +549,7 @@ template <int D> __global__ void __launch_bounds__(THREADS) attend_shared_bf16_k
 
 // A token's own keys: up to 16 of its query heads (one tile of the instruction), tiles of 32 keys, eight a warp, in a ring of three.
 template <int D> struct OwnTiles {
-    static constexpr int KEYS = 32, RING = TVB_RING, PITCH = D + 8, TILE = KEYS * PITCH;
+    static constexpr int KEYS = 32, RING = 3, PITCH = D + 8, TILE = KEYS * PITCH;
     static constexpr int RING_BYTES = (16 + 2 * RING * KEYS) * PITCH * 2, END_BYTES = Ends<D, 16>::FLOATS * 4;
     static constexpr int BYTES = (RING_BYTES > END_BYTES ? RING_BYTES : END_BYTES) + 8 * KEYS * 4 + 8 * 4;
     static constexpr int CTAS = D == 64 ? 6 : D == 128 ? 4 : 2;                 // on an SM
@@ -558,16 +559,15 @@ __device__ __forceinline__ void mma_1688(float (&d)[4], uint32_t a0, uint32_t a1
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(b0));
 }
 
-template <int D> __global__ void __launch_bounds__(THREADS, TVB_RING == 3 ? OwnTiles<D>::CTAS : 1) attend_own_bf16_kernel(Attend a) {
+template <int D> __global__ void __launch_bounds__(THREADS, OwnTiles<D>::CTAS) attend_own_bf16_kernel(Attend a) {
     using S = OwnTiles<D>;
     constexpr int PITCH = S::PITCH, WORDS = D / 8;
     extern __shared__ __align__(16) unsigned char raw[];
     start_own(a);
     Piece p;
-    int shared = 0;
-    if (!find_own_piece(a, 16, p, shared)) {
+    if (!find_own_piece(a, 16, p)) {
         store_zeros<bf16, D>(a, p);
-        if (a.shared_pieces > 0) pdl_wait();
+        end_own(a);
         return;
     }
     bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [16][PITCH]
@@ -719,7 +719,8 @@ template <int D> __global__ void __launch_bounds__(THREADS, TVB_RING == 3 ? OwnT
             *reinterpret_cast<float2*>(ends.o + at * Ends<D, 16>::PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         if (t4 == 0) *reinterpret_cast<float2*>(ends.ml + 2 * at) = make_float2(m[h], l[h]);
     }
-    join_pieces<bf16, D, 16>(a, p, shared, ends);
+    finish_own<bf16, D, 16>(a, p, ends);
+    end_own(a);
 }
 
 // ------------------------------------------------------------------- float32
@@ -833,10 +834,9 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
     extern __shared__ __align__(16) unsigned char raw[];
     start_own(a);
     Piece p;
-    int shared = 0;
-    if (!find_own_piece(a, OWN, p, shared)) {
+    if (!find_own_piece(a, OWN, p)) {
         store_zeros<float, D>(a, p);
-        if (a.shared_pieces > 0) pdl_wait();
+        end_own(a);
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -851,19 +851,28 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
         const int token = token_of(a, p, r, head);
         load_lane<V>(reinterpret_cast<const float*>(a.q) + token * a.q_stride + head * D + lane * V, q[r]);
     }
-    for (int key0 = p.range.first + warp; key0 < p.range.end; key0 += AHEAD * WARPS) {
-        float k[AHEAD][V] = {}, v[AHEAD][V] = {};
-        bool there[AHEAD];
+    // The warp's keys are p.range.first + warp + 4 n; a lane looks up where every 32nd of them lies, and those of the next 32 meanwhile.
+    const int mine = max(0, (p.range.end - p.range.first - warp + WARPS - 1) / WARPS);
+    auto place = [&](int n) -> int { return n < mine ? cache_row(a, p, p.range.first + warp + WARPS * n) : -1; };
+    int places = place(lane), next_places = place(lane + 32);
+    float k[2][AHEAD][V], v[2][AHEAD][V];       // of these keys, and of the next
+    uint32_t there[2];
+    auto fetch = [&](int n, int buffer, int from) {                              // from: the places of keys n / 32 * 32 ..
+        there[buffer] = 0;
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
-            const int key = key0 + i * WARPS;
-            const int64_t at = key < p.range.end ? cache_row(a, p, key) : -1;
-            there[i] = at >= 0;
-            if (there[i]) {
-                load_lane<V>(keys + at * D + lane * V, k[i]);
-                load_lane<V>(values + at * D + lane * V, v[i]);
+            const int64_t at = __shfl_sync(0xffffffffu, from, (n + i) & 31);
+            if (at >= 0) {
+                there[buffer] |= 1u << i;
+                load_lane<V>(keys + at * D + lane * V, k[buffer][i]);
+                load_lane<V>(values + at * D + lane * V, v[buffer][i]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) k[buffer][i][e] = v[buffer][i][e] = 0.0f;
             }
         }
+    };
+    auto take = [&](int buffer) {
 #pragma unroll
         for (int r = 0; r < OWN; ++r) {
             if (r >= p.rows) continue;
@@ -872,9 +881,9 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
             for (int i = 0; i < AHEAD; ++i) {
                 float dot = 0.0f;
 #pragma unroll
-                for (int e = 0; e < V; ++e) dot = fmaf(q[r][e], k[i][e], dot);
+                for (int e = 0; e < V; ++e) dot = fmaf(q[r][e], k[buffer][i][e], dot);
                 s[i] = warp_sum(dot) * a.scale_log2;
-                if (!there[i]) s[i] = -INFINITY;
+                if (!(there[buffer] >> i & 1)) s[i] = -INFINITY;
                 now = fmaxf(now, s[i]);
             }
             const float subtract = now == -INFINITY ? 0.0f : now, factor = exp2f(m[r] - subtract);
@@ -887,9 +896,20 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
                 const float w = exp2f(s[i] - subtract);
                 l[r] += w;
 #pragma unroll
-                for (int e = 0; e < V; ++e) o[r][e] = fmaf(w, v[i][e], o[r][e]);
+                for (int e = 0; e < V; ++e) o[r][e] = fmaf(w, v[buffer][i][e], o[r][e]);
             }
         }
+    };
+    fetch(0, 0, places);
+    for (int n = 0; n < mine; n += 2 * AHEAD) {
+        fetch(n + AHEAD, 1, places);            // (AHEAD divides 16: the same 32 keys)
+        take(0);
+        if ((n + 2 * AHEAD) % 32 == 0) {
+            places = next_places;
+            next_places = place(n + 2 * AHEAD + 32 + lane);
+        }
+        fetch(n + 2 * AHEAD, 0, places);
+        take(1);
     }
     const E ends(reinterpret_cast<float*>(raw));
 #pragma unroll
@@ -899,7 +919,8 @@ __global__ void __launch_bounds__(THREADS) attend_own_f32_kernel(Attend a) {
         for (int i = 0; i < V; ++i) ends.o[at * E::PITCH + lane * V + i] = o[r][i];
         if (lane == 0) { ends.ml[2 * at] = m[r]; ends.ml[2 * at + 1] = l[r]; }
     }
-    join_pieces<float, D, OWN>(a, p, shared, ends);
+    finish_own<float, D, OWN>(a, p, ends);
+    end_own(a);
 }
 
 #include "attention_shared_tc.cuh"
@@ -911,57 +932,74 @@ long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 struct Plan {
     long long shared_items, own_items;
     int shared_pieces, own_pieces, own_tiles;
+    int pieces() const { return shared_pieces + own_pieces; }   // of a row; with 1 there is nothing to join
     int tile_tokens;                            // tokens of a tile on the tensor cores of the fifth generation; 0: the other kernels
 };
 
-// Into how many pieces the keys are cut: the shared ones so that the CTAs have one round on the GPU, the tokens' own into about
-// three CTAs an SM; none shorter than MIN_KEYS.
-Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size, int max_shared, int max_own, int dtype) {
+// Into how many pieces the keys are cut, none shorter than MIN_KEYS: the tokens' own for about four CTAs an SM; the shared ones, on the
+// tensor cores, for one CTA on as many SMs as are their share of the work (a block of 128 keys takes a tile 1.2 us, a token's own
+// keys come in at 47 KB a us and SM), half of them at least, so that attend_own's CTAs run on the others meanwhile (60 tokens with up
+// to 431 keys behind 6,144: 39.0 us with all 148, 35.5 with 100, 32.6 with 74; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42, 53, 87).
+Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size, long long max_shared, long long max_own, int dtype) {
     constexpr int MIN_KEYS = 128, SMS = 148;
     const int heads = num_q / num_kv;
     Plan p;
     p.tile_tokens = dtype == TVB_BF16 && tc_takes(head_dim, heads, page_size) ? TC_ROWS / heads : 0;
-    long long tiles = 0;
-    if (groups > 0 && max_shared > 0)
-        tiles = groups + (p.tile_tokens > 0 ? tokens / p.tile_tokens : (long long)tokens * heads / (dtype == TVB_F32 ? 16 : 64));
-    auto pieces_of = [&](long long ctas, long long items, int keys, int most) {
+    // CTAs' tiles: at most, and as a rule
+    long long tiles = 0, usual = 1;
+    // Up to so many values (32 MB of bfloat16) the tokens read the shared keys by themselves, in one launch or two: the third
+    // and the reading in pieces cost more (16 / 8 heads, head size 128, us alone / shared: 2 tokens behind 2,048 keys 9.8 / 13.6, 4 12 /
+    // 13.5, 8 behind 1,024 12.5 / 12.3, 16 behind 512 12.7 / 11.6; float32 8 behind 1,024 25 / 37, 16 behind 512 33 / 36).
+    constexpr long long FEW_VALUES = 1ll << 23;
+    const bool alone = (long long)tokens * num_kv * head_dim * max_shared <= FEW_VALUES;
+    if (alone) max_own += max_shared;
+    if (groups > 0 && max_shared > 0 && !alone) {
+        const long long in_tile = p.tile_tokens > 0 ? p.tile_tokens * heads : dtype == TVB_F32 ? 16 : 64;
+        tiles = groups + (long long)tokens * heads / in_tile;
+        usual = max((long long)groups, ceil_div((long long)tokens * heads, in_tile));
+    }
+    auto pieces_of = [&](long long ctas, long long items, long long keys, int most) {
         const long long wanted = items > 0 ? max(1ll, ctas / items) : 1;
-        return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1), MIN_KEYS)), (long long)most));
+        return (int)max(1ll, min(min(wanted, ceil_div(max(keys, 1ll), MIN_KEYS)), (long long)most));
     };
     p.own_tiles = (int)ceil_div(heads, dtype == TVB_F32 ? 4 : 16);
-    p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? SMS : 3 * SMS, tiles * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
-    p.own_pieces = pieces_of(TVB_CTAS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
+    const double own_us = (double)tokens * num_kv * max_own * head_dim * (dtype == TVB_F32 ? 8 : 4) / 47e3;
+    const double shared_us = 1.2 * usual * num_kv * (max_shared / 128.0);
+    const int share = max(SMS / 2, (int)(SMS * shared_us / (shared_us + own_us + 1e-9)));
+    p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? share : 3 * SMS, usual * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
+    p.own_pieces = pieces_of(4 * SMS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
+    if (tiles == 0 && dtype == TVB_BF16 && max_own <= 2 * MIN_KEYS) p.own_pieces = 1;            // not worth the launch that joins them
     p.shared_items = tiles * num_kv * p.shared_pieces;
     p.own_items = (long long)tokens * num_kv * p.own_tiles * p.own_pieces;
     return p;
 }
 
-template <typename K> int launch(K kernel, long long grid, size_t shared, int pdl, int cluster, cudaStream_t stream, const Attend& a) {
+template <typename K> int launch(K kernel, long long grid, size_t shared, int pdl, cudaStream_t stream, const Attend& a) {
     if (shared > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
         if (e != cudaSuccess) return (int)e;
     }
-    TvbLaunch at(dim3((unsigned)grid), dim3(THREADS), shared, stream, pdl, cluster);
+    TvbLaunch at(dim3((unsigned)grid), dim3(THREADS), shared, stream, pdl);
     const cudaError_t e = cudaLaunchKernelEx(&at.config, kernel, a);
     return e == cudaSuccess ? tvb_last_error() : (int)e;
 }
 
+template <int D> int launch_shared(const Attend& a, const Plan& p, int dtype, int pdl, cudaStream_t s) {
+    if (dtype == TVB_F32)
+        return launch(attend_shared_f32_kernel<D>, p.shared_items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, s, a);
+    if constexpr (D <= 128)
+        if (p.tile_tokens > 0) return launch_shared_tc<D>(a, p.shared_items, p.tile_tokens, pdl, s);
+    return launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, s, a);
+}
 template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int pdl, cudaStream_t s) {
-    const int cluster = p.own_pieces > 1 ? p.own_pieces : 0;
-    if (dtype == TVB_F32) {
-        const int e = p.shared_items == 0 ? 0 : launch(attend_shared_f32_kernel<D>, p.shared_items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, 0, s, a);
-        return e ? e : launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, cluster, s, a);
-    }
-    int e = 0;
-    if (p.shared_items > 0) {
-        if constexpr (D <= 128) {
-            if (p.tile_tokens > 0) e = launch_shared_tc<D>(a, p.shared_items, p.tile_tokens, pdl, s);
-            else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
-        } else e = launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, 0, s, a);
-    }
+    int e = p.shared_items > 0 ? launch_shared<D>(a, p, dtype, pdl, s) : 0;
     if (e) return e;
-    if (own_tma_takes(a.page_size)) return launch_own_tma<D>(a, p.own_items, cluster, pdl, s);
-    return launch(attend_own_bf16_kernel<D>, p.own_items, OwnTiles<D>::BYTES, pdl, cluster, s, a);
+    if (dtype == TVB_F32) e = launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, s, a);
+    else if (own_tma_takes(a.page_size)) e = launch_own_tma<D>(a, p.own_items, pdl, s);
+    else e = launch(attend_own_bf16_kernel<D>, p.own_items, OwnTiles<D>::BYTES, pdl, s, a);
+    if (e || !a.part_o) return e;
+    const long long joins = ceil_div((long long)a.tokens * a.num_q, WARPS);
+    return dtype == TVB_F32 ? launch(join_kernel<float, D>, joins, 0, pdl, s, a) : launch(join_kernel<bf16, D>, joins, 0, pdl, s, a);
 }
 
 }  // namespace
@@ -972,8 +1010,8 @@ extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int nu
     *launches = 0;
     if (tokens <= 0 || num_kv <= 0) return 0;
     const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
-    *launches = p.shared_items > 0 ? 2 : 1;
-    return (long long)tokens * num_q * p.shared_pieces * (head_dim + 2);
+    *launches = p.pieces() > 1 ? 2 + (p.shared_items > 0) : 1;
+    return p.pieces() > 1 ? (long long)tokens * num_q * p.pieces() * (head_dim + 2) : 0;
 }
 
 // 0, or which bounded wait gave up in some launch since the last call; reading clears it.  Synchronises.
@@ -996,9 +1034,9 @@ extern "C" int tvb_attention_shared(const void* q, long long q_stride, const voi
         return TVB_BAD_ARGUMENT;
     const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
     if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
-    Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, scratch, nullptr, out, out_stride,
+    Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, p.pieces() > 1 ? scratch : nullptr, nullptr, out, out_stride,
              tokens, rows, width, groups, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, scale * LOG2E};
-    a.part_ml = scratch + (long long)tokens * num_q * p.shared_pieces * head_dim;
+    a.part_ml = scratch + (long long)tokens * num_q * p.pieces() * head_dim;
     cudaStream_t s = (cudaStream_t)stream;
     if (head_dim == 64) return launch_all<64>(a, p, dtype, pdl, s);
     if (head_dim == 128) return launch_all<128>(a, p, dtype, pdl, s);

@@ -23,12 +23,12 @@ constexpr uint32_t TC_COLUMNS = 512;
 
 template <int HD> struct TcShared {
     static constexpr int TILE = HD / 64 * TC_HALF;                              // a Q, K or V tile
-    static constexpr int K_RING = 2, V_RING = 2;                                 // (leaves room for a CTA of attend_own beside)
-    static constexpr int EXCHANGE = TC_ROWS * 2 * 4 + TC_ROWS * 8;              // [row][reference, denominator] of the second group; [row] place of the result
+    // A tile takes 2,500 cycles to come in beside what else the GPU reads, a block's products and softmax 2,000.
+    static constexpr int K_RING = 3, V_RING = 3;
     static constexpr int Q_FULL = 0, K_FULL = 1, K_EMPTY = K_FULL + K_RING, V_FULL = K_EMPTY + K_RING, V_EMPTY = V_FULL + V_RING,
                          S_FULL = V_EMPTY + V_RING, P_FULL = S_FULL + 2,
                          P_READ = P_FULL + 2, O_LAST = P_READ + 2, SECOND_DONE = O_LAST + 2, BARRIERS = SECOND_DONE + 1;
-    static constexpr int BYTES = TILE * (1 + K_RING + V_RING) + EXCHANGE + BARRIERS * 8 + 16 + 1024;
+    static constexpr int BYTES = TILE * (1 + K_RING + V_RING) + BARRIERS * 8 + 16 + 1024;
 };
 
 __device__ int tvb_attention_shared_status_word = 0;
@@ -43,10 +43,12 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     const uint32_t base = (smem_address(raw_tc) + 1023u) & ~1023u;
     uint8_t* aligned = raw_tc + (base - smem_address(raw_tc));
     const uint32_t q_at = base, kv_at = base + T::TILE;
-    float* exchange = reinterpret_cast<float*>(aligned + T::TILE * (1 + T::K_RING + T::V_RING));
-    const uint32_t bars = base + T::TILE * (1 + T::K_RING + T::V_RING) + T::EXCHANGE;
+    // over the first Q tile, when it has been multiplied for the last time: [row][reference, denominator] of the second group, then
+    // [row] place of the result
+    float* exchange = reinterpret_cast<float*>(aligned);
+    const uint32_t bars = base + T::TILE * (1 + T::K_RING + T::V_RING);
     auto bar = [&](int i) { return bars + 8u * i; };
-    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + T::TILE * (1 + T::K_RING + T::V_RING) + T::EXCHANGE + T::BARRIERS * 8);
+    uint32_t* tmem_base_slot = reinterpret_cast<uint32_t*>(aligned + T::TILE * (1 + T::K_RING + T::V_RING) + T::BARRIERS * 8);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_base_slot + 1);
     int* status = &tvb_attention_shared_status_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -64,7 +66,8 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
     pdl_wait();
     pdl_launch_dependents();
     Piece p;
-    const bool found = find_shared_piece(a, tile_tokens * heads, p);            // the same for the whole CTA
+    const int tile_rows = tile_tokens * heads;
+    const bool found = find_shared_piece(a, tile_rows, p);                      // the same for the whole CTA
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
@@ -90,7 +93,7 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         const CUtensorMap* map = of_k ? &map_k : &map_v;
         int page = page_of(0), next_page = page_of(1);
         if (of_k && lane == 0) {
-            mbar_arrive_expect(bar(T::Q_FULL), (uint32_t)(tile_tokens * heads * HD * 2));
+            mbar_arrive_expect(bar(T::Q_FULL), (uint32_t)(tile_rows * HD * 2));
 #pragma unroll
             for (int h = 0; h < HD / 64; ++h)
                 tma_load_3d(q_at + h * TC_HALF, &map_q, 64 * h, p.kv_head * heads, p.token0 + p.row0 / heads, bar(T::Q_FULL));
@@ -162,7 +165,7 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
                 for (int kk = 0; kk < TC_KEYS / 16; ++kk)
                     // 16 keys: 8 columns of P (two bfloat16 a column), two 1024-byte atoms of V
                     tc_mma_a_in_tmem(tmem_base + 2 * TC_KEYS + b * HD, tmem_base + b * TC_KEYS + kk * 8,
-                                     tile_descriptor_mn_major(v_tile + kk * 2048, TC_HALF), idesc, !(j < 2 && kk == 0));
+                                     tile_descriptor_mn_major(v_tile + kk * 2048, TC_HALF), idesc, !(n == 0 && kk == 0));
                 tc_commit(bar(T::V_EMPTY + slot));
                 tc_commit(bar(T::P_READ + b));
                 if (j + 2 >= blocks) tc_commit(bar(T::O_LAST + b));
@@ -259,51 +262,54 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             tc_fence_before_sync();
             warp_arrive(T::P_FULL + group);
         }
-        const bool second = blocks > 1;         // else the second group had no block, and its O holds nothing
-        if (alive && (group == 0 || second)) alive = warp_wait(T::O_LAST + group, 0, 13);
-        int64_t* places = reinterpret_cast<int64_t*>(exchange + TC_ROWS * 2);
-        // The rows' O goes out through shared memory (that of the tiles, which are all consumed), so that a warp stores whole rows;
-        // 16-byte word w of row r lies in place w ^ (r % 32, or % 16 for 64 values).
+        // ---- the rows' results.  O goes out through shared memory (that of the keys and values, of which all are consumed), so that a
+        // warp stores whole rows; 16-byte word w of row r lies in place w ^ (r % 32, or % 16 for 64 values).
         constexpr int WORDS = HD / 4;
+        const bool second = blocks > 1;         // else the second group had no block, and its O holds nothing
+        int64_t* places = reinterpret_cast<int64_t*>(exchange + TC_ROWS * 2);
         uint4* staged = reinterpret_cast<uint4*>(aligned + T::TILE);
-        if (alive && group == 1) {
+        static_assert(TC_ROWS * HD * 4 <= (T::K_RING + T::V_RING) * T::TILE, "room for the results");
+        if (alive) alive = warp_wait(T::O_LAST, 0, 13);
+        if (alive && second) alive = warp_wait(T::O_LAST + 1, 0, 13);
+        if (group == 1) {
             exchange[row * 2] = reference;
             exchange[row * 2 + 1] = l;
             tc_fence_before_sync();
-            warp_arrive(T::SECOND_DONE);
-        } else if (alive && (alive = warp_wait(T::SECOND_DONE, 0, 17))) {
+            if (alive) warp_arrive(T::SECOND_DONE);
+        } else {
+            if (alive) alive = warp_wait(T::SECOND_DONE, 0, 17);
             tc_fence_after_sync();
-            const float other = exchange[row * 2], other_l = exchange[row * 2 + 1], top = fmaxf(reference, other);
+            const float other = alive ? exchange[row * 2] : -INFINITY, other_l = alive ? exchange[row * 2 + 1] : 0.0f;
+            const float top = fmaxf(reference, other);
             const float mine = reference == -INFINITY ? 0.0f : exp2_unit(reference - top);
             const float theirs = other == -INFINITY ? 0.0f : exp2_unit(other - top);
+            const bool here = alive && row < p.rows;
             int head = 0;
-            const int token = row < p.rows ? token_of(a, p, row, head) : 0;
-            const bool takes = row < p.rows && takes_part(a, p, token);
+            const int token = here ? token_of(a, p, row, head) : 0;
+            const bool takes = here && takes_part(a, p, token);
             const int64_t at = takes ? part_of(a, token, head, p.slot) : -1;
             places[row] = at;
             if (takes) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, l * mine + other_l * theirs);
+            if (alive)
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-                uint32_t x[32], y[32];
-                tmem_load_32(lane_address + 2 * TC_KEYS + c, x);
-                if (second) tmem_load_32(lane_address + 2 * TC_KEYS + HD + c, y);
-                tmem_load_wait();
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t x[32], y[32];
+                    tmem_load_32(o_address + c, x);
+                    if (second) tmem_load_32(o_address + HD + c, y);
+                    tmem_load_wait();
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    float f = __uint_as_float(x[e]) * mine;
-                    if (second) f = fmaf(__uint_as_float(y[e]), theirs, f);
-                    x[e] = __float_as_uint(f);
+                    for (int e = 0; e < 32; ++e) {
+                        float f = __uint_as_float(x[e]) * mine;
+                        if (second) f = fmaf(__uint_as_float(y[e]), theirs, f);
+                        x[e] = __float_as_uint(f);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        staged[row * WORDS + (((c + e) / 4) ^ (row % WORDS))] = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
                 }
-#pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    staged[row * WORDS + (((c + e) / 4) ^ (row % WORDS))] = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
-            }
-        } else if (group == 0) {
-            places[row] = -1;                   // a wait ran out
         }
         asm volatile("bar.sync 1, 256;\n" ::: "memory");                        // the softmax warps
-        const int w8 = warp - 2;
-        for (int r = w8; r < TC_ROWS; r += 8) {
+        for (int r = warp - 2; r < TC_ROWS; r += 8) {
             const int64_t at = places[r];
             if (at >= 0 && lane < WORDS) *reinterpret_cast<uint4*>(a.part_o + at * HD + lane * 4) = staged[r * WORDS + (lane ^ (r % WORDS))];
         }

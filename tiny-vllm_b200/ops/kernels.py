@@ -2155,7 +2155,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     ``shared_lens[g]`` (int32 [groups]) positions hold the same keys and values for all of them, which are read once, through
     the table of the group's first token that reaches them all.  A token that ends before them, or stands in no group, reads
     its keys by itself.  ``max_shared`` and ``max_own``: no group shares more, no token has more keys behind its group's;
-    by them the work is cut up, the result does not depend on them beyond rounding (default: what the tables hold).  A key
+    by them the work is cut up (and groups whose keys are few are not read together at all), the result does not depend on
+    them beyond rounding (default: what the tables hold).  A key
     whose page is no page of the cache is not seen.  bfloat16 and float32, head sizes 64, 128 and 256."""
     tokens = positions.shape[0] if positions.dim() == 1 else -1
     tag = dtype_tag(q.dtype)
@@ -2179,10 +2180,10 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
             or tokens > 0 and q.untyped_storage().nbytes() < (q.storage_offset() + (tokens - 1) * q_token_stride + width) * size:
         raise KernelError("attention_shared: the heads of token t stand at q + t * q_token_stride, on 16 bytes, inside its memory")
     held = block_tables.shape[1] * key_cache.shape[2]
-    max_shared = held if max_shared is None else min(max_shared, held)
-    max_own = held if max_own is None else min(max_own, held)
-    if max_shared < 0 or max_own < 0:
-        raise KernelError("attention_shared: max_shared and max_own are not negative")
+    max_shared = held if max_shared is None else max_shared
+    max_own = held if max_own is None else max_own
+    if not 0 <= max_shared < 2**31 or not 0 <= max_own < 2**31:
+        raise KernelError("attention_shared: max_shared and max_own are not negative and have 31 bits")
     if not 0.0 < scale < float("inf"):
         raise KernelError("attention_shared: the scale is positive and finite")
     if out is None:
