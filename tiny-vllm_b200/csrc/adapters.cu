@@ -93,6 +93,12 @@ template <int ROWS> __device__ __forceinline__ int find_adapters(const int* all,
     }
     if (tid < 2) counts[tid] = 0;
     __syncthreads();
+    // as a rule all rows have one
+    if (__syncthreads_and(tid >= ROWS || ids[tid] == ids[0])) {
+        if (tid == 0) distinct[0] = ids[0];
+        __syncthreads();
+        return ids[0] >= 0 ? 1 : 0;
+    }
     bool first = false;
     uint32_t firsts = 0;
     if (tid < 64) {                             // whole warps
@@ -294,88 +300,118 @@ struct Expand {
     void* y;
     int64_t ldy;
     int m, n, rank, adapters;
+    int columns_apart;
 };
 
-// A tile of 16 MT rows and 128 columns of y, 32 columns a warp, one adapter after another.  The columns of an n-tile are
-// spread so that a thread holds eight neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.
-template <int MT, typename Y, bool WIDE>
-__global__ void __launch_bounds__(THREADS) expand_kernel(Expand s) {
-    constexpr int ROWS = 16 * MT, NT = 4, STEPS = 4;                            // steps of 16 ranks whose B is held
-    __shared__ int ids[ROWS], distinct[ROWS];
+// A warp has 16 rows of y and walks over tiles of 32 columns, one adapter of its rows after another (those of few rows side by side
+// in the grid): the rows' u stays in registers, y and B of the next tile are asked for before this one's products.  The columns of an
+// n-tile are spread so that a thread holds eight neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.  The warps of
+// a CTA have different columns of the same rows (`columns_apart`, few rows), or different rows and the same columns, whose B they find
+// in L1.
+template <typename Y, bool WIDE>
+__global__ void __launch_bounds__(THREADS, sizeof(Y) == 2 ? 4 : 3) expand_kernel(Expand s) {
+    constexpr int NT = 4, STEPS = 4, WORDS = sizeof(Y) / 2;                     // steps of 16 ranks held; 16-byte words of eight values of y
     const int padded = padded_rank(s.rank);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = blockIdx.y * ROWS, n0 = blockIdx.x * 128 + warp * 32, column = n0 + 8 * t;
-    const bf16* u = reinterpret_cast<const bf16*>(s.u);
-    const bool whole = WIDE && column + 8 <= s.n;
+    const int row0 = (s.columns_apart ? blockIdx.y : blockIdx.y * WARPS + warp) * 16;
+    const int first_tile = s.columns_apart ? blockIdx.x * WARPS + warp : blockIdx.x;
+    const int step = s.columns_apart ? gridDim.x * WARPS : gridDim.x, tiles = (s.n + 31) / 32;
     pdl_wait();
     pdl_launch_dependents();
-    const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
-    for (int d = blockIdx.z; d < count; d += gridDim.z) {
-        const int adapter = distinct[d];
+    if (row0 >= s.m || first_tile >= tiles) return;
+    int id = -1;
+    if (lane < 16 && row0 + lane < s.m) {
+        id = s.ids[row0 + lane];
+        if ((unsigned)id >= (unsigned)s.adapters) id = -1;
+    }
+    const uint32_t alike = __match_any_sync(0xffffffffu, id);
+    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
+    for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
+    while (leaders) {
+        const int leader = __ffs(leaders) - 1;
+        for (int d = 0; d < (int)gridDim.z; ++d) leaders &= leaders - 1;
+        const int adapter = __shfl_sync(0xffffffffu, id, leader);
+        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader);
+        const bool mine[2] = {(rows >> g & 1) != 0, (rows >> (g + 8) & 1) != 0};
         const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
-        bool mine[MT][2];
-        uint4 old[MT][2][sizeof(Y) / 2];                                        // of y, asked for first
+        const bf16* u = reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + g) * 2 * padded + 4 * t;
+        Y* y[2] = {reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g) * s.ldy + 8 * t, reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g + 8) * s.ldy + 8 * t};
+        uint2 held[STEPS][4];                   // u of rows g and g + 8, its heads and its rests
+        auto load_u = [&](int r0) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = 16 * i + g + 8 * half;
-                mine[i][half] = ids[row] == adapter;
-                if (mine[i][half] && whole) {
-                    const uint4* y = reinterpret_cast<const uint4*>(reinterpret_cast<const Y*>(s.y) + (int64_t)(row0 + row) * s.ldy + column);
-#pragma unroll
-                    for (int q = 0; q < (int)sizeof(Y) / 2; ++q) old[i][half][q] = y[q];
+                for (int q = 0; q < 4; ++q) {
+                    const bool there = mine[q & 1] && r0 + 16 * k < padded;
+                    held[k][q] = there ? *reinterpret_cast<const uint2*>(u + ((q & 1) * 16 + (q >> 1)) * padded + r0 + 16 * k) : make_uint2(0, 0);
                 }
-            }
-        float sums[MT][NT][4] = {};
-        for (int r0 = 0; r0 < padded; r0 += 16 * STEPS) {
-            uint2 w[STEPS][NT];
+        };
+        uint4 old[2][WORDS];                    // of y
+        auto load_y = [&](int tile) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                if (WIDE && mine[half] && tile * 32 + 8 * t + 8 <= s.n)
+#pragma unroll
+                    for (int q = 0; q < WORDS; ++q) old[half][q] = reinterpret_cast<const uint4*>(y[half] + tile * 32)[q];
+        };
+        uint2 w[STEPS][NT];
+        auto load_b = [&](int tile, int r0) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const int at = n0 + (g >> 1) * 8 + 2 * j + (g & 1);
+                    const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
                     w[k][j] = load_4<WIDE>(b + (int64_t)at * s.rank, r0 + 16 * k + 4 * t, s.rank, at < s.n);
                 }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
+        };
+        load_y(first_tile);
+        load_b(first_tile, 0);
+        load_u(0);
+        for (int tile = first_tile; tile < tiles; tile += step) {
+            float sums[NT][4] = {};
+            for (int r0 = 0; r0 < padded; r0 += 16 * STEPS) {
+                if (padded > 16 * STEPS && (r0 > 0 || tile != first_tile)) {
+                    load_u(r0);
+                    if (r0 > 0) load_b(tile, r0);
+                }
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
                     if (r0 + 16 * k >= padded) break;
-                    const bf16* at = u + ((int64_t)(row0 + 16 * i + g) * 2) * padded + r0 + 16 * k + 4 * t;
-                    const uint2 none = make_uint2(0, 0);
-                    const uint2 hl = mine[i][0] ? *reinterpret_cast<const uint2*>(at) : none;
-                    const uint2 ll = mine[i][0] ? *reinterpret_cast<const uint2*>(at + padded) : none;
-                    const uint2 hh = mine[i][1] ? *reinterpret_cast<const uint2*>(at + 16 * padded) : none;
-                    const uint2 lh = mine[i][1] ? *reinterpret_cast<const uint2*>(at + 17 * padded) : none;
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        mma_16816(sums[i][j], hl.x, hh.x, hl.y, hh.y, w[k][j].x, w[k][j].y);
-                        mma_16816(sums[i][j], ll.x, lh.x, ll.y, lh.y, w[k][j].x, w[k][j].y);
+                        mma_16816(sums[j], held[k][0].x, held[k][1].x, held[k][0].y, held[k][1].y, w[k][j].x, w[k][j].y);
+                        mma_16816(sums[j], held[k][2].x, held[k][3].x, held[k][2].y, held[k][3].y, w[k][j].x, w[k][j].y);
                     }
                 }
-        }
+            }
+            uint4 now[2][WORDS];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int q = 0; q < WORDS; ++q) now[half][q] = old[half][q];
+            if (tile + step < tiles) {
+                load_y(tile + step);
+                load_b(tile + step, 0);
+            }
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                if (!mine[i][half]) continue;
-                Y* y = reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + 16 * i + g + 8 * half) * s.ldy + column;
+                if (!mine[half]) continue;
+                Y* to = y[half] + tile * 32;
                 float add[8];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[i][j][2 * half]; add[2 * j + 1] = sums[i][j][2 * half + 1]; }
-                if (whole) {
+                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * half]; add[2 * j + 1] = sums[j][2 * half + 1]; }
+                if (WIDE && tile * 32 + 8 * t + 8 <= s.n) {
                     if constexpr (sizeof(Y) == 2) {
                         float v[8];
-                        unpack_bf16x8(old[i][half][0], v);
+                        unpack_bf16x8(now[half][0], v);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) add[e] += v[e];
-                        *reinterpret_cast<uint4*>(y) = pack_bf16x8(add);
+                        *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
                     } else {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            const uint4 v = old[i][half][q];
-                            reinterpret_cast<float4*>(y)[q] =
+                            const uint4 v = now[half][q];
+                            reinterpret_cast<float4*>(to)[q] =
                                 make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
                                             __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
                         }
@@ -383,9 +419,10 @@ __global__ void __launch_bounds__(THREADS) expand_kernel(Expand s) {
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
-                        if (column + e < s.n) y[e] = from_float<Y>(to_float<Y>(y[e]) + add[e]);
+                        if (tile * 32 + 8 * t + e < s.n) to[e] = from_float<Y>(to_float<Y>(to[e]) + add[e]);
                 }
             }
+        }
     }
 }
 
@@ -499,9 +536,12 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
                 : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-template <int MT, typename Y> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
-    const dim3 grid(ceil_div(a.n, 128), ceil_div(a.m, 16 * MT), side_by_side);
-    return wide ? launch(expand_kernel<MT, Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<MT, Y, false>, grid, 0, 0, pdl, s, a);
+template <typename Y> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
+    // few rows: a tile of 32 columns a warp; more: enough CTAs for about four an SM, which walk over the columns
+    const int tiles = ceil_div(a.n, 32), rows = ceil_div(a.m, a.columns_apart ? 16 : 16 * WARPS);
+    const int across = a.columns_apart ? ceil_div(tiles, WARPS) : min(tiles, max(1, 4 * 148 / rows));
+    const dim3 grid(across, rows, side_by_side);
+    return wide ? launch(expand_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<Y, false>, grid, 0, 0, pdl, s, a);
 }
 
 }  // namespace
@@ -539,9 +579,9 @@ extern "C" int tvb_adapters_shrink(const void* x, long long ldx, const void* dow
         const dim3 grid(a.splits * ceil_div(rank, 16), ceil_div(m, 16), min(min(16, m), adapters));
         return wide ? launch(shrink_few_kernel<true>, grid, 0, a.splits, pdl, s, a) : launch(shrink_few_kernel<false>, grid, 0, a.splits, pdl, s, a);
     }
-    // as many pieces of k as give every SM two CTAs
+    // pieces of k while the CTAs still have one round on the GPU (three an SM)
     const int chunks = rank <= 16 ? 1 : ceil_div(rank, 64), stages = ceil_div(k, STAGE_K);
-    while (a.splits < MAX_SPLITS && a.splits * 4 <= stages && ceil_div(m, 64) * chunks * a.splits < 2 * 148) a.splits *= 2;
+    while (a.splits < MAX_SPLITS && a.splits * 4 <= stages && (long long)ceil_div(m, 64) * chunks * a.splits * 2 <= 3 * 148) a.splits *= 2;
     a.per_split = ceil_div(stages, a.splits);
     return rank <= 16 ? launch_many<16>(a, chunks, wide, pdl, s) : launch_many<64>(a, chunks, wide, pdl, s);
 }
@@ -552,7 +592,8 @@ extern "C" int tvb_adapters_expand(const void* u, const void* up, const int* ids
     if (m <= 0 || n <= 0 || adapters <= 0) return 0;
     if (rank <= 0 || rank > MAX_RANK || ceil_div(m, 16) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters};
+    const bool few = m <= FEW_ROWS;
+    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters, few};
     if (dtype == TVB_F32) {
         if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
         const dim3 grid(ceil_div(n, THREADS), ceil_div(m, 16));
@@ -563,10 +604,7 @@ extern "C" int tvb_adapters_expand(const void* u, const void* up, const int* ids
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const int size = y_dtype == TVB_F32 ? 4 : 2;
     const bool wide = rank % 4 == 0 && !((uintptr_t)up & 7) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
-    const bool few = m <= FEW_ROWS;
     const int side_by_side = few ? min(min(16, m), adapters) : 1;
-    if (y_dtype == TVB_F32)
-        return few ? launch_expand<1, float>(a, wide, side_by_side, pdl, s) : launch_expand<4, float>(a, wide, side_by_side, pdl, s);
-    if (y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    return few ? launch_expand<1, bf16>(a, wide, side_by_side, pdl, s) : launch_expand<4, bf16>(a, wide, side_by_side, pdl, s);
+    if (y_dtype == TVB_F32) return launch_expand<float>(a, wide, side_by_side, pdl, s);
+    return y_dtype == TVB_BF16 ? launch_expand<bf16>(a, wide, side_by_side, pdl, s) : TVB_BAD_ARGUMENT;
 }
