@@ -45,17 +45,6 @@ template <bool WIDE> __device__ __forceinline__ uint4 load_8(const bf16* row, in
         return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
-template <bool WIDE> __device__ __forceinline__ uint2 load_4(const bf16* row, int at, int size, bool there) {
-    if constexpr (WIDE) {                       // size is a multiple of 4, the row lies on 8 bytes
-        return there && at < size ? *reinterpret_cast<const uint2*>(row + at) : make_uint2(0, 0);
-    } else {
-        uint32_t h[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) h[e] = there && at + e < size ? (uint32_t)reinterpret_cast<const unsigned short*>(row)[at + e] : 0u;
-        return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
-    }
-}
-
 __device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_address(p)) : "memory");
@@ -303,24 +292,25 @@ struct Expand {
     int columns_apart;
 };
 
-// A warp has 16 rows of y and walks over tiles of 32 columns, one adapter of its rows after another (those of few rows side by side
-// in the grid): the rows' u stays in registers, y and B of the next tile are asked for before this one's products.  The columns of an
-// n-tile are spread so that a thread holds eight neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.  The warps of
-// a CTA have different columns of the same rows (`columns_apart`, few rows), or different rows and the same columns, whose B they find
-// in L1.
+// A warp has 16 rows of y and walks over tiles of 32 columns, one adapter of its rows after another (those of few rows side by
+// side in the grid): the rows' u stays in registers, y and B of the next tile are asked for before this one's products.  A thread
+// takes 16 bytes, eight neighbouring ranks, of a row of B and of u (which rank a fragment's place stands for is permuted alike in
+// both).  The columns of an n-tile are spread so that a thread holds eight neighbours of y: place c of tile j is column
+// (c / 2) * 8 + 2 j + c % 2.  The warps of a CTA have different columns of the same rows (`columns_apart`, few rows), or different
+// rows and the same columns, whose B they find in L1.
 template <typename Y, bool WIDE>
-__global__ void __launch_bounds__(THREADS, sizeof(Y) == 2 ? 4 : 3) expand_kernel(Expand s) {
-    constexpr int NT = 4, STEPS = 4, WORDS = sizeof(Y) / 2;                     // steps of 16 ranks held; 16-byte words of eight values of y
+__global__ void __launch_bounds__(THREADS, 4) expand_kernel(Expand s) {
+    constexpr int ROWS = 16, NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;     // steps of 32 ranks held; 16-byte words of eight values of y
     const int padded = padded_rank(s.rank);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = (s.columns_apart ? blockIdx.y : blockIdx.y * WARPS + warp) * 16;
+    const int row0 = (s.columns_apart ? blockIdx.y : blockIdx.y * WARPS + warp) * ROWS;
     const int first_tile = s.columns_apart ? blockIdx.x * WARPS + warp : blockIdx.x;
     const int step = s.columns_apart ? gridDim.x * WARPS : gridDim.x, tiles = (s.n + 31) / 32;
     pdl_wait();
     pdl_launch_dependents();
     if (row0 >= s.m || first_tile >= tiles) return;
     int id = -1;
-    if (lane < 16 && row0 + lane < s.m) {
+    if (lane < ROWS && row0 + lane < s.m) {
         id = s.ids[row0 + lane];
         if ((unsigned)id >= (unsigned)s.adapters) id = -1;
     }
@@ -331,37 +321,39 @@ __global__ void __launch_bounds__(THREADS, sizeof(Y) == 2 ? 4 : 3) expand_kernel
         const int leader = __ffs(leaders) - 1;
         for (int d = 0; d < (int)gridDim.z; ++d) leaders &= leaders - 1;
         const int adapter = __shfl_sync(0xffffffffu, id, leader);
-        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader);
-        const bool mine[2] = {(rows >> g & 1) != 0, (rows >> (g + 8) & 1) != 0};
+        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader) >> g;     // bit 8 h: row g + 8 h is this adapter's
         const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
-        const bf16* u = reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + g) * 2 * padded + 4 * t;
-        Y* y[2] = {reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g) * s.ldy + 8 * t, reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g + 8) * s.ldy + 8 * t};
-        uint2 held[STEPS][4];                   // u of rows g and g + 8, its heads and its rests
+        const bf16* u = reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + g) * 2 * padded;
+        Y* y = reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g) * s.ldy + 8 * t;
+        uint4 held[STEPS][2][2];           // u of rows g + 8 h, its heads and its rests
         auto load_u = [&](int r0) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const bool there = mine[q & 1] && r0 + 16 * k < padded;
-                    held[k][q] = there ? *reinterpret_cast<const uint2*>(u + ((q & 1) * 16 + (q >> 1)) * padded + r0 + 16 * k) : make_uint2(0, 0);
-                }
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int at = r0 + 32 * k + 8 * t;
+                        held[k][h][q] = rows >> (8 * h) & 1 && at < padded ? *reinterpret_cast<const uint4*>(u + (int64_t)(16 * h + q) * padded + at)
+                                                                          : make_uint4(0, 0, 0, 0);
+                    }
         };
-        uint4 old[2][WORDS];                    // of y
+        uint4 old[2][WORDS];               // of y
         auto load_y = [&](int tile) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
-                if (WIDE && mine[half] && tile * 32 + 8 * t + 8 <= s.n)
+            for (int h = 0; h < 2; ++h)
+                if (WIDE && rows >> (8 * h) & 1 && tile * 32 + 8 * t + 8 <= s.n)
 #pragma unroll
-                    for (int q = 0; q < WORDS; ++q) old[half][q] = reinterpret_cast<const uint4*>(y[half] + tile * 32)[q];
+                    for (int q = 0; q < WORDS; ++q) old[h][q] = reinterpret_cast<const uint4*>(y + 8 * h * s.ldy + tile * 32)[q];
         };
-        uint2 w[STEPS][NT];
+        uint4 w[STEPS][NT];
         auto load_b = [&](int tile, int r0) {
 #pragma unroll
             for (int k = 0; k < STEPS; ++k)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-                    w[k][j] = load_4<WIDE>(b + (int64_t)at * s.rank, r0 + 16 * k + 4 * t, s.rank, at < s.n);
+                    w[k][j] = load_8<WIDE>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
                 }
         };
         load_y(first_tile);
@@ -369,48 +361,52 @@ __global__ void __launch_bounds__(THREADS, sizeof(Y) == 2 ? 4 : 3) expand_kernel
         load_u(0);
         for (int tile = first_tile; tile < tiles; tile += step) {
             float sums[NT][4] = {};
-            for (int r0 = 0; r0 < padded; r0 += 16 * STEPS) {
-                if (padded > 16 * STEPS && (r0 > 0 || tile != first_tile)) {
+            for (int r0 = 0; r0 < padded; r0 += 32 * STEPS) {
+                if (padded > 32 * STEPS && (r0 > 0 || tile != first_tile)) {
                     load_u(r0);
                     if (r0 > 0) load_b(tile, r0);
                 }
 #pragma unroll
                 for (int k = 0; k < STEPS; ++k) {
-                    if (r0 + 16 * k >= padded) break;
+                    if (r0 + 32 * k >= padded) break;
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        mma_16816(sums[j], held[k][0].x, held[k][1].x, held[k][0].y, held[k][1].y, w[k][j].x, w[k][j].y);
-                        mma_16816(sums[j], held[k][2].x, held[k][3].x, held[k][2].y, held[k][3].y, w[k][j].x, w[k][j].y);
+                    for (int q = 0; q < 2; ++q) {
+                        const uint4 &lo = held[k][0][q], &hi = held[k][1][q];
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            mma_16816(sums[j], lo.x, hi.x, lo.y, hi.y, w[k][j].x, w[k][j].y);
+                            mma_16816(sums[j], lo.z, hi.z, lo.w, hi.w, w[k][j].z, w[k][j].w);
+                        }
                     }
                 }
             }
             uint4 now[2][WORDS];
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int q = 0; q < WORDS; ++q) now[half][q] = old[half][q];
+                for (int q = 0; q < WORDS; ++q) now[h][q] = old[h][q];
             if (tile + step < tiles) {
                 load_y(tile + step);
                 load_b(tile + step, 0);
             }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                if (!mine[half]) continue;
-                Y* to = y[half] + tile * 32;
+            for (int h = 0; h < 2; ++h) {
+                if (!(rows >> (8 * h) & 1)) continue;
+                Y* to = y + 8 * h * s.ldy + tile * 32;
                 float add[8];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * half]; add[2 * j + 1] = sums[j][2 * half + 1]; }
+                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
                 if (WIDE && tile * 32 + 8 * t + 8 <= s.n) {
                     if constexpr (sizeof(Y) == 2) {
                         float v[8];
-                        unpack_bf16x8(now[half][0], v);
+                        unpack_bf16x8(now[h][0], v);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) add[e] += v[e];
                         *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
                     } else {
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
-                            const uint4 v = now[half][q];
+                            const uint4 v = now[h][q];
                             reinterpret_cast<float4*>(to)[q] =
                                 make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
                                             __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
@@ -537,25 +533,20 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
 }
 
 template <typename Y> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
-    // few rows: a tile of 32 columns a warp; more: enough CTAs for about four an SM, which walk over the columns
+    // few rows: a tile of 32 columns a warp; more: several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us
+    // with three CTAs an SM, 34 with six, 33 with twelve)
     const int tiles = ceil_div(a.n, 32), rows = ceil_div(a.m, a.columns_apart ? 16 : 16 * WARPS);
-    const int across = a.columns_apart ? ceil_div(tiles, WARPS) : min(tiles, max(1, 4 * 148 / rows));
+    const int across = a.columns_apart ? ceil_div(tiles, WARPS) : min(tiles, max(1, 12 * 148 / rows));
     const dim3 grid(across, rows, side_by_side);
     return wide ? launch(expand_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<Y, false>, grid, 0, 0, pdl, s, a);
 }
 
 }  // namespace
 
-// bytes of scratch: u
-extern "C" long long tvb_adapters_scratch(int m, int rank, int dtype) {
-    return m <= 0 ? 0 : (long long)m * (dtype == TVB_F32 ? rank * 4 : ceil_div(rank, 16) * 16 * 4);
-}
+namespace {
 
-extern "C" int tvb_adapters_shrink(const void* x, long long ldx, const void* down, const int* ids, const float* scales, void* u, int m,
-                                   int k, int rank, int adapters, int dtype, int pdl, void* stream) {
-    if (m <= 0 || adapters <= 0) return 0;
-    if (k <= 0 || rank <= 0 || rank > MAX_RANK || ceil_div(m, 64) > 65535) return TVB_BAD_ARGUMENT;
-    cudaStream_t s = (cudaStream_t)stream;
+int shrink(const void* x, long long ldx, const void* down, const int* ids, const float* scales, void* u, int m, int k, int rank,
+           int adapters, int dtype, int pdl, cudaStream_t s) {
     if (dtype == TVB_F32) {
         const bool wide = k % 4 == 0 && ldx % 4 == 0 && !(((uintptr_t)x | (uintptr_t)down) & 15);
         // pieces of at least 512 k, and not more CTAs than eight an SM
@@ -587,11 +578,8 @@ extern "C" int tvb_adapters_shrink(const void* x, long long ldx, const void* dow
 }
 
 // dtype: of x, A and B; y_dtype: of y (float32 with either, bfloat16 with bfloat16)
-extern "C" int tvb_adapters_expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank,
-                                   int adapters, int dtype, int y_dtype, int pdl, void* stream) {
-    if (m <= 0 || n <= 0 || adapters <= 0) return 0;
-    if (rank <= 0 || rank > MAX_RANK || ceil_div(m, 16) > 65535) return TVB_BAD_ARGUMENT;
-    cudaStream_t s = (cudaStream_t)stream;
+int expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank, int adapters, int dtype, int y_dtype,
+           int pdl, cudaStream_t s) {
     const bool few = m <= FEW_ROWS;
     const Expand a{u, up, ids, y, ldy, m, n, rank, adapters, few};
     if (dtype == TVB_F32) {
@@ -603,8 +591,33 @@ extern "C" int tvb_adapters_expand(const void* u, const void* up, const int* ids
     }
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const int size = y_dtype == TVB_F32 ? 4 : 2;
-    const bool wide = rank % 4 == 0 && !((uintptr_t)up & 7) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
-    const int side_by_side = few ? min(min(16, m), adapters) : 1;
+    const bool wide = rank % 8 == 0 && !((uintptr_t)up & 15) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
+    const int side_by_side = min(few ? min(16, m) : 2, adapters);
     if (y_dtype == TVB_F32) return launch_expand<float>(a, wide, side_by_side, pdl, s);
     return y_dtype == TVB_BF16 ? launch_expand<bf16>(a, wide, side_by_side, pdl, s) : TVB_BAD_ARGUMENT;
+}
+
+}  // namespace
+
+// The call's arguments as the Python side packs them.
+struct AdaptersCall {
+    const void* x;
+    long long ldx;
+    const void* down;
+    const void* up;
+    const int* ids;
+    const float* scales;
+    void* u;                                    // scratch: m rows of rank float32, for bfloat16 of the rank filled up to sixteens
+    void* y;
+    long long ldy;
+    int m, n, k, rank, adapters, dtype, y_dtype, pdl;
+};
+
+extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
+    const AdaptersCall& c = *call;
+    if (c.m <= 0 || c.n <= 0 || c.adapters <= 0) return 0;
+    if (c.k <= 0 || c.rank <= 0 || c.rank > MAX_RANK || ceil_div(c.m, 16) > 65535) return TVB_BAD_ARGUMENT;
+    cudaStream_t s = (cudaStream_t)stream;
+    const int e = shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
+    return e ? e : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);
 }

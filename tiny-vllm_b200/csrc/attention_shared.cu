@@ -1022,24 +1022,40 @@ extern "C" int tvb_attention_shared_status() {
     return value;
 }
 
-extern "C" int tvb_attention_shared(const void* q, long long q_stride, const void* keys, const void* values, const int* tables, int rows,
-                                    int width, const int* token_row, const int* positions, const int* group_starts, const int* shared_lens,
-                                    int groups, float* scratch, void* out, long long out_stride, int tokens, int pages, int page_size,
-                                    int num_q, int num_kv, int head_dim, int max_shared, int max_own, float scale, int dtype, int pdl,
-                                    void* stream) {
-    if (tokens <= 0) return 0;
-    if ((dtype != TVB_F32 && dtype != TVB_BF16) || num_kv <= 0 || num_q <= 0 || num_q % num_kv || page_size <= 0 || groups < 0 || rows < 0 ||
-        width < 0 || max_shared < 0 || max_own < 0 || (long long)width * page_size > 0x7fffffffLL - 4096 ||
-        (long long)pages * num_kv * page_size > 0x7fffffffLL)
+// The call's arguments as the Python side packs them.
+struct SharedCall {
+    const void* q;
+    long long q_stride;
+    const void* keys;
+    const void* values;
+    const int* tables;
+    const int* token_row;
+    const int* positions;
+    const int* group_starts;
+    const int* shared_lens;
+    float* scratch;
+    void* out;
+    long long out_stride;
+    int rows, width, groups, tokens, pages, page_size, num_q, num_kv, head_dim, max_shared, max_own, dtype, pdl;
+    float scale;
+};
+
+extern "C" int tvb_attention_shared(const SharedCall* call, void* stream) {
+    const SharedCall& c = *call;
+    if (c.tokens <= 0) return 0;
+    if ((c.dtype != TVB_F32 && c.dtype != TVB_BF16) || c.num_kv <= 0 || c.num_q <= 0 || c.num_q % c.num_kv || c.page_size <= 0 || c.groups < 0 ||
+        c.rows < 0 || c.width < 0 || c.max_shared < 0 || c.max_own < 0 || (long long)c.width * c.page_size > 0x7fffffffLL - 4096 ||
+        (long long)c.pages * c.num_kv * c.page_size > 0x7fffffffLL)
         return TVB_BAD_ARGUMENT;
-    const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
-    if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
-    Attend a{q, q_stride, keys, values, tables, token_row, positions, group_starts, shared_lens, p.pieces() > 1 ? scratch : nullptr, nullptr, out, out_stride,
-             tokens, rows, width, groups, pages, page_size, num_q, num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, scale * LOG2E};
-    a.part_ml = scratch + (long long)tokens * num_q * p.pieces() * head_dim;
+    const Plan p = plan_of(c.tokens, c.groups, c.num_q, c.num_kv, c.head_dim, c.page_size, c.max_shared, c.max_own, c.dtype);
+    if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL || (p.pieces() > 1 && !c.scratch)) return TVB_BAD_ARGUMENT;
+    Attend a{c.q, c.q_stride, c.keys, c.values, c.tables, c.token_row, c.positions, c.group_starts, c.shared_lens,
+             p.pieces() > 1 ? c.scratch : nullptr, nullptr, c.out, c.out_stride, c.tokens, c.rows, c.width, c.groups, c.pages, c.page_size,
+             c.num_q, c.num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, c.scale * LOG2E};
+    a.part_ml = c.scratch + (long long)c.tokens * c.num_q * p.pieces() * c.head_dim;
     cudaStream_t s = (cudaStream_t)stream;
-    if (head_dim == 64) return launch_all<64>(a, p, dtype, pdl, s);
-    if (head_dim == 128) return launch_all<128>(a, p, dtype, pdl, s);
-    if (head_dim == 256) return launch_all<256>(a, p, dtype, pdl, s);
+    if (c.head_dim == 64) return launch_all<64>(a, p, c.dtype, c.pdl, s);
+    if (c.head_dim == 128) return launch_all<128>(a, p, c.dtype, c.pdl, s);
+    if (c.head_dim == 256) return launch_all<256>(a, p, c.dtype, c.pdl, s);
     return TVB_BAD_ARGUMENT;
 }

@@ -204,40 +204,51 @@ __global__ void append_tokens_kernel(const int* slots, const int* tokens, int ro
     }
 }
 
-template <typename T, int VEC>
-int launch_rules(const void* logits, long long row_stride, void* out, long long out_stride, int rows, int vocab, const Rules& rules,
-                 cudaStream_t stream) {
-    const int slices = (vocab + SLICE - 1) / SLICE;
-    if ((long long)rows * slices > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
-    const size_t shared = rules.biases > 0 ? SLICE * 4 : 0;
-    logit_rules_kernel<T, VEC><<<rows * slices, THREADS, shared, stream>>>((const T*)logits, row_stride, (T*)out, out_stride, vocab,
-                                                                          slices, rules);
-    return tvb_last_error();
-}
-
 }  // namespace
 
 extern "C" int tvb_logit_rules_max_biases() { return MAX_BIASES; }
 
-extern "C" int tvb_logit_rules(const void* logits, long long row_stride, void* out, long long out_stride, int rows, int vocab,
-                               const int* slots, const float* penalties, const int* lengths, const int* history,
-                               const int* bias_tokens, const float* bias_values, const void* masks, const int* mask_rows,
-                               int slot_count, int room, int biases, int mask_count, int mask_words, int dtype, void* stream) {
-    if (rows <= 0 || vocab <= 0) return 0;
-    if (slot_count < 0 || room < 0 || biases < 0 || biases > MAX_BIASES || (biases > 0 && (!bias_tokens || !bias_values)) ||
-        (masks && (!mask_rows || (long long)mask_words * 32 < vocab)))
+// The call's arguments as the Python side packs them.
+struct RulesCall {
+    const void* logits;
+    long long row_stride;
+    void* out;
+    long long out_stride;
+    const int* slots;
+    const float* penalties;
+    const int* lengths;
+    const int* history;
+    const int* bias_tokens;
+    const float* bias_values;
+    const uint32_t* masks;
+    const int* mask_rows;
+    int rows, vocab, slot_count, room, biases, mask_count, mask_words, dtype;
+};
+
+namespace {
+template <typename T, int VEC> int launch_rules(const RulesCall& c, const Rules& rules, cudaStream_t stream) {
+    const int slices = (c.vocab + SLICE - 1) / SLICE;
+    if ((long long)c.rows * slices > 0x7fffffffLL) return TVB_BAD_ARGUMENT;
+    const size_t shared = rules.biases > 0 ? SLICE * 4 : 0;
+    logit_rules_kernel<T, VEC><<<c.rows * slices, THREADS, shared, stream>>>((const T*)c.logits, c.row_stride, (T*)c.out, c.out_stride, c.vocab,
+                                                                            slices, rules);
+    return tvb_last_error();
+}
+}  // namespace
+
+extern "C" int tvb_logit_rules(const RulesCall* call, void* stream) {
+    const RulesCall& c = *call;
+    if (c.rows <= 0 || c.vocab <= 0) return 0;
+    if (c.slot_count < 0 || c.room < 0 || c.biases < 0 || c.biases > MAX_BIASES || (c.biases > 0 && (!c.bias_tokens || !c.bias_values)) ||
+        (c.masks && (!c.mask_rows || (long long)c.mask_words * 32 < c.vocab)))
         return TVB_BAD_ARGUMENT;
-    const Rules rules{slots, penalties, lengths, history, bias_tokens, bias_values, (const uint32_t*)masks, mask_rows,
-                      slot_count, room, biases, mask_count, mask_words};
+    const Rules rules{c.slots, c.penalties, c.lengths, c.history, c.bias_tokens, c.bias_values, c.masks, c.mask_rows,
+                      c.slot_count, c.room, c.biases, c.mask_count, c.mask_words};
     cudaStream_t s = (cudaStream_t)stream;
-    const int size = dtype == TVB_F32 ? 4 : 2;
-    const bool wide = !(((uintptr_t)logits | (uintptr_t)out) & 15) && row_stride * size % 16 == 0 && out_stride * size % 16 == 0;
-    if (dtype == TVB_F32)
-        return wide ? launch_rules<float, 4>(logits, row_stride, out, out_stride, rows, vocab, rules, s)
-                    : launch_rules<float, 1>(logits, row_stride, out, out_stride, rows, vocab, rules, s);
-    if (dtype == TVB_BF16)
-        return wide ? launch_rules<bf16, 8>(logits, row_stride, out, out_stride, rows, vocab, rules, s)
-                    : launch_rules<bf16, 1>(logits, row_stride, out, out_stride, rows, vocab, rules, s);
+    const int size = c.dtype == TVB_F32 ? 4 : 2;
+    const bool wide = !(((uintptr_t)c.logits | (uintptr_t)c.out) & 15) && c.row_stride * size % 16 == 0 && c.out_stride * size % 16 == 0;
+    if (c.dtype == TVB_F32) return wide ? launch_rules<float, 4>(c, rules, s) : launch_rules<float, 1>(c, rules, s);
+    if (c.dtype == TVB_BF16) return wide ? launch_rules<bf16, 8>(c, rules, s) : launch_rules<bf16, 1>(c, rules, s);
     return TVB_BAD_ARGUMENT;
 }
 

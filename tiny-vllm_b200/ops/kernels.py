@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -1983,8 +1984,9 @@ def sample_rows(logits: torch.Tensor, packed: torch.Tensor, out: torch.Tensor | 
     return out
 
 
-def _here(who: str, *tensors: torch.Tensor | None) -> None:
-    """Refuse tensors that are not on the current CUDA device, whose current stream the kernel is launched on."""
+def _here(who: str, *tensors: torch.Tensor | None) -> int:
+    """Refuse tensors that are not on the current CUDA device; the raw handle of its current stream, which the kernel is
+    launched on."""
     for tensor in tensors:
         if tensor is not None and not tensor.is_cuda:
             raise KernelError("the kernels run on CUDA tensors only; there is no CPU path")
@@ -1993,6 +1995,11 @@ def _here(who: str, *tensors: torch.Tensor | None) -> None:
         if tensor is not None and tensor.get_device() != index:
             raise KernelError(f"{who}: every tensor has to be on the current device (cuda:{index}; "
                               f"torch.cuda.device(...) makes another one current), got {tensor.device}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+# Calls whose arguments go over packed as the C side's struct has them: some twenty through ctypes take 2.5 us, packed 0.6.
+_PACKED = [ctypes.c_char_p, c_void_p]
 
 
 def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -2013,7 +2020,10 @@ APPEND_MAX_ROWS = 8192
 
 
 def _is(t: torch.Tensor, dtype: torch.dtype, *shape: int) -> bool:
-    return t.dtype == dtype and t.shape == shape and t.is_contiguous()
+    return t.dtype is dtype and t.shape == shape and t.is_contiguous()
+
+
+_RULES_CALL = struct.Struct("@PqPqPPPPPPPPiiiiiiii")
 
 
 def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.Tensor, lengths: torch.Tensor,
@@ -2035,7 +2045,7 @@ def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.T
 
     Computed in float32 and rounded once to the type of the logits.  ``out``: where the result goes, ``logits`` itself
     among others (in place); else a new tensor."""
-    if logits.dim() != 2 or logits.stride(1) != 1 and logits.shape[1] > 1:
+    if logits.dim() != 2 or logits.stride()[1] != 1 and logits.shape[1] > 1:
         raise KernelError("logit_rules wants logits [rows, vocab] whose rows are contiguous")
     tag = dtype_tag(logits.dtype)
     (rows, vocab), (count, room) = logits.shape, history.shape if history.dim() == 2 else (-1, 0)
@@ -2060,21 +2070,21 @@ def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.T
             raise KernelError(f"logit_rules: masks must be contiguous int32 [masks, at least {-(-vocab // 32)}], "
                               f"mask_rows int32 [{count}]")
     if out is None:
-        _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows)
-        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        stream = _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     else:
         if out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1 and vocab > 1 \
                 or rows > 1 and out.stride(0) < vocab:
             raise KernelError("logit_rules: out must be [rows, vocab] of the type of the logits with contiguous rows of its own")
         if (out.data_ptr() != logits.data_ptr() or out.stride(0) != logits.stride(0)) and _overlaps(out, logits):
             raise KernelError("logit_rules: out is the logits themselves, or memory of its own")
-        _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows, out)
-    fn = _fn("logit_rules", "tvb_logit_rules",
-             [c_void_p, c_longlong, c_void_p, c_longlong, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-              c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p])
-    _check(fn(logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0), rows, vocab, slots.data_ptr(),
-              penalties.data_ptr(), lengths.data_ptr(), history.data_ptr(), _ptr(bias_tokens), _ptr(bias_values), _ptr(masks),
-              _ptr(mask_rows), count, room, biases, mask_count, words, tag, _stream()), "logit_rules")
+        stream = _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows, out)
+    call = _RULES_CALL.pack(
+        logits.data_ptr(), logits.stride()[0], out.data_ptr(), out.stride()[0], slots.data_ptr(), penalties.data_ptr(),
+        lengths.data_ptr(), history.data_ptr(), 0 if bias_tokens is None else bias_tokens.data_ptr(),
+        0 if bias_values is None else bias_values.data_ptr(), 0 if masks is None else masks.data_ptr(),
+        0 if mask_rows is None else mask_rows.data_ptr(), rows, vocab, count, room, biases, mask_count, words, tag)
+    _check(_fn("logit_rules", "tvb_logit_rules", _PACKED)(call, stream), "logit_rules")
     return out
 
 
@@ -2097,28 +2107,21 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
 ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
 
 
-def adapters_shrink(x: torch.Tensor, down: torch.Tensor, ids: torch.Tensor, scales: torch.Tensor | None) -> torch.Tensor:
-    """The first half of :func:`tinyvllm_b200.ops.linear_adapted`: u = scale * x . A^T of every row, as
-    :func:`adapters_expand` reads it.  Arguments as checked there."""
-    m, k = x.shape
-    adapters, rank, _ = down.shape
+_ADAPTERS_CALL = struct.Struct("@PqPPPPPPqiiiiiiii")
+
+
+def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,
+                 scales: torch.Tensor | None, stream: int) -> None:
+    """y[t] += scale * (x[t] . A^T) . B^T in place, rounded once more to the type of y; arguments as
+    :func:`tinyvllm_b200.ops.linear_adapted` has checked them."""
+    (m, n), (adapters, rank, k) = y.shape, down.shape
     tag = dtype_tag(x.dtype)
-    u = torch.empty(_fn("adapters", "tvb_adapters_scratch", [c_int, c_int, c_int], c_longlong)(m, rank, tag),
-                    dtype=torch.uint8, device=x.device)
-    fn = _fn("adapters", "tvb_adapters_shrink",
-             [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p] + [c_int] * 6 + [c_void_p])
-    _check(fn(x.data_ptr(), x.stride(0), down.data_ptr(), ids.data_ptr(), _ptr(scales), u.data_ptr(), m, k, rank, adapters, tag,
-              _pdl("gemm"), _stream()), "adapters_shrink")
-    return u
-
-
-def adapters_expand(u: torch.Tensor, up: torch.Tensor, ids: torch.Tensor, y: torch.Tensor) -> None:
-    """The second half: y[t] += u[t] . B^T in place, rounded once more to the type of y."""
-    (m, n), (adapters, _, rank) = y.shape, up.shape
-    fn = _fn("adapters", "tvb_adapters_expand",
-             [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong] + [c_int] * 7 + [c_void_p])
-    _check(fn(u.data_ptr(), up.data_ptr(), ids.data_ptr(), y.data_ptr(), y.stride(0), m, n, rank, adapters,
-              dtype_tag(up.dtype), dtype_tag(y.dtype), _pdl("gemm"), _stream()), "adapters_expand")
+    # u: float32, or two bfloat16 a value with the rank filled up to sixteens
+    u = torch.empty(m * (rank if tag == F32 else -(-rank // 16) * 16), dtype=torch.float32, device=x.device)
+    call = _ADAPTERS_CALL.pack(
+        x.data_ptr(), x.stride()[0], down.data_ptr(), up.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
+        u.data_ptr(), y.data_ptr(), y.stride()[0], m, n, k, rank, adapters, tag, dtype_tag(y.dtype), _pdl("gemm"))
+    _check(_fn("adapters", "tvb_add_adapters", _PACKED)(call, stream), "add_adapters", 2)
 
 
 # ------------------------------------------ attention over keys in common (paged)
@@ -2131,6 +2134,7 @@ def _shared_plan(*sizes: int) -> tuple[int, int]:
     return floats, launches.value
 
 
+_SHARED_CALL = struct.Struct("@PqPPPPPPPPPqiiiiiiiiiiiiif")
 _attention_shared_unchecked = False
 
 
@@ -2163,9 +2167,9 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     if head_dim not in DECODE_HEAD_DIMS or num_kv < 1 or num_q < 1 or num_q % num_kv:
         raise KernelError(f"attention_shared takes head sizes {DECODE_HEAD_DIMS} and whole groups of q heads "
                           f"(head_dim {head_dim}, {num_q} / {num_kv} heads)")
-    if key_cache.dim() != 4 or key_cache.shape[1] != num_kv or key_cache.shape[3] != head_dim or key_cache.shape[2] < 1 \
-            or key_cache.dtype != q.dtype or not key_cache.is_contiguous() or value_cache.shape != key_cache.shape \
-            or value_cache.dtype != q.dtype or not value_cache.is_contiguous():
+    pages, _, page_size, _ = key_cache.shape if key_cache.dim() == 4 else (0, 0, 0, 0)
+    if page_size < 1 or not _is(key_cache, q.dtype, pages, num_kv, page_size, head_dim) \
+            or not _is(value_cache, q.dtype, pages, num_kv, page_size, head_dim):
         raise KernelError("attention_shared: caches must be contiguous [pages, num_kv, page_size, head_dim] of the type of q")
     if tokens < 0 or not _is(positions, torch.int32, tokens) or not _is(token_row, torch.int32, tokens):
         raise KernelError("attention_shared: token_row and positions must be contiguous int32 [tokens]")
@@ -2175,11 +2179,10 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     if groups < 0 or not _is(shared_lens, torch.int32, groups) or not _is(group_starts, torch.int32, groups + 1):
         raise KernelError("attention_shared: shared_lens must be contiguous int32 [groups], group_starts int32 [groups + 1]")
     size, width = q.element_size(), num_q * head_dim
-    last = q.stride(-1) if q.dim() else 0
-    if last != 1 or q_token_stride < width or q_token_stride * size % 16 or q.data_ptr() % 16 \
+    if not q.dim() or q.stride()[-1] != 1 or q_token_stride < width or q_token_stride * size % 16 or q.data_ptr() % 16 \
             or tokens > 0 and q.untyped_storage().nbytes() < (q.storage_offset() + (tokens - 1) * q_token_stride + width) * size:
         raise KernelError("attention_shared: the heads of token t stand at q + t * q_token_stride, on 16 bytes, inside its memory")
-    held = block_tables.shape[1] * key_cache.shape[2]
+    held = block_tables.shape[1] * page_size
     max_shared = held if max_shared is None else max_shared
     max_own = held if max_own is None else max_own
     if not 0 <= max_shared < 2**31 or not 0 <= max_own < 2**31:
@@ -2187,26 +2190,24 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     if not 0.0 < scale < float("inf"):
         raise KernelError("attention_shared: the scale is positive and finite")
     if out is None:
-        _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
+        stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
         out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
     else:
         if out.shape != (tokens, width) or out.dtype != q.dtype or out.stride(1) != 1 or tokens > 1 and out.stride(0) < width:
             raise KernelError("attention_shared: out must be [tokens, num_q * head_dim] of the type of q with contiguous rows")
-        _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
+        stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
     if tokens == 0:
         return out
-    need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, key_cache.shape[2], max_shared, max_own, tag)
-    scratch = torch.empty(need, dtype=torch.float32, device=q.device)
-    fn = _fn("attention_shared", "tvb_attention_shared",
-             [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-              c_void_p, c_void_p, c_longlong] + [c_int] * 8 + [c_float, c_int, c_int, c_void_p])
-    _check(fn(q.data_ptr(), q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(),
-              block_tables.shape[0], block_tables.shape[1], token_row.data_ptr(), positions.data_ptr(), group_starts.data_ptr(),
-              shared_lens.data_ptr(), groups, scratch.data_ptr(), out.data_ptr(), out.stride(0), tokens, key_cache.shape[0],
-              key_cache.shape[2], num_q, num_kv, head_dim, max_shared, max_own, scale, tag, _pdl("attention_shared"), _stream()),
-           "attention_shared", launches)
+    need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, tag)
+    scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
+    call = _SHARED_CALL.pack(
+        q.data_ptr(), q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_row.data_ptr(),
+        positions.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+        out.data_ptr(), out.stride()[0], block_tables.shape[0], block_tables.shape[1], groups, tokens, pages, page_size, num_q,
+        num_kv, head_dim, max_shared, max_own, tag, _pdl("attention_shared"), scale)
+    _check(_fn("attention_shared", "tvb_attention_shared", _PACKED)(call, stream), "attention_shared", launches)
     global _attention_shared_unchecked
-    _attention_shared_unchecked = _attention_shared_unchecked or launches > 1
+    _attention_shared_unchecked = _attention_shared_unchecked or tag == BF16
     return out
 
 

@@ -87,7 +87,7 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
         raise kernels.KernelError(f"linear_adapted: ids must be contiguous int32 [{m}]")
     if scales is not None and not kernels._is(scales, torch.float32, adapters):
         raise kernels.KernelError(f"linear_adapted: scales must be contiguous float32 [{adapters}]")
-    if x.stride(1) != 1 and k > 1:
+    if x.stride()[1] != 1 and k > 1:
         raise kernels.KernelError("linear_adapted: the rows of x must be contiguous")
     out_dtype = out_dtype or (x.dtype if out is None else out.dtype)
     if out_dtype not in (x.dtype, torch.float32):
@@ -95,13 +95,11 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     if out is not None and (out.shape != (m, n) or out.dtype != out_dtype or out.stride(1) != 1 and n > 1
                             or m > 1 and out.stride(0) < n or any(kernels._overlaps(out, t) for t in (x, weight, down, up))):
         raise kernels.KernelError(f"linear_adapted: out must be {out_dtype} [{m}, {n}] with contiguous rows, in memory of its own")
-    kernels._here("linear_adapted", x, weight, down, up, ids, scales, out)
+    stream = kernels._here("linear_adapted", x, weight, down, up, ids, scales, out)
     if m == 0 or n == 0:
         return torch.empty((m, n), dtype=out_dtype, device=x.device) if out is None else out
-    # the short product first: the projection's kernel may then ask for its weight while that ends
-    u = kernels.adapters_shrink(x, down, ids, scales)
     y = linear(x, weight, out_dtype=out_dtype, out=out, weight_constant=weight_constant)
-    kernels.adapters_expand(u, up, ids, y)
+    kernels.add_adapters(y, x, down, up, ids, scales, stream)
     return y
 
 
