@@ -20,6 +20,7 @@ namespace {
 constexpr int THREADS = 256;
 constexpr int SLICE = 4096;                        // tokens of the vocabulary a CTA takes
 constexpr int MAX_BIASES = 1024;                   // biases of a slot
+constexpr int BIASES_EACH = MAX_BIASES / THREADS;  // ... and of a thread
 constexpr uint32_t HAS_BIAS = 1u << 31, IN_PROMPT = 1u << 30, COUNT = IN_PROMPT - 1;
 
 struct Rules {
@@ -52,7 +53,7 @@ template <typename T, int VEC> __device__ __forceinline__ void store_vec(T* p, c
 
 // logits may be out itself (every thread reads what it will write before it writes): plain pointers
 template <typename T, int VEC>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, VEC == 1 ? 4 : 5)
 logit_rules_kernel(const T* logits, int64_t row_stride, T* out, int64_t out_stride, int vocab, int slices, Rules rules) {
     __shared__ __align__(16) uint32_t words[SLICE];
     __shared__ int any_twice;
@@ -74,65 +75,82 @@ logit_rules_kernel(const T* logits, int64_t row_stride, T* out, int64_t out_stri
             for (int e = 0; e < VEC; ++e) v[p][e] = at + e < count ? to_float<T>(x[at + e]) : 0.0f;
     }
     const int slot = rules.slots[row];
+    for (int i = 4 * tid; i < SLICE; i += 4 * THREADS) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
+    if (tid == 0) any_twice = 0;
+    __syncthreads();
     const bool ruled = (unsigned)slot < (unsigned)rules.slot_count;       // the same for the whole CTA
     float repetition = 1.0f, presence = 0.0f, frequency = 0.0f;
     const uint32_t* mask = nullptr;
-    bool counted = false, biased = false;
+    uint32_t allowed[PASSES];                      // the mask's words of this thread's tokens
+    bool counted = false;
+    const bool biased = ruled && rules.biases > 0;
     if (ruled) {
+        // (everything that the slot leads to, side by side)
+        int bias_token[BIASES_EACH];
+        const int* tokens = rules.bias_tokens + (int64_t)slot * rules.biases;
+        const float* values = rules.bias_values + (int64_t)slot * rules.biases;
+#pragma unroll
+        for (int n = 0; n < BIASES_EACH; ++n)
+            bias_token[n] = tid + n * THREADS < rules.biases ? __ldcg(tokens + tid + n * THREADS) : -1;
         repetition = rules.penalties[3 * (int64_t)slot];
         presence = rules.penalties[3 * (int64_t)slot + 1];
         frequency = rules.penalties[3 * (int64_t)slot + 2];
-        if (rules.masks) {
-            const int m = rules.mask_rows[slot];
-            if ((unsigned)m < (unsigned)rules.mask_count) mask = rules.masks + (int64_t)m * rules.mask_words;
-        }
         const int total = min(max(rules.lengths[2 * (int64_t)slot], 0), rules.room);
         const int prompt = min(max(rules.lengths[2 * (int64_t)slot + 1], 0), total);
+        if (rules.masks) {
+            const int m = rules.mask_rows[slot];
+            if ((unsigned)m < (unsigned)rules.mask_count) {
+                mask = rules.masks + (int64_t)m * rules.mask_words;
+#pragma unroll
+                for (int p = 0; p < PASSES; ++p) {
+                    const int at = (p * THREADS + tid) * VEC;
+                    if (at < count) allowed[p] = __ldg(mask + ((begin + at) >> 5));
+                }
+            }
+        }
         // without a penalty for repetition the prompt is not looked at
         const int first = repetition == 1.0f ? (presence == 0.0f && frequency == 0.0f ? total : prompt) : 0;
         counted = first < total;
-        biased = rules.biases > 0;
-        if (counted || biased) {
-            for (int i = 4 * tid; i < SLICE; i += 4 * THREADS) *reinterpret_cast<uint4*>(words + i) = make_uint4(0, 0, 0, 0);
-            if (tid == 0) any_twice = 0;
-            __syncthreads();
-            const int* history = rules.history + (int64_t)slot * rules.room;
-#pragma unroll 4
-            for (int i = first + tid; i < total; i += THREADS) {
-                const unsigned at = (unsigned)history[i] - (unsigned)begin;
-                if (at < (unsigned)count) {
-                    if (i >= prompt) atomicAdd(words + at, 1u);
+        const int* history = rules.history + (int64_t)slot * rules.room;
+        // (in batches, so that the loads of one do not wait for the counts of the one before)
+        constexpr int BATCH = 8;
+        for (int i0 = first + tid; i0 < total; i0 += BATCH * THREADS) {
+            int token[BATCH];
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) token[n] = i0 + n * THREADS < total ? __ldcg(history + i0 + n * THREADS) : -1;
+#pragma unroll
+            for (int n = 0; n < BATCH; ++n) {
+                const unsigned at = (unsigned)token[n] - (unsigned)begin;
+                if (token[n] >= 0 && at < (unsigned)count) {
+                    if (i0 + n * THREADS >= prompt) atomicAdd(words + at, 1u);
                     else atomicOr(words + at, IN_PROMPT);
                 }
             }
-            if (biased) {
-                const int* tokens = rules.bias_tokens + (int64_t)slot * rules.biases;
-                const float* values = rules.bias_values + (int64_t)slot * rules.biases;
-                for (int i = tid; i < rules.biases; i += THREADS) {
-                    const int token = tokens[i];
-                    const unsigned at = (unsigned)token - (unsigned)begin;
-                    if (token >= 0 && at < (unsigned)count) {
-                        if (atomicOr(words + at, HAS_BIAS) & HAS_BIAS) any_twice = 1;
-                        else bias[at] = values[i];
+        }
+#pragma unroll
+        for (int n = 0; n < BIASES_EACH; ++n) {
+            const unsigned at = (unsigned)bias_token[n] - (unsigned)begin;
+            if (bias_token[n] >= 0 && at < (unsigned)count) {
+                if (atomicOr(words + at, HAS_BIAS) & HAS_BIAS) any_twice = 1;
+                else bias[at] = __ldcg(values + tid + n * THREADS);
+            }
+        }
+        if (counted || biased) __syncthreads();
+        if (biased && any_twice) {
+            // a token named more than once: its first entry adds them all up, in their order
+#pragma unroll
+            for (int n = 0; n < BIASES_EACH; ++n) {
+                const int i = tid + n * THREADS, token = bias_token[n];
+                const unsigned at = (unsigned)token - (unsigned)begin;
+                if (token < 0 || at >= (unsigned)count) continue;
+                bool first_entry = true;
+                float sum = 0.0f;
+                for (int j = 0; j < rules.biases && first_entry; ++j)
+                    if (tokens[j] == token) {
+                        if (j < i) first_entry = false;
+                        else sum = __fadd_rn(sum, values[j]);
                     }
-                }
-                __syncthreads();
-                if (any_twice) {
-                    // a token named more than once: its first entry adds them all up, in their order
-                    for (int i = tid; i < rules.biases; i += THREADS) {
-                        const int token = tokens[i];
-                        const unsigned at = (unsigned)token - (unsigned)begin;
-                        if (token < 0 || at >= (unsigned)count) continue;
-                        bool first_entry = true;
-                        float sum = 0.0f;
-                        for (int j = 0; j < rules.biases && first_entry; ++j)
-                            if (tokens[j] == token) {
-                                if (j < i) first_entry = false;
-                                else sum = __fadd_rn(sum, values[j]);
-                            }
-                        if (first_entry) bias[at] = sum;
-                    }
-                }
+                if (first_entry) bias[at] = sum;
             }
             __syncthreads();
         }
@@ -161,11 +179,10 @@ logit_rules_kernel(const T* logits, int64_t row_stride, T* out, int64_t out_stri
             }
         }
         if (mask) {
+            const uint32_t bits = allowed[p] >> (at & 31);                      // (a slice starts at a whole word, VEC divides 32)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                const int token = begin + at + e;
-                if (at + e < count && !(mask[token >> 5] >> (token & 31) & 1u)) v[p][e] = -INFINITY;
-            }
+            for (int e = 0; e < VEC; ++e)
+                if (!(bits >> e & 1u)) v[p][e] = -INFINITY;
         }
         if (at + VEC <= count) store_vec<T, VEC>(y + at, v[p]);
         else
