@@ -39,6 +39,16 @@ def test_refusals(changed):
     assert "CUDA tensors only" not in str(refusal.value)
 
 
+@pytest.mark.parametrize("name", ["x", "weight", "down", "up", "scales"])
+def test_operands_that_want_gradients_are_refused(name):
+    arguments = good()
+    arguments[name].requires_grad_(True)
+    with pytest.raises(kernels.KernelError, match="backward"):
+        linear_adapted(**arguments)
+    with torch.no_grad(), pytest.raises(kernels.KernelError, match="CUDA tensors only"):
+        linear_adapted(**arguments)
+
+
 def test_a_result_over_an_operand_is_refused():
     arguments = good(n=16)
     for name in ("x", "weight"):

@@ -166,6 +166,15 @@ def test_strided_q_and_results(dtype):
         memory[:, 20:276] = 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_a_cache_without_pages(dtype):
+    s, sizes = made([(48, [5, 2])], dtype=dtype)
+    for cache in ("key_cache", "value_cache"):
+        s[cache] = s[cache][:0]
+    for hints in ({}, TOGETHER):
+        assert (shared(s, sizes, **hints) == 0).all()
+
+
 def test_no_tokens():
     s, sizes = made([(48, [5])])
     empty = {name: s[name][:0] for name in ("q", "token_row", "positions")}

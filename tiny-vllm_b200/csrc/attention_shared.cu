@@ -940,11 +940,11 @@ struct Plan {
 // tensor cores, for one CTA on as many SMs as are their share of the work (a block of 128 keys takes a tile 1.2 us, a token's own
 // keys come in at 47 KB a us and SM), half of them at least, so that attend_own's CTAs run on the others meanwhile (60 tokens with up
 // to 431 keys behind 6,144: 39.0 us with all 148, 35.5 with 100, 32.6 with 74; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42, 53, 87).
-Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size, long long max_shared, long long max_own, int dtype) {
+Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pages, int page_size, long long max_shared, long long max_own, int dtype) {
     constexpr int MIN_KEYS = 128, SMS = 148;
     const int heads = num_q / num_kv;
     Plan p;
-    p.tile_tokens = dtype == TVB_BF16 && tc_takes(head_dim, heads, page_size) ? TC_ROWS / heads : 0;
+    p.tile_tokens = dtype == TVB_BF16 && pages > 0 && tc_takes(head_dim, heads, page_size) ? TC_ROWS / heads : 0;
     // CTAs' tiles: at most, and as a rule
     long long tiles = 0, usual = 1;
     // Up to so many values (32 MB of bfloat16) the tokens read the shared keys by themselves, in one launch or two: the third
@@ -995,7 +995,7 @@ template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int p
     int e = p.shared_items > 0 ? launch_shared<D>(a, p, dtype, pdl, s) : 0;
     if (e) return e;
     if (dtype == TVB_F32) e = launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, s, a);
-    else if (own_tma_takes(a.page_size)) e = launch_own_tma<D>(a, p.own_items, pdl, s);
+    else if (a.pages > 0 && own_tma_takes(a.page_size)) e = launch_own_tma<D>(a, p.own_items, pdl, s);
     else e = launch(attend_own_bf16_kernel<D>, p.own_items, OwnTiles<D>::BYTES, pdl, s, a);
     if (e || !a.part_o) return e;
     const long long joins = ceil_div((long long)a.tokens * a.num_q, WARPS);
@@ -1005,11 +1005,11 @@ template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int p
 }  // namespace
 
 // float32 of scratch, and the launches that a call takes in `launches`
-extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int num_q, int num_kv, int head_dim, int page_size,
+extern "C" long long tvb_attention_shared_scratch(int tokens, int groups, int num_q, int num_kv, int head_dim, int pages, int page_size,
                                                   int max_shared, int max_own, int dtype, int* launches) {
     *launches = 0;
     if (tokens <= 0 || num_kv <= 0) return 0;
-    const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, dtype);
+    const Plan p = plan_of(tokens, groups, num_q, num_kv, head_dim, pages, page_size, max_shared, max_own, dtype);
     *launches = p.pieces() > 1 ? 2 + (p.shared_items > 0) : 1;
     return p.pieces() > 1 ? (long long)tokens * num_q * p.pieces() * (head_dim + 2) : 0;
 }
@@ -1047,7 +1047,7 @@ extern "C" int tvb_attention_shared(const SharedCall* call, void* stream) {
         c.rows < 0 || c.width < 0 || c.max_shared < 0 || c.max_own < 0 || (long long)c.width * c.page_size > 0x7fffffffLL - 4096 ||
         (long long)c.pages * c.num_kv * c.page_size > 0x7fffffffLL)
         return TVB_BAD_ARGUMENT;
-    const Plan p = plan_of(c.tokens, c.groups, c.num_q, c.num_kv, c.head_dim, c.page_size, c.max_shared, c.max_own, c.dtype);
+    const Plan p = plan_of(c.tokens, c.groups, c.num_q, c.num_kv, c.head_dim, c.pages, c.page_size, c.max_shared, c.max_own, c.dtype);
     if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL || (p.pieces() > 1 && !c.scratch)) return TVB_BAD_ARGUMENT;
     Attend a{c.q, c.q_stride, c.keys, c.values, c.tables, c.token_row, c.positions, c.group_starts, c.shared_lens,
              p.pieces() > 1 ? c.scratch : nullptr, nullptr, c.out, c.out_stride, c.tokens, c.rows, c.width, c.groups, c.pages, c.page_size,

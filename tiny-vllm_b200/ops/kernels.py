@@ -1987,15 +1987,17 @@ def sample_rows(logits: torch.Tensor, packed: torch.Tensor, out: torch.Tensor | 
 def _here(who: str, *tensors: torch.Tensor | None) -> int:
     """Refuse tensors that are not on the current CUDA device; the raw handle of its current stream, which the kernel is
     launched on."""
-    for tensor in tensors:
-        if tensor is not None and not tensor.is_cuda:
-            raise KernelError("the kernels run on CUDA tensors only; there is no CPU path")
-    index = torch._C._cuda_getDevice()
-    for tensor in tensors:
-        if tensor is not None and tensor.get_device() != index:
-            raise KernelError(f"{who}: every tensor has to be on the current device (cuda:{index}; "
-                              f"torch.cuda.device(...) makes another one current), got {tensor.device}")
-    return torch._C._cuda_getCurrentRawStream(index)
+    if tensors[0].is_cuda:                       # (without a GPU there is no current device to ask for)
+        index = torch._C._cuda_getDevice()
+        for tensor in tensors:
+            if tensor is not None and tensor.get_device() != index:
+                break
+        else:
+            return torch._C._cuda_getCurrentRawStream(index)
+    if not all(tensor is None or tensor.is_cuda for tensor in tensors):
+        raise KernelError("the kernels run on CUDA tensors only; there is no CPU path")
+    raise KernelError(f"{who}: every tensor has to be on the current device (cuda:{torch.cuda.current_device()}; "
+                      f"torch.cuda.device(...) makes another one current), got {[str(t.device) for t in tensors if t is not None]}")
 
 
 # Calls whose arguments go over packed as the C side's struct has them: some twenty through ctypes take 2.5 us, packed 0.6.
@@ -2129,7 +2131,7 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch
 def _shared_plan(*sizes: int) -> tuple[int, int]:
     """(float32 of scratch, launches) of an :func:`attention_shared` of these sizes."""
     launches = ctypes.c_int(0)
-    floats = _fn("attention_shared", "tvb_attention_shared_scratch", [c_int] * 9 + [ctypes.POINTER(c_int)], c_longlong)(
+    floats = _fn("attention_shared", "tvb_attention_shared_scratch", [c_int] * 10 + [ctypes.POINTER(c_int)], c_longlong)(
         *sizes, ctypes.byref(launches))
     return floats, launches.value
 
@@ -2161,7 +2163,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     its keys by itself.  ``max_shared`` and ``max_own``: no group shares more, no token has more keys behind its group's;
     by them the work is cut up (and groups whose keys are few are not read together at all), the result does not depend on
     them beyond rounding (default: what the tables hold).  A key
-    whose page is no page of the cache is not seen.  bfloat16 and float32, head sizes 64, 128 and 256."""
+    whose page is no page of the cache is not seen.  bfloat16 and float32, head sizes 64, 128 and 256.  (The bfloat16 kernels
+    have bounded waits: :func:`check_finished_launches` says whether one ran out.)"""
     tokens = positions.shape[0] if positions.dim() == 1 else -1
     tag = dtype_tag(q.dtype)
     if head_dim not in DECODE_HEAD_DIMS or num_kv < 1 or num_q < 1 or num_q % num_kv:
@@ -2198,7 +2201,7 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
     if tokens == 0:
         return out
-    need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, page_size, max_shared, max_own, tag)
+    need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, pages, page_size, max_shared, max_own, tag)
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     call = _SHARED_CALL.pack(
         q.data_ptr(), q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_row.data_ptr(),
