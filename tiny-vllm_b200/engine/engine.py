@@ -447,15 +447,13 @@ class Engine:
         if lowered.bucket is not None:
             tokens_device, logits = self.graphs.launch(lowered.bucket, scheduled.cache_plan)
             self.graph_steps += 1
-            if lowered.rule_slots is not None:           # the graph sampled without the rules: sample again
-                tokens_device = self.sampler.sample(logits, lowered.params, lowered.draws, rules=self.rules,
-                                                    slots=lowered.rule_slots)
         else:
             logits = self.runner.launch(lowered.prepared)
-            if logits is not None:
-                tokens_device = self.sampler.sample(
-                    logits, lowered.params, lowered.draws, slots=lowered.rule_slots or (),
-                    rules=self.rules if lowered.rule_slots is not None else None)
+            if logits is not None and lowered.rule_slots is None:
+                tokens_device = self.sampler.sample(logits, lowered.params, lowered.draws)
+        if logits is not None and lowered.rule_slots is not None:       # (a graph has sampled without the rules: again)
+            tokens_device = self.sampler.sample(logits, lowered.params, lowered.draws, rules=self.rules,
+                                                slots=lowered.rule_slots)
         if tokens_device is None:
             return {}
         host = tokens_device.tolist()
