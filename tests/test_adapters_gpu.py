@@ -80,6 +80,15 @@ def test_sizes(k, n, m, dtype):
     check(adapted(**s), s)
 
 
+@pytest.mark.parametrize("rank", [8, 16, 24, 64])
+@pytest.mark.parametrize("m, k, n", [(129, 72, 8), (191, 8, 72), (300, 2056, 200), (1025, 520, 1032)])
+def test_more_rows_with_tails_of_every_size(m, k, n, rank):
+    s = made(m, k, n, rank, 6)
+    check(adapted(**s), s)
+    s["x"] = s["x"][:1].expand(m, k)                                   # one row for all
+    check(adapted(**s), s)
+
+
 @pytest.mark.parametrize("kind", ["one", "none", "spans"])
 @pytest.mark.parametrize("m", [20, 333])
 def test_which_rows_have_which(kind, m):
@@ -87,9 +96,10 @@ def test_which_rows_have_which(kind, m):
     check(adapted(**s), s)
 
 
+@pytest.mark.parametrize("rank", [4, 32])
 @pytest.mark.parametrize("m", [64, 260])
-def test_every_row_another_adapter(m):
-    s = made(m, 128, 96, 4, m)
+def test_every_row_another_adapter(m, rank):
+    s = made(m, 128, 96, rank, m)
     s["ids"] = torch.randperm(m, generator=torch.Generator().manual_seed(m)).to(torch.int32).to(DEV)
     check(adapted(**s), s)
 

@@ -10,7 +10,8 @@
 // bfloat16: mma.sync m16n8k16 (the products are a hundredth of the projection's: what counts is that A, B, x and y come in
 // with enough of them in flight).  Up to FEW_ROWS rows a CTA of `shrink` has 16 rows and loads straight into registers: a
 // thread takes 16 bytes, eight neighbouring k, of each row, and which k a fragment's place stands for is permuted alike in
-// both operands.  More rows go 64 a CTA through a ring in shared memory that cp.async fills.  u leaves in two bfloat16 whose
+// both operands.  More rows go 64 a CTA through a ring in shared memory: tensor-map copies fill it where types, ranks and alignment
+// allow (adapters_tma.cuh, which has its own `expand` too), else cp.async.  u leaves in two bfloat16 whose
 // sum is u to 2^-17 of it, so that no rounding of u is seen beside that of the result.  A row takes the sums of its own
 // adapter alone: what other adapters hold, infinities among them, does not reach it.
 // float32: the float32 cores.
@@ -511,6 +512,8 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
     }
 }
 
+#include "adapters_tma.cuh"
+
 // ------------------------------------------------------------------ host side
 constexpr int FEW_ROWS = 128;                   // rows up to which a CTA of `shrink` has 16 rows and one adapter
 
@@ -618,6 +621,20 @@ extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
     if (c.m <= 0 || c.n <= 0 || c.adapters <= 0) return 0;
     if (c.k <= 0 || c.rank <= 0 || c.rank > MAX_RANK || ceil_div(c.m, 16) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
+    if (c.m > FEW_ROWS && c.dtype == TVB_BF16 &&
+        adapters_tma_takes(c.x, c.ldx, c.down, c.up, c.y, c.ldy, c.k, c.n, c.rank, c.adapters, c.y_dtype)) {
+        const int e = shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0},
+                                 c.pdl, s);
+        return e ? e : expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, 0}, c.pdl, s);
+    }
     const int e = shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
     return e ? e : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);
+}
+
+// 0, or which bounded wait gave up in some launch since the last call; reading clears it.  Synchronises.
+extern "C" int tvb_adapters_status() {
+    int value = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&value, tvb_adapters_status_word, sizeof(int)) != cudaSuccess) return -1;
+    if (value != 0) cudaMemcpyToSymbol(tvb_adapters_status_word, &zero, sizeof(int));
+    return value;
 }

@@ -2107,6 +2107,7 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
 
 # ------------------------------------------------------------- low-rank adapters
 ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
+ADAPTERS_FEW_ROWS = 128            # FEW_ROWS there: more rows may go through the kernels with bounded waits
 
 
 _ADAPTERS_CALL = struct.Struct("@PqPPPPPPqiiiiiiii")
@@ -2124,6 +2125,19 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch
         x.data_ptr(), x.stride()[0], down.data_ptr(), up.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
         u.data_ptr(), y.data_ptr(), y.stride()[0], m, n, k, rank, adapters, tag, dtype_tag(y.dtype), _pdl("gemm"))
     _check(_fn("adapters", "tvb_add_adapters", _PACKED)(call, stream), "add_adapters", 2)
+    global _adapters_unchecked
+    _adapters_unchecked = _adapters_unchecked or (tag == BF16 and m > ADAPTERS_FEW_ROWS)
+
+
+_adapters_unchecked = False
+
+
+def adapters_status() -> int:
+    """0, or which bounded wait of an :func:`add_adapters` launch gave up since the last call (the results of that launch are not
+    valid).  Synchronises the device; reading clears the record."""
+    global _adapters_unchecked
+    _adapters_unchecked = False
+    return _fn("adapters", "tvb_adapters_status", [])()
 
 
 # ------------------------------------------ attention over keys in common (paged)
@@ -2811,4 +2825,9 @@ def check_finished_launches() -> None:
         status = attention_shared_status()
         if status:
             raise KernelError(f"attention_shared: a wait inside the kernel ran out (code {status}); "
+                              "the results of this step are not valid")
+    if _adapters_unchecked:
+        status = adapters_status()
+        if status:
+            raise KernelError(f"add_adapters: a wait inside the kernel ran out (code {status}); "
                               "the results of this step are not valid")
