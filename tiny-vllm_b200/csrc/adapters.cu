@@ -35,14 +35,18 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// values at, .., at + 7 of a row of `size` (zeros past its end, or where the row is not there)
-template <bool WIDE> __device__ __forceinline__ uint4 load_8(const bf16* row, int at, int size, bool there) {
+// values at, .., at + 7 of a row of `size` (zeros past its end, or where the row is not there); L2: past L1
+template <bool WIDE, bool L2 = false> __device__ __forceinline__ uint4 load_8(const bf16* row, int at, int size, bool there) {
     if constexpr (WIDE) {                       // size is a multiple of 8, the row lies on 16 bytes
-        return there && at < size ? *reinterpret_cast<const uint4*>(row + at) : make_uint4(0, 0, 0, 0);
+        const uint4* from = reinterpret_cast<const uint4*>(row + at);
+        return !there || at >= size ? make_uint4(0, 0, 0, 0) : L2 ? __ldcg(from) : *from;
     } else {
         uint32_t h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = there && at + e < size ? (uint32_t)reinterpret_cast<const unsigned short*>(row)[at + e] : 0u;
+        for (int e = 0; e < 8; ++e) {
+            const unsigned short* from = reinterpret_cast<const unsigned short*>(row) + at + e;
+            h[e] = !there || at + e >= size ? 0u : L2 ? (uint32_t)__ldcg(from) : (uint32_t)*from;
+        }
         return make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
     }
 }
@@ -78,7 +82,7 @@ template <int ROWS> __device__ __forceinline__ int find_adapters(const int* all,
     __shared__ int counts[2];
     const int tid = threadIdx.x;
     if (tid < ROWS) {
-        const int id = row0 + tid < m ? all[row0 + tid] : -1;
+        const int id = row0 + tid < m ? __ldcg(all + row0 + tid) : -1;
         ids[tid] = (unsigned)id < (unsigned)adapters ? id : -1;
     }
     if (tid < 2) counts[tid] = 0;
@@ -290,34 +294,37 @@ struct Expand {
     void* y;
     int64_t ldy;
     int m, n, rank, adapters;
-    int columns_apart;
 };
 
 // A warp has 16 rows of y and walks over tiles of 32 columns, one adapter of its rows after another (those of few rows side by
 // side in the grid): the rows' u stays in registers, y and B of the next tile are asked for before this one's products.  A thread
 // takes 16 bytes, eight neighbouring ranks, of a row of B and of u (which rank a fragment's place stands for is permuted alike in
 // both).  The columns of an n-tile are spread so that a thread holds eight neighbours of y: place c of tile j is column
-// (c / 2) * 8 + 2 j + c % 2.  The warps of a CTA have different columns of the same rows (`columns_apart`, few rows), or different
-// rows and the same columns, whose B they find in L1.
-template <typename Y, bool WIDE>
+// (c / 2) * 8 + 2 j + c % 2.  The warps of a CTA have different columns of the same rows (FEW rows), or different rows and the
+// same columns, whose B they find in L1.
+//
+// All that comes from before `shrink` (whose threads wait for it before they let this kernel start) may be read before `shrink` is
+// through: ids, and with FEW rows the first tiles of y and B, past L1.  u may not, and nothing is written before.
+template <typename Y, bool WIDE, bool FEW>
 __global__ void __launch_bounds__(THREADS, 4) expand_kernel(Expand s) {
     constexpr int ROWS = 16, NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;     // steps of 32 ranks held; 16-byte words of eight values of y
     const int padded = padded_rank(s.rank);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = (s.columns_apart ? blockIdx.y : blockIdx.y * WARPS + warp) * ROWS;
-    const int first_tile = s.columns_apart ? blockIdx.x * WARPS + warp : blockIdx.x;
-    const int step = s.columns_apart ? gridDim.x * WARPS : gridDim.x, tiles = (s.n + 31) / 32;
-    pdl_wait();
-    pdl_launch_dependents();
-    if (row0 >= s.m || first_tile >= tiles) return;
+    const int row0 = (FEW ? blockIdx.y : blockIdx.y * WARPS + warp) * ROWS;
+    const int first_tile = FEW ? blockIdx.x * WARPS + warp : blockIdx.x;
+    const int step = FEW ? gridDim.x * WARPS : gridDim.x, tiles = (s.n + 31) / 32;
     int id = -1;
-    if (lane < ROWS && row0 + lane < s.m) {
-        id = s.ids[row0 + lane];
+    if (lane < ROWS && row0 + lane < s.m && first_tile < tiles) {
+        id = __ldcg(s.ids + row0 + lane);
         if ((unsigned)id >= (unsigned)s.adapters) id = -1;
     }
     const uint32_t alike = __match_any_sync(0xffffffffu, id);
     uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
     for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
+    if (!FEW || leaders == 0) {                 // (a thread that has nothing to do waits too: what follows relies on this kernel's end)
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     while (leaders) {
         const int leader = __ffs(leaders) - 1;
         for (int d = 0; d < (int)gridDim.z; ++d) leaders &= leaders - 1;
@@ -345,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_kernel(Expand s) {
             for (int h = 0; h < 2; ++h)
                 if (WIDE && rows >> (8 * h) & 1 && tile * 32 + 8 * t + 8 <= s.n)
 #pragma unroll
-                    for (int q = 0; q < WORDS; ++q) old[h][q] = reinterpret_cast<const uint4*>(y + 8 * h * s.ldy + tile * 32)[q];
+                    for (int q = 0; q < WORDS; ++q) old[h][q] = __ldcg(reinterpret_cast<const uint4*>(y + 8 * h * s.ldy + tile * 32) + q);
         };
         uint4 w[STEPS][NT];
         auto load_b = [&](int tile, int r0) {
@@ -354,11 +361,15 @@ __global__ void __launch_bounds__(THREADS, 4) expand_kernel(Expand s) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-                    w[k][j] = load_8<WIDE>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
+                    w[k][j] = load_8<WIDE, FEW>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
                 }
         };
         load_y(first_tile);
         load_b(first_tile, 0);
+        if (FEW) {
+            pdl_wait();
+            pdl_launch_dependents();
+        }
         load_u(0);
         for (int tile = first_tile; tile < tiles; tile += step) {
             float sums[NT][4] = {};
@@ -483,18 +494,23 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
     __shared__ int ids[ROWS], distinct[ROWS];
     float* u = reinterpret_cast<float*>(raw);                                   // [ROWS][rank]
     const int row0 = blockIdx.y * ROWS, rows = min(ROWS, s.m - row0), column = blockIdx.x * THREADS + threadIdx.x;
+    // before `shrink` is through (see expand_kernel): the adapters, y, and B on its way into L2
+    const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
+    float* y = reinterpret_cast<float*>(s.y) + (int64_t)row0 * s.ldy + column;
+    float old[ROWS];
+#pragma unroll
+    for (int row = 0; row < ROWS; ++row) old[row] = column < s.n && ids[row] >= 0 ? __ldcg(y + row * s.ldy) : 0.0f;
+    if (column < s.n)
+        for (int d = 0; d < count; ++d)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const float*>(s.up) + ((int64_t)distinct[d] * s.n + column) * s.rank));
     pdl_wait();
     pdl_launch_dependents();
     for (int i = threadIdx.x; i < rows * s.rank; i += THREADS) u[i] = reinterpret_cast<const float*>(s.u)[(int64_t)row0 * s.rank + i];
-    const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
+    __syncthreads();
     if (column >= s.n) return;
     for (int d = 0; d < count; ++d) {
         const int adapter = distinct[d];
         const float* b = reinterpret_cast<const float*>(s.up) + ((int64_t)adapter * s.n + column) * s.rank;
-        float* y = reinterpret_cast<float*>(s.y) + (int64_t)row0 * s.ldy + column;
-        float sums[ROWS];
-#pragma unroll
-        for (int row = 0; row < ROWS; ++row) sums[row] = ids[row] == adapter ? y[row * s.ldy] : 0.0f;
         float total[ROWS] = {};
 #pragma unroll 2
         for (int r = 0; r < s.rank; r += VEC) {
@@ -508,7 +524,7 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
         }
 #pragma unroll
         for (int row = 0; row < ROWS; ++row)
-            if (ids[row] == adapter) y[row * s.ldy] = sums[row] + total[row];
+            if (ids[row] == adapter) y[row * s.ldy] = old[row] + total[row];
     }
 }
 
@@ -535,13 +551,13 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
                 : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-template <typename Y> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
+template <typename Y, bool FEW> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
     // few rows: a tile of 32 columns a warp; more: several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us
     // with three CTAs an SM, 34 with six, 33 with twelve)
-    const int tiles = ceil_div(a.n, 32), rows = ceil_div(a.m, a.columns_apart ? 16 : 16 * WARPS);
-    const int across = a.columns_apart ? ceil_div(tiles, WARPS) : min(tiles, max(1, 12 * 148 / rows));
+    const int tiles = ceil_div(a.n, 32), rows = ceil_div(a.m, FEW ? 16 : 16 * WARPS);
+    const int across = FEW ? ceil_div(tiles, WARPS) : min(tiles, max(1, 12 * 148 / rows));
     const dim3 grid(across, rows, side_by_side);
-    return wide ? launch(expand_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<Y, false>, grid, 0, 0, pdl, s, a);
+    return wide ? launch(expand_kernel<Y, true, FEW>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<Y, false, FEW>, grid, 0, 0, pdl, s, a);
 }
 
 }  // namespace
@@ -584,7 +600,7 @@ int shrink(const void* x, long long ldx, const void* down, const int* ids, const
 int expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank, int adapters, int dtype, int y_dtype,
            int pdl, cudaStream_t s) {
     const bool few = m <= FEW_ROWS;
-    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters, few};
+    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters};
     if (dtype == TVB_F32) {
         if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
         const dim3 grid(ceil_div(n, THREADS), ceil_div(m, 16));
@@ -596,8 +612,9 @@ int expand(const void* u, const void* up, const int* ids, void* y, long long ldy
     const int size = y_dtype == TVB_F32 ? 4 : 2;
     const bool wide = rank % 8 == 0 && !((uintptr_t)up & 15) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
     const int side_by_side = min(few ? min(16, m) : 2, adapters);
-    if (y_dtype == TVB_F32) return launch_expand<float>(a, wide, side_by_side, pdl, s);
-    return y_dtype == TVB_BF16 ? launch_expand<bf16>(a, wide, side_by_side, pdl, s) : TVB_BAD_ARGUMENT;
+    if (y_dtype != TVB_F32 && y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
+    if (few) return y_dtype == TVB_F32 ? launch_expand<float, true>(a, wide, side_by_side, pdl, s) : launch_expand<bf16, true>(a, wide, side_by_side, pdl, s);
+    return y_dtype == TVB_F32 ? launch_expand<float, false>(a, wide, side_by_side, pdl, s) : launch_expand<bf16, false>(a, wide, side_by_side, pdl, s);
 }
 
 }  // namespace
@@ -625,7 +642,7 @@ extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
         adapters_tma_takes(c.x, c.ldx, c.down, c.up, c.y, c.ldy, c.k, c.n, c.rank, c.adapters, c.y_dtype)) {
         const int e = shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0},
                                  c.pdl, s);
-        return e ? e : expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, 0}, c.pdl, s);
+        return e ? e : expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters}, c.pdl, s);
     }
     const int e = shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
     return e ? e : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);

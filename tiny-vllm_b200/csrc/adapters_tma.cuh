@@ -184,9 +184,12 @@ __global__ void __launch_bounds__(TMA_THREADS, 4) expand_tma_kernel(const __grid
         prefetch_tensormap(&map_out);
         prefetch_tensormap(&map_b);
     }
-    pdl_wait();
-    pdl_launch_dependents();
+    // (before `shrink` is through, see expand_kernel: the adapters here, the first tiles of y and B below)
     const int count = find_adapters<TMA_ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);       // (its barriers: ours are set up)
+    if (warp < WARPS || count == 0) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
     if (count == 0) return;                     // the whole CTA
     if (warp == WARPS) {
         if (lane == 0) {

@@ -95,7 +95,8 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     if out is not None and (out.shape != (m, n) or out.dtype != out_dtype or out.stride(1) != 1 and n > 1
                             or m > 1 and out.stride(0) < n or any(kernels._overlaps(out, t) for t in (x, weight, down, up))):
         raise kernels.KernelError(f"linear_adapted: out must be {out_dtype} [{m}, {n}] with contiguous rows, in memory of its own")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, down, up, scales, out)):
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or down.requires_grad or up.requires_grad
+                                    or scales is not None and scales.requires_grad or out is not None and out.requires_grad):
         raise kernels.KernelError("linear_adapted has no backward pass: call it under torch.no_grad() or torch.inference_mode()")
     stream = kernels._here("linear_adapted", x, weight, down, up, ids, scales, out)
     if m == 0 or n == 0:
