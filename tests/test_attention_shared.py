@@ -45,3 +45,11 @@ def test_refusals(changed):
     with pytest.raises(kernels.KernelError) as refusal:
         call(good() | changed)
     assert "CUDA tensors only" not in str(refusal.value)
+
+
+@pytest.mark.parametrize("of", ["q", "key_cache", "value_cache"])
+def test_a_result_in_memory_that_is_read(of):
+    arguments = good()
+    memory = arguments[of].view(-1)
+    with pytest.raises(kernels.KernelError, match="memory of its own"):
+        call(arguments | dict(out=memory[: 3 * 256].view(3, 256)))

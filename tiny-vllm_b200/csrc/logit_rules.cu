@@ -223,8 +223,6 @@ __global__ void append_tokens_kernel(const int* slots, const int* tokens, int ro
 
 }  // namespace
 
-extern "C" int tvb_logit_rules_max_biases() { return MAX_BIASES; }
-
 // The call's arguments as the Python side packs them.
 struct RulesCall {
     const void* logits;
