@@ -89,6 +89,19 @@ def test_more_rows_with_tails_of_every_size(m, k, n, rank):
     check(adapted(**s), s)
 
 
+@pytest.mark.parametrize("rank", [8, 40])
+@pytest.mark.parametrize("adapters", [2, 8, 9, 60])
+@pytest.mark.parametrize("m", [33, 128, 192, 193, 511, 512, 513])
+def test_rows_in_any_order(m, adapters, rank):
+    s = made(m, 200, 168, rank, adapters)
+    got = adapted(**s)
+    check(got, s)
+    order = torch.randperm(m, generator=torch.Generator().manual_seed(m)).to(DEV)
+    other = s | dict(x=s["x"][order], ids=s["ids"][order])
+    check(adapted(**other), other)
+    check(adapted(**other, out_dtype=torch.float32), other)
+
+
 @pytest.mark.parametrize("kind", ["one", "none", "spans"])
 @pytest.mark.parametrize("m", [20, 333])
 def test_which_rows_have_which(kind, m):

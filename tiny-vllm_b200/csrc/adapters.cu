@@ -4,19 +4,21 @@
 //
 // with A [adapters, rank, k] and B [adapters, n, rank].  Two kernels: `shrink` makes u = s x A^T (float32 sums over k in
 // pieces that the CTAs of a cluster add in order, through distributed shared memory), `expand` takes u through B and adds
-// it to y.  Rows come in any order; a tile of rows goes once over every adapter that one of its rows has, the adapters of a
-// tile side by side in the grid as far as it goes.
+// it to y.  Rows come in any order; a tile of rows goes once over every adapter that one of its rows has.
 //
 // bfloat16: mma.sync m16n8k16 (the products are a hundredth of the projection's: what counts is that A, B, x and y come in
-// with enough of them in flight).  Up to FEW_ROWS rows a CTA of `shrink` has 16 rows and loads straight into registers: a
-// thread takes 16 bytes, eight neighbouring k, of each row, and which k a fragment's place stands for is permuted alike in
-// both operands.  More rows go 64 a CTA through a ring in shared memory: tensor-map copies fill it where types, ranks and alignment
-// allow (adapters_tma.cuh, which has its own `expand` too), else cp.async.  u leaves in two bfloat16 whose
-// sum is u to 2^-17 of it, so that no rounding of u is seen beside that of the result.  A row takes the sums of its own
-// adapter alone: what other adapters hold, infinities among them, does not reach it.
+// with enough of them in flight).  Few rows (see rows_go): 16 rows of one adapter a CTA, as they lie or sorted, straight into
+// registers: a thread takes 16 bytes, eight neighbouring k, of each row, and which k a fragment's place stands for is permuted
+// alike in both operands.  More rows go 64 a CTA through a ring in shared memory: tensor-map copies fill it where types, ranks and
+// alignment allow (adapters_tma.cuh, which has its own `expand` too), else cp.async.  u leaves in two bfloat16 whose sum is u
+// to 2^-17 of it, so that no rounding of u is seen beside that of the result.  A row takes the sums of its own adapter
+// alone: what other adapters hold, infinities among them, does not reach it.
 // float32: the float32 cores.
 //
-// Bound by the latency of their chains of loads for few rows, by reading x and reading and writing y for many.
+// Bound by the latency of their chains of loads (ids, A and x, u, B and y) for few rows: one row 1024 -> 4096 of rank 16 takes 4.1 us
+// beside a projection of 2.8, 48 rows 4096 -> 6144 with 13 adapters of rank 16 9.9 us beside 11.6 (7 MB, 1 us at the speed of HBM).
+// Bound by the traffic of x and y and the instructions between it for many: adapters_tma.cuh.  float32, 301 rows 1024 -> 2048 of
+// rank 8: 8 to 10 us beside 25 to 28.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -109,48 +111,31 @@ template <int ROWS> __device__ __forceinline__ int find_adapters(const int* all,
     return counts[0] + counts[1];
 }
 
-// ---- up to FEW_ROWS rows: 16 rows, 16 ranks and one adapter (the blockIdx.z-th of the rows') a CTA, its warps share k
-template <bool WIDE>
-__global__ void __launch_bounds__(THREADS) shrink_few_kernel(Shrink s) {
+// ---- few rows: 16 rows, 16 ranks and a piece of k a CTA, its warps share the piece; the CTAs of a cluster have the pieces
+struct FewShared {
+    float met[WARPS][16][16];
+    float pieces[MAX_SPLITS][16 * 16];          // of the cluster's first CTA
+};
+// u of up to 16 rows of one adapter (lane group g: rows g and g + 8), 16 ranks of it; `row_of` says which row the i-th is, -1: none
+// of this adapter.  The cluster's first barrier has been arrived at, and the one that ends this is left to be waited for.
+template <bool WIDE, typename R> __device__ __forceinline__ void shrink_rows(const Shrink& s, int adapter, int rank0, const R& row_of, FewShared& shared) {
     constexpr int NR = 2, AHEAD = 4;            // groups of 8 ranks; blocks of 32 k in flight
-    __shared__ float met[WARPS][16][8 * NR];
-    __shared__ float pieces[MAX_SPLITS][16 * 8 * NR];                           // of the cluster's first CTA
     cg::cluster_group cluster = cg::this_cluster();
-    cluster_arrive_relaxed();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x % s.splits, rank0 = blockIdx.x / s.splits * 8 * NR, ranks = s.rank - rank0;
-    const int row0 = blockIdx.y * 16;
+    const int split = blockIdx.x % s.splits, ranks = s.rank - rank0, padded = padded_rank(s.rank);
     const int end = min((s.k + 31) / 32, (split + 1) * s.per_split);
-    pdl_wait();
-    pdl_launch_dependents();
-    // lanes 0 .. 15: a row's adapter, and the rows that share it
-    int id = -1;
-    if (lane < 16 && row0 + lane < s.m) {
-        id = s.ids[row0 + lane];
-        if ((unsigned)id >= (unsigned)s.adapters) id = -1;
-    }
-    const uint32_t alike = __match_any_sync(0xffffffffu, id);
-    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
-    for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
-    if (leaders == 0) {                         // the whole cluster
-        cluster_wait();
-        return;
-    }
-    const int leader = __ffs(leaders) - 1;
-    const int adapter = __shfl_sync(0xffffffffu, id, leader);
-    const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader);
     const bf16* down = s.down + ((int64_t)adapter * s.rank + rank0) * s.k;
-    const bool lo_there = rows >> g & 1, hi_there = rows >> (g + 8) & 1;
-    const bf16* lo = s.x + (int64_t)(row0 + g) * s.ldx;
-    const bf16* hi = s.x + (int64_t)(row0 + g + 8) * s.ldx;
+    const int lo_row = row_of(g), hi_row = row_of(g + 8);
+    const bf16* lo = s.x + max(lo_row, 0) * s.ldx;
+    const bf16* hi = s.x + max(hi_row, 0) * s.ldx;
     float sums[NR][4] = {};
     for (int b0 = split * s.per_split + warp; b0 < end; b0 += AHEAD * WARPS) {
         uint4 xl[AHEAD], xh[AHEAD], w[AHEAD][NR];
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             const int b = b0 + i * WARPS, at = b * 32 + 8 * t;
-            xl[i] = load_8<WIDE>(lo, at, s.k, lo_there && b < end);
-            xh[i] = load_8<WIDE>(hi, at, s.k, hi_there && b < end);
+            xl[i] = load_8<WIDE>(lo, at, s.k, lo_row >= 0 && b < end);
+            xh[i] = load_8<WIDE>(hi, at, s.k, hi_row >= 0 && b < end);
 #pragma unroll
             for (int j = 0; j < NR; ++j)
                 w[i][j] = load_8<WIDE>(down + (int64_t)(8 * j + g) * s.k, at, s.k, 8 * j + g < ranks && b < end);
@@ -166,29 +151,180 @@ __global__ void __launch_bounds__(THREADS) shrink_few_kernel(Shrink s) {
 #pragma unroll
     for (int j = 0; j < NR; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) met[warp][e < 2 ? g : g + 8][8 * j + 2 * t + (e & 1)] = sums[j][e];
+        for (int e = 0; e < 4; ++e) shared.met[warp][e < 2 ? g : g + 8][8 * j + 2 * t + (e & 1)] = sums[j][e];
     __syncthreads();
-    cluster_wait();                             // the first CTA runs
-    float* first_pieces = cluster.map_shared_rank(&pieces[0][0], 0);
+    cluster_wait();                             // the first CTA runs, and is through with the pieces before
+    float* first_pieces = cluster.map_shared_rank(&shared.pieces[0][0], 0);
     for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
         const int row = i / (8 * NR), rank = i % (8 * NR);
-        float sum = met[0][row][rank];
+        float sum = shared.met[0][row][rank];
 #pragma unroll
-        for (int w = 1; w < WARPS; ++w) sum += met[w][row][rank];
+        for (int w = 1; w < WARPS; ++w) sum += shared.met[w][row][rank];
         first_pieces[split * 16 * 8 * NR + i] = sum;
     }
     cluster_arrive();
     cluster_wait();
-    if (split != 0) return;
-    const float scale = s.scales ? s.scales[adapter] : 1.0f;
-    const int padded = padded_rank(s.rank);
-    for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
-        const int row = i / (8 * NR), rank = i % (8 * NR);
-        if (!(rows >> row & 1)) continue;
-        float sum = pieces[0][i];
-        for (int p = 1; p < s.splits; ++p) sum += pieces[p][i];
-        store_u(s.u, row0 + row, rank0 + rank, padded, rank < ranks ? sum * scale : 0.0f);
+    if (split == 0) {
+        const float scale = s.scales ? s.scales[adapter] : 1.0f;
+        for (int i = threadIdx.x; i < 16 * 8 * NR; i += THREADS) {
+            const int rank = i % (8 * NR), row = row_of(i / (8 * NR));
+            if (row < 0) continue;
+            float sum = shared.pieces[0][i];
+            for (int p = 1; p < s.splits; ++p) sum += shared.pieces[p][i];
+            store_u(s.u, row, rank0 + rank, padded, rank < ranks ? sum * scale : 0.0f);
+        }
     }
+    cluster_arrive();
+}
+
+// The d-th adapter of 16 rows as they lie, in the order of the rows: its number, -1: none; `mask`: which of the rows have it.
+// A whole warp calls.
+__device__ __forceinline__ int find_adapter(const int* all, int m, int adapters, int row0, int d, uint32_t& mask) {
+    const int lane = threadIdx.x & 31;
+    int id = -1;
+    if (lane < 16 && row0 + lane < m) {
+        id = __ldcg(all + row0 + lane);
+        if ((unsigned)id >= (unsigned)adapters) id = -1;
+    }
+    const uint32_t alike = __match_any_sync(0xffffffffu, id);
+    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
+    for (; d > 0; --d) leaders &= leaders - 1;
+    const int leader = leaders ? __ffs(leaders) - 1 : 31;
+    mask = __shfl_sync(0xffffffffu, alike, leader);
+    return __shfl_sync(0xffffffffu, id, leader);
+}
+
+// rows as they lie, the blockIdx.z-th of their adapters
+template <bool WIDE> __global__ void __launch_bounds__(THREADS) shrink_few_kernel(Shrink s) {
+    __shared__ FewShared shared;
+    cluster_arrive_relaxed();
+    const int rank0 = blockIdx.x / s.splits * 16, row0 = blockIdx.y * 16;
+    pdl_wait();
+    pdl_launch_dependents();
+    uint32_t rows;
+    const int adapter = find_adapter(s.ids, s.m, s.adapters, row0, blockIdx.z, rows);
+    if (adapter >= 0)                           // the same for the whole cluster
+        shrink_rows<WIDE>(s, adapter, rank0, [&](int i) { return rows >> i & 1 ? row0 + i : -1; }, shared);
+    cluster_wait();
+}
+
+// ---- some more rows, and more than a few adapters: chunks of up to 16 rows with one adapter
+//
+// The rows of a decode step come in any order (as its requests were admitted).  Every CTA sorts them by their adapters for itself,
+// in shared memory, and takes chunks of rows that share one, so that an adapter is read once for 16 of them however they lie.
+// Adapters come in the order of their first rows, and their rows as they lie, so that all CTAs agree.
+constexpr int MAX_SORTED_ROWS = 512, TABLE = 2 * MAX_SORTED_ROWS, SORTED_BLOCKS = MAX_SORTED_ROWS / 32;
+static_assert(SORTED_BLOCKS == 16 && TABLE == 1 << 10, "a byte of a uint4 a block of 32 rows, 10 bits of a hash");
+struct Sorted {
+    uint4 counts[TABLE];                        // rows of a hashed adapter in every block of 32 rows, a byte each
+    int keys[TABLE];                            // the adapter, -1: none; then its first chunk and, << 16, place
+    int of_rows[MAX_SORTED_ROWS];               // a row's adapter, -1: none
+    int slots[MAX_SORTED_ROWS];                 // a row's place in the table, and how many rows before have its adapter << 16
+    int sums[SORTED_BLOCKS];
+    int ids[MAX_SORTED_ROWS];                   // a chunk's adapter
+    int starts[MAX_SORTED_ROWS];                // its place among the sorted rows, and how many they are << 16
+    unsigned short rows[MAX_SORTED_ROWS];       // sorted
+    __device__ __forceinline__ int row(int chunk, int i) const { return i < starts[chunk] >> 16 ? rows[(starts[chunk] & 0xffff) + i] : -1; }
+};
+// How many chunks there are.  All threads call.  (Loops as they are: code that runs once is read as slowly as it is long.)
+__device__ __forceinline__ int sort_rows(const int* all, int m, int adapters, Sorted& c) {
+    const int tid = threadIdx.x, lane = tid & 31, padded = (m + 31) / 32 * 32;
+    const uint32_t lower = (1u << lane) - 1u;
+#pragma unroll 1
+    for (int row = tid; row < padded; row += THREADS) {
+        const int id = row < m ? __ldcg(all + row) : -1;
+        c.of_rows[row] = (unsigned)id < (unsigned)adapters ? id : -1;
+    }
+#pragma unroll 1
+    for (int i = tid; i < TABLE; i += THREADS) {
+        c.keys[i] = -1;
+        c.counts[i] = make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int row = tid; row < padded; row += THREADS) {                         // (whole warps)
+        const int id = c.of_rows[row];
+        const uint32_t alike = __match_any_sync(0xffffffffu, id);
+        const int rank = __popc(alike & lower);
+        int at = (int)((uint32_t)id * 0x9e3779b1u >> 22);
+        if (id >= 0 && rank == 0) {
+            for (;;) {                          // half of the table at least stays empty
+                const int held = atomicCAS(c.keys + at, -1, id);
+                if (held == -1 || held == id) break;
+                at = (at + 1) & (TABLE - 1);
+            }
+            reinterpret_cast<unsigned char*>(c.counts + at)[row / 32] = (unsigned char)__popc(alike);
+        }
+        c.slots[row] = __shfl_sync(0xffffffffu, at, __ffs(alike) - 1) | rank << 16;
+    }
+    __syncthreads();
+    // rows and chunks of the adapters that begin at a row, added up over the rows
+#pragma unroll 1
+    for (int row = tid; row < padded; row += THREADS) {
+        const int block = row / 32, slot = c.slots[row] & 0xffff;
+        int sum = 0;
+        if (c.of_rows[row] >= 0) {
+            const uint4 of = c.counts[slot];
+            const uint32_t words[4] = {of.x, of.y, of.z, of.w};
+            uint32_t before = 0, total = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int bytes = block - 4 * w;
+                total = __dp4a(words[w], 0x01010101u, total);
+                before = __dp4a(bytes >= 4 ? words[w] : bytes <= 0 ? 0u : words[w] & ((1u << (8 * bytes)) - 1u), 0x01010101u, before);
+            }
+            const int rank = (c.slots[row] >> 16) + before;
+            c.slots[row] = slot | rank << 16;
+            if (rank == 0) sum = (total + 15) / 16 | total << 16;
+        }
+        const int own = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        if (own) c.keys[slot] = sum - own;      // (behind the sums of the blocks before)
+        if (lane == 31) c.sums[block] = sum;
+    }
+    __syncthreads();
+    int upto = 0;
+#pragma unroll 1
+    for (int block = 0; block < padded / 32; ++block) {
+        const int row = block * 32 + lane;
+        if (block % WARPS == tid / 32 && c.of_rows[row] >= 0 && c.slots[row] >> 16 == 0) c.keys[c.slots[row]] += upto;
+        upto += c.sums[block];
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int row = tid; row < padded; row += THREADS) {
+        const int id = c.of_rows[row];
+        if (id < 0) continue;
+        const int slot = c.slots[row] & 0xffff, rank = c.slots[row] >> 16, at = c.keys[slot], place = (at >> 16) + rank;
+        c.rows[place] = (unsigned short)row;
+        if (rank % 16 == 0) {
+            const uint4 of = c.counts[slot];
+            const int total = __dp4a(of.x, 0x01010101u, __dp4a(of.y, 0x01010101u, __dp4a(of.z, 0x01010101u, __dp4a(of.w, 0x01010101u, 0u))));
+            c.ids[(at & 0xffff) + rank / 16] = id;
+            c.starts[(at & 0xffff) + rank / 16] = place | min(16, total - rank) << 16;
+        }
+    }
+    __syncthreads();
+    return upto & 0xffff;
+}
+
+template <bool WIDE> __global__ void __launch_bounds__(THREADS) shrink_sorted_kernel(Shrink s) {
+    __shared__ FewShared shared;
+    __shared__ Sorted sorted;
+    cluster_arrive_relaxed();
+    const int rank_chunks = (s.rank + 15) / 16;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int items = sort_rows(s.ids, s.m, s.adapters, sorted) * rank_chunks;
+    for (int item = blockIdx.x / s.splits; item < items; item += gridDim.x / s.splits) {          // the same for the whole cluster
+        const int chunk = item / rank_chunks;
+        shrink_rows<WIDE>(s, sorted.ids[chunk], item % rank_chunks * 16, [&](int i) { return sorted.row(chunk, i); }, shared);
+    }
+    cluster_wait();
 }
 
 // ---- more rows: 64 rows and RANKS ranks a CTA, 16 rows a warp; stages of 64 k
@@ -296,141 +432,184 @@ struct Expand {
     int m, n, rank, adapters;
 };
 
-// A warp has 16 rows of y and walks over tiles of 32 columns, one adapter of its rows after another (those of few rows side by
-// side in the grid): the rows' u stays in registers, y and B of the next tile are asked for before this one's products.  A thread
-// takes 16 bytes, eight neighbouring ranks, of a row of B and of u (which rank a fragment's place stands for is permuted alike in
-// both).  The columns of an n-tile are spread so that a thread holds eight neighbours of y: place c of tile j is column
-// (c / 2) * 8 + 2 j + c % 2.  The warps of a CTA have different columns of the same rows (FEW rows), or different rows and the
-// same columns, whose B they find in L1.
+// A warp has 16 rows of y with one adapter and walks over tiles of 32 columns: the rows' u stays in registers, y and B of the next tile
+// are asked for before this one's products.  A thread takes 16 bytes, eight neighbouring ranks, of a row of B and of u (which rank
+// a fragment's place stands for is permuted alike in both).  The columns of an n-tile are spread so that a thread holds eight
+// neighbours of y: place c of tile j is column (c / 2) * 8 + 2 j + c % 2.
 //
 // All that comes from before `shrink` (whose threads wait for it before they let this kernel start) may be read before `shrink` is
-// through: ids, and with FEW rows the first tiles of y and B, past L1.  u may not, and nothing is written before.
-template <typename Y, bool WIDE, bool FEW>
-__global__ void __launch_bounds__(THREADS, 4) expand_kernel(Expand s) {
-    constexpr int ROWS = 16, NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;     // steps of 32 ranks held; 16-byte words of eight values of y
-    const int padded = padded_rank(s.rank);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = (FEW ? blockIdx.y : blockIdx.y * WARPS + warp) * ROWS;
-    const int first_tile = FEW ? blockIdx.x * WARPS + warp : blockIdx.x;
-    const int step = FEW ? gridDim.x * WARPS : gridDim.x, tiles = (s.n + 31) / 32;
+// through: ids, and where EARLY says so the first tiles of y and B, past L1.  u may not, and nothing is written before.
+template <typename Y, bool WIDE, bool EARLY>
+__device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const int (&row)[2], const bool (&there)[2], int first_tile, int end, int step) {
+    constexpr int NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;                     // steps of 32 ranks held; 16-byte words of eight values of y
+    const int padded = padded_rank(s.rank), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
+    const bf16* u[2];
+    Y* y[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        u[h] = reinterpret_cast<const bf16*>(s.u) + (int64_t)row[h] * 2 * padded;
+        y[h] = reinterpret_cast<Y*>(s.y) + row[h] * s.ldy + 8 * t;
+    }
+    uint4 held[STEPS][2][2];                    // u of rows g + 8 h, its heads and its rests
+    auto load_u = [&](int r0) {
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const int at = r0 + 32 * k + 8 * t;
+                    held[k][h][q] = there[h] && at < padded ? *reinterpret_cast<const uint4*>(u[h] + q * padded + at) : make_uint4(0, 0, 0, 0);
+                }
+    };
+    uint4 old[2][WORDS];                        // of y
+    auto load_y = [&](int tile) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            if (WIDE && there[h] && tile * 32 + 8 * t + 8 <= s.n)
+#pragma unroll
+                for (int q = 0; q < WORDS; ++q) old[h][q] = __ldcg(reinterpret_cast<const uint4*>(y[h] + tile * 32) + q);
+    };
+    uint4 w[STEPS][NT];
+    auto load_b = [&](int tile, int r0) {
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
+                w[k][j] = load_8<WIDE, EARLY>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
+            }
+    };
+    load_y(first_tile);
+    load_b(first_tile, 0);
+    if (EARLY) {
+        pdl_wait();
+        pdl_launch_dependents();
+    }
+    load_u(0);
+    for (int tile = first_tile; tile < end; tile += step) {
+        float sums[NT][4] = {};
+        for (int r0 = 0; r0 < padded; r0 += 32 * STEPS) {
+            if (padded > 32 * STEPS && (r0 > 0 || tile != first_tile)) {
+                load_u(r0);
+                if (r0 > 0) load_b(tile, r0);
+            }
+#pragma unroll
+            for (int k = 0; k < STEPS; ++k) {
+                if (r0 + 32 * k >= padded) break;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const uint4 &lo = held[k][0][q], &hi = held[k][1][q];
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        mma_16816(sums[j], lo.x, hi.x, lo.y, hi.y, w[k][j].x, w[k][j].y);
+                        mma_16816(sums[j], lo.z, hi.z, lo.w, hi.w, w[k][j].z, w[k][j].w);
+                    }
+                }
+            }
+        }
+        uint4 now[2][WORDS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int q = 0; q < WORDS; ++q) now[h][q] = old[h][q];
+        if (tile + step < end) {
+            load_y(tile + step);
+            load_b(tile + step, 0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (!there[h]) continue;
+            Y* to = y[h] + tile * 32;
+            float add[8];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
+            if (WIDE && tile * 32 + 8 * t + 8 <= s.n) {
+                if constexpr (sizeof(Y) == 2) {
+                    float v[8];
+                    unpack_bf16x8(now[h][0], v);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) add[e] += v[e];
+                    *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint4 v = now[h][q];
+                        reinterpret_cast<float4*>(to)[q] =
+                            make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
+                                        __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (tile * 32 + 8 * t + e < s.n) to[e] = from_float<Y>(to_float<Y>(to[e]) + add[e]);
+            }
+        }
+    }
+}
+
+// few rows: 16 rows as they lie, the blockIdx.z-th of their adapters, a tile of 32 columns a warp
+template <typename Y, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
+    const int tile = blockIdx.x * WARPS + (threadIdx.x >> 5), row0 = blockIdx.y * 16, g = (threadIdx.x & 31) >> 2;
+    uint32_t rows;
+    const int adapter = find_adapter(s.ids, s.m, s.adapters, row0, blockIdx.z, rows);
+    if (adapter >= 0 && tile * 32 < s.n) {
+        const bool there[2] = {(bool)(rows >> g & 1), (bool)(rows >> (g + 8) & 1)};
+        const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
+        expand_rows<Y, WIDE, true>(s, adapter, row, there, tile, tile + 1, 1);
+    } else {
+        pdl_wait();                             // (a warp that has nothing to do waits too: what follows relies on this kernel's end)
+        pdl_launch_dependents();
+    }
+}
+
+// rows sorted into chunks: a chunk and a strip of its columns a CTA, as many strips as fill the GPU; the warps take every fourth tile
+// of the strip
+template <typename Y, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
+    __shared__ Sorted sorted;
+    const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, tiles = (s.n + 31) / 32;
+    const int count = sort_rows(s.ids, s.m, s.adapters, sorted);
+    const int strips = max(1, min((tiles + WARPS - 1) / WARPS, (int)gridDim.x / max(count, 1))), per = (tiles + strips - 1) / strips;
+    for (int item = blockIdx.x; item < count * strips; item += gridDim.x) {
+        const int chunk = item % count, first = item / count * per + warp, end = min(tiles, (item / count + 1) * per);
+        int row[2] = {sorted.row(chunk, g), sorted.row(chunk, g + 8)};
+        const bool there[2] = {row[0] >= 0, row[1] >= 0};
+        row[0] = max(row[0], 0);
+        row[1] = max(row[1], 0);
+        if (first < end) expand_rows<Y, WIDE, true>(s, sorted.ids[chunk], row, there, first, end, WARPS);
+    }
+    pdl_wait();                                 // (see above)
+    pdl_launch_dependents();
+}
+
+// more rows: the warps of a CTA have 16 rows each as they lie and the same columns, whose B they find in L1; one adapter of the rows
+// after another
+template <typename Y, bool WIDE>
+__global__ void __launch_bounds__(THREADS, 4) expand_many_kernel(Expand s) {
+    constexpr int ROWS = 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    const int row0 = (blockIdx.y * WARPS + warp) * ROWS, tiles = (s.n + 31) / 32;
     int id = -1;
-    if (lane < ROWS && row0 + lane < s.m && first_tile < tiles) {
+    if (lane < ROWS && row0 + lane < s.m) {
         id = __ldcg(s.ids + row0 + lane);
         if ((unsigned)id >= (unsigned)s.adapters) id = -1;
     }
     const uint32_t alike = __match_any_sync(0xffffffffu, id);
     uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
     for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
-    if (!FEW || leaders == 0) {                 // (a thread that has nothing to do waits too: what follows relies on this kernel's end)
-        pdl_wait();
-        pdl_launch_dependents();
-    }
+    pdl_wait();
+    pdl_launch_dependents();
     while (leaders) {
         const int leader = __ffs(leaders) - 1;
         for (int d = 0; d < (int)gridDim.z; ++d) leaders &= leaders - 1;
-        const int adapter = __shfl_sync(0xffffffffu, id, leader);
-        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader) >> g;     // bit 8 h: row g + 8 h is this adapter's
-        const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
-        const bf16* u = reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + g) * 2 * padded;
-        Y* y = reinterpret_cast<Y*>(s.y) + (int64_t)(row0 + g) * s.ldy + 8 * t;
-        uint4 held[STEPS][2][2];           // u of rows g + 8 h, its heads and its rests
-        auto load_u = [&](int r0) {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int at = r0 + 32 * k + 8 * t;
-                        held[k][h][q] = rows >> (8 * h) & 1 && at < padded ? *reinterpret_cast<const uint4*>(u + (int64_t)(16 * h + q) * padded + at)
-                                                                          : make_uint4(0, 0, 0, 0);
-                    }
-        };
-        uint4 old[2][WORDS];               // of y
-        auto load_y = [&](int tile) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                if (WIDE && rows >> (8 * h) & 1 && tile * 32 + 8 * t + 8 <= s.n)
-#pragma unroll
-                    for (int q = 0; q < WORDS; ++q) old[h][q] = __ldcg(reinterpret_cast<const uint4*>(y + 8 * h * s.ldy + tile * 32) + q);
-        };
-        uint4 w[STEPS][NT];
-        auto load_b = [&](int tile, int r0) {
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-                    w[k][j] = load_8<WIDE, FEW>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
-                }
-        };
-        load_y(first_tile);
-        load_b(first_tile, 0);
-        if (FEW) {
-            pdl_wait();
-            pdl_launch_dependents();
-        }
-        load_u(0);
-        for (int tile = first_tile; tile < tiles; tile += step) {
-            float sums[NT][4] = {};
-            for (int r0 = 0; r0 < padded; r0 += 32 * STEPS) {
-                if (padded > 32 * STEPS && (r0 > 0 || tile != first_tile)) {
-                    load_u(r0);
-                    if (r0 > 0) load_b(tile, r0);
-                }
-#pragma unroll
-                for (int k = 0; k < STEPS; ++k) {
-                    if (r0 + 32 * k >= padded) break;
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint4 &lo = held[k][0][q], &hi = held[k][1][q];
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            mma_16816(sums[j], lo.x, hi.x, lo.y, hi.y, w[k][j].x, w[k][j].y);
-                            mma_16816(sums[j], lo.z, hi.z, lo.w, hi.w, w[k][j].z, w[k][j].w);
-                        }
-                    }
-                }
-            }
-            uint4 now[2][WORDS];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int q = 0; q < WORDS; ++q) now[h][q] = old[h][q];
-            if (tile + step < tiles) {
-                load_y(tile + step);
-                load_b(tile + step, 0);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (!(rows >> (8 * h) & 1)) continue;
-                Y* to = y + 8 * h * s.ldy + tile * 32;
-                float add[8];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
-                if (WIDE && tile * 32 + 8 * t + 8 <= s.n) {
-                    if constexpr (sizeof(Y) == 2) {
-                        float v[8];
-                        unpack_bf16x8(now[h][0], v);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) add[e] += v[e];
-                        *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const uint4 v = now[h][q];
-                            reinterpret_cast<float4*>(to)[q] =
-                                make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
-                                            __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (tile * 32 + 8 * t + e < s.n) to[e] = from_float<Y>(to_float<Y>(to[e]) + add[e]);
-                }
-            }
-        }
+        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader) >> g;
+        const bool there[2] = {(bool)(rows & 1), (bool)(rows >> 8 & 1)};
+        const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
+        expand_rows<Y, WIDE, false>(s, __shfl_sync(0xffffffffu, id, leader), row, there, blockIdx.x, tiles, gridDim.x);
     }
 }
 
@@ -531,7 +710,14 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
 #include "adapters_tma.cuh"
 
 // ------------------------------------------------------------------ host side
-constexpr int FEW_ROWS = 128;                   // rows up to which a CTA of `shrink` has 16 rows and one adapter
+// How the rows go: 16 as they lie, sorted by their adapters, or 64 as they lie.  Where there are few adapters, or few rows, the ones a
+// tile meets are read side by side quickly enough; sorting costs 2 us for 48 rows, 8 for 512.  Measured (4096 -> 4096, rank 16, us FEW /
+// SORTED / MANY): 32 adapters in random order, 48 rows 9.0 / 10.2 / 70, 96 rows 13.4 / 11.2 / 76, 256 rows 33 / 14.7 / 79, 512 rows
+// 60 / 22.7 / 102; one after another, 48 rows 8.2 / 10.6 / 80, 96 rows 10.0 / 10.8 / 57, 256 rows 15.0 / 13.5 / 23, 512 rows 24.7 /
+// 18.7 / 18.3; 4 adapters in random order, 192 rows 9.8 / 10.4 / 14.4, 256 rows 11.4 / 12.4 / 14.7, 512 rows 21.3 / 19.2 / 19.5; one
+// after another, 192 rows 6.6 / 10.3 / 8.9, 256 rows 7.4 / 11.9 / 7.5, 512 rows 10.9 / 18.6 / 8.3.
+enum Rows { FEW, SORTED, MANY };
+Rows rows_go(int m, int adapters) { return adapters > 8 && m >= 96 && m <= MAX_SORTED_ROWS ? SORTED : m <= 192 ? FEW : MANY; }
 
 int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
@@ -551,13 +737,20 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
                 : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-template <typename Y, bool FEW> int launch_expand(const Expand& a, bool wide, int side_by_side, int pdl, cudaStream_t s) {
-    // few rows: a tile of 32 columns a warp; more: several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us
-    // with three CTAs an SM, 34 with six, 33 with twelve)
-    const int tiles = ceil_div(a.n, 32), rows = ceil_div(a.m, FEW ? 16 : 16 * WARPS);
-    const int across = FEW ? ceil_div(tiles, WARPS) : min(tiles, max(1, 12 * 148 / rows));
-    const dim3 grid(across, rows, side_by_side);
-    return wide ? launch(expand_kernel<Y, true, FEW>, grid, 0, 0, pdl, s, a) : launch(expand_kernel<Y, false, FEW>, grid, 0, 0, pdl, s, a);
+template <typename Y> int launch_expand(const Expand& a, Rows rows_are, bool wide, int pdl, cudaStream_t s) {
+    const int tiles = ceil_div(a.n, 32);
+    if (rows_are == FEW) {
+        const dim3 grid(ceil_div(tiles, WARPS), ceil_div(a.m, 16), min(min(16, a.m), a.adapters));
+        return wide ? launch(expand_few_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_few_kernel<Y, false>, grid, 0, 0, pdl, s, a);
+    }
+    if (rows_are == SORTED) {
+        const dim3 grid((unsigned)min((long long)a.m * ceil_div(tiles, WARPS), 4ll * 148));       // one round of CTAs, four an SM
+        return wide ? launch(expand_sorted_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_sorted_kernel<Y, false>, grid, 0, 0, pdl, s, a);
+    }
+    // several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us with three CTAs an SM, 34 with six, 33 with twelve)
+    const int rows = ceil_div(a.m, 16 * WARPS);
+    const dim3 grid(min(tiles, max(1, 12 * 148 / rows)), rows, min(2, a.adapters));
+    return wide ? launch(expand_many_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_many_kernel<Y, false>, grid, 0, 0, pdl, s, a);
 }
 
 }  // namespace
@@ -582,12 +775,18 @@ int shrink(const void* x, long long ldx, const void* down, const int* ids, const
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const bool wide = k % 8 == 0 && ldx % 8 == 0 && !(((uintptr_t)x | (uintptr_t)down) & 15);
     Shrink a{(const bf16*)x, ldx, (const bf16*)down, ids, scales, (bf16*)u, m, k, rank, adapters, 1, 0};
-    if (m <= FEW_ROWS) {
+    const Rows rows_are = rows_go(m, adapters);
+    if (rows_are != MANY) {
         // a warp keeps a block of 32 k at least
         while (a.splits < MAX_SPLITS && a.splits * 2 * WARPS <= ceil_div(k, 32)) a.splits *= 2;
         a.per_split = ceil_div(ceil_div(k, 32), a.splits);
-        const dim3 grid(a.splits * ceil_div(rank, 16), ceil_div(m, 16), min(min(16, m), adapters));
-        return wide ? launch(shrink_few_kernel<true>, grid, 0, a.splits, pdl, s, a) : launch(shrink_few_kernel<false>, grid, 0, a.splits, pdl, s, a);
+        const int chunks = ceil_div(rank, 16);
+        if (rows_are == FEW) {
+            const dim3 grid(a.splits * chunks, ceil_div(m, 16), min(min(16, m), adapters));
+            return wide ? launch(shrink_few_kernel<true>, grid, 0, a.splits, pdl, s, a) : launch(shrink_few_kernel<false>, grid, 0, a.splits, pdl, s, a);
+        }
+        const dim3 grid(a.splits * (unsigned)min((long long)m * chunks, 4ll * 148 / a.splits));   // one round of clusters
+        return wide ? launch(shrink_sorted_kernel<true>, grid, 0, a.splits, pdl, s, a) : launch(shrink_sorted_kernel<false>, grid, 0, a.splits, pdl, s, a);
     }
     // pieces of k while the CTAs still have one round on the GPU (three an SM)
     const int chunks = rank <= 16 ? 1 : ceil_div(rank, 64), stages = ceil_div(k, STAGE_K);
@@ -599,7 +798,6 @@ int shrink(const void* x, long long ldx, const void* down, const int* ids, const
 // dtype: of x, A and B; y_dtype: of y (float32 with either, bfloat16 with bfloat16)
 int expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank, int adapters, int dtype, int y_dtype,
            int pdl, cudaStream_t s) {
-    const bool few = m <= FEW_ROWS;
     const Expand a{u, up, ids, y, ldy, m, n, rank, adapters};
     if (dtype == TVB_F32) {
         if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
@@ -611,10 +809,9 @@ int expand(const void* u, const void* up, const int* ids, void* y, long long ldy
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const int size = y_dtype == TVB_F32 ? 4 : 2;
     const bool wide = rank % 8 == 0 && !((uintptr_t)up & 15) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
-    const int side_by_side = min(few ? min(16, m) : 2, adapters);
     if (y_dtype != TVB_F32 && y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    if (few) return y_dtype == TVB_F32 ? launch_expand<float, true>(a, wide, side_by_side, pdl, s) : launch_expand<bf16, true>(a, wide, side_by_side, pdl, s);
-    return y_dtype == TVB_F32 ? launch_expand<float, false>(a, wide, side_by_side, pdl, s) : launch_expand<bf16, false>(a, wide, side_by_side, pdl, s);
+    const Rows rows_are = rows_go(m, adapters);
+    return y_dtype == TVB_F32 ? launch_expand<float>(a, rows_are, wide, pdl, s) : launch_expand<bf16>(a, rows_are, wide, pdl, s);
 }
 
 }  // namespace
@@ -638,7 +835,7 @@ extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
     if (c.m <= 0 || c.n <= 0 || c.adapters <= 0) return 0;
     if (c.k <= 0 || c.rank <= 0 || c.rank > MAX_RANK || ceil_div(c.m, 16) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    if (c.m > FEW_ROWS && c.dtype == TVB_BF16 &&
+    if (c.dtype == TVB_BF16 && rows_go(c.m, c.adapters) == MANY &&
         adapters_tma_takes(c.x, c.ldx, c.down, c.up, c.y, c.ldy, c.k, c.n, c.rank, c.adapters, c.y_dtype)) {
         const int e = shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0},
                                  c.pdl, s);

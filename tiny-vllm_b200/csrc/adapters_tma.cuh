@@ -1,4 +1,4 @@
-// The adapters' two products for more than FEW_ROWS rows (included by adapters.cu): bfloat16, ranks of up to 64 that are a
+// The adapters' two products for many rows as they lie (included by adapters.cu): bfloat16, ranks of up to 64 that are a
 // multiple of 8, operands on 16 bytes.  Tiles come in by tensor-map copies in the 128-byte swizzle that a warp of its own issues,
 // four warps multiply them with mma.sync; full and empty mbarriers between them, every wait bounded (tc5.cuh).
 //

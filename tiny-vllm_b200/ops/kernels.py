@@ -2107,7 +2107,7 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
 
 # ------------------------------------------------------------- low-rank adapters
 ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
-ADAPTERS_FEW_ROWS = 128            # FEW_ROWS there: more rows may go through the kernels with bounded waits
+ADAPTERS_FEW_ROWS = 192            # more rows may go through the kernels with bounded waits there
 
 
 _ADAPTERS_CALL = struct.Struct("@PqPPPPPPqiiiiiiii")
