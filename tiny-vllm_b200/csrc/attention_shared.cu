@@ -291,24 +291,37 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) join_ker
     const int lane = threadIdx.x & 31;
     const int64_t at = (int64_t)blockIdx.x * WARPS + (threadIdx.x >> 5);
     const int token = (int)(at / a.num_q), head = (int)(at % a.num_q), slots = a.shared_pieces + a.own_pieces;
+    // which pieces there are: by what was there before attend_shared, so before this waits
+    int shared_used = 0, own_used = 0;
+    if (token < a.tokens) {
+        const Facts f = facts_of(a, token);
+        if (f.row >= 0) {
+            const int own = f.keys - f.shared;
+            if (f.shared > 0) shared_used = (f.shared - 1) / shared_piece_keys(f.shared, a.shared_pieces) + 1;
+            if (own > 0) own_used = (own - 1) / piece_keys(own, a.own_pieces) + 1;
+        }
+    }
+    const int parts = shared_used + own_used, gap = a.shared_pieces - shared_used;
     pdl_wait();
     pdl_launch_dependents();
     if (token >= a.tokens) return;
     const int64_t first = part_of(a, token, head, 0);
-    // all slots' m and l, whether they have been written or not, beside what says so
     float m[EACH], weight[EACH], top = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const float2 v = lane + 32 * i < slots ? __ldcg(reinterpret_cast<const float2*>(a.part_ml) + first + lane + 32 * i) : make_float2(0, 0);
         m[i] = v.x; weight[i] = v.y;
     }
-    const Facts f = facts_of(a, token);
-    int shared_used = 0, own_used = 0;
-    if (f.row >= 0) {
-        const int own = f.keys - f.shared;
-        if (f.shared > 0) shared_used = (f.shared - 1) / shared_piece_keys(f.shared, a.shared_pieces) + 1;
-        if (own > 0) own_used = (own - 1) / piece_keys(own, a.own_pieces) + 1;
-    }
+    float v[AHEAD][V];
+    const float* from = a.part_o + first * D + lane * V;
+    auto load = [&](int part) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int slot = part + j < shared_used ? part + j : part + j + gap;
+            if (part + j < parts) load_lane<V>(from + (int64_t)slot * D, v[j]);
+        }
+    };
+    load(0);
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const int slot = lane + 32 * i;
@@ -328,15 +341,8 @@ template <typename T, int D> __global__ void __launch_bounds__(THREADS) join_ker
 #pragma unroll
     for (int i = 0; i < EACH; ++i) m[i] *= inverse;
     float sum[V] = {};
-    const float* from = a.part_o + first * D + lane * V;
-    const int parts = shared_used + own_used, gap = a.shared_pieces - shared_used;
     for (int part = 0; part < parts; part += AHEAD) {
-        float v[AHEAD][V];
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) {
-            const int slot = part + j < shared_used ? part + j : part + j + gap;
-            if (part + j < parts) load_lane<V>(from + (int64_t)slot * D, v[j]);
-        }
+        if (part > 0) load(part);
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
             const int slot = part + j < shared_used ? part + j : part + j + gap;
@@ -573,8 +579,8 @@ template <int D> __global__ void __launch_bounds__(THREADS, OwnTiles<D>::CTAS) a
     bf16* q_s = reinterpret_cast<bf16*>(raw);                                   // [16][PITCH]
     bf16* k_s = q_s + 16 * PITCH;                                               // [RING][KEYS][PITCH]
     bf16* v_s = k_s + S::RING * S::TILE;
-    // of a tile's keys: the place of their rows (-1: none), and which there are; four tiles of them, the last being looked up while
-    // a slow warp is still at the first
+    // of a tile's keys: the place of their rows (-1: none), and which there are; eight places, of which four are in use at once: the last
+    // is looked up while a slow warp is still at the first
     int* at_s = reinterpret_cast<int*>(raw + S::BYTES - 8 * S::KEYS * 4 - 8 * 4);                // [8][KEYS]
     uint32_t* there_s = reinterpret_cast<uint32_t*>(at_s + 8 * S::KEYS);        // [8]
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
