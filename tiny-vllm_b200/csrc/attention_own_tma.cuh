@@ -5,6 +5,11 @@
 //
 // Tiles are those of the positions (32 from 0 on), so that boxes lie on the 1024 bytes of the 128-byte swizzle; keys of a tile that
 // are not the piece's get no weight, and their values are zeroed in the fragments (what lies there is of no account).
+//
+// Bound by reading keys and values, of which the 96 KB of the four CTAs' rings are in flight on an SM: whole calls, us with this kernel /
+// with attend_own_bf16_kernel: 60 tokens with up to 431 keys behind 6,144, 32 / 8 heads of size 128, 30.1 / 33.0; three groups of 13 with
+// up to 777 behind 2,896, 64 / 8 heads, 33.8 / 38.9; 2 tokens with 231 keys, 16 / 8 heads, alone 7.6 / 9.8, which is the chain of
+// position, page number, eight tiles one after another and the meeting of the warps.
 #pragma once
 
 template <int D> struct OwnTma {
@@ -18,7 +23,8 @@ template <int D> struct OwnTma {
     static constexpr int THREADS_ALL = THREADS + 32;                            // four warps of products, one of copies
 };
 
-template <int D>
+// SHARED: a piece of a group's shared keys instead, for 16 of the group's query rows.
+template <int D, bool SHARED>
 __global__ void __launch_bounds__(OwnTma<D>::THREADS_ALL, OwnTma<D>::CTAS)
 attend_own_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Attend a) {
     using S = OwnTma<D>;
@@ -43,12 +49,21 @@ attend_own_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
     }
-    start_own(a);
     Piece p;
-    if (!find_own_piece(a, 16, p)) {
-        store_zeros<bf16, D>(a, p);
-        end_own(a);
-        return;
+    uint32_t rows = ~0u;
+    if constexpr (SHARED) {
+        pdl_wait();
+        pdl_launch_dependents();
+        if (!find_shared_piece(a, 16, p)) return;
+        int head;
+        rows = __ballot_sync(0xffffffffu, lane < p.rows && takes_part(a, p, token_of(a, p, min(lane, p.rows - 1), head)));
+    } else {
+        start_own(a);
+        if (!find_own_piece(a, 16, p)) {
+            store_zeros<bf16, D>(a, p);
+            end_own(a);
+            return;
+        }
     }
     const int key0 = p.range.first / S::KEYS * S::KEYS;                          // of the first tile
     const int tiles = (p.range.end - key0 + S::KEYS - 1) / S::KEYS;
@@ -194,20 +209,20 @@ attend_own_tma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             *reinterpret_cast<float2*>(ends.o + row * Ends<D, 16>::PITCH + n * 8 + 2 * t4) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         if (t4 == 0) *reinterpret_cast<float2*>(ends.ml + 2 * row) = make_float2(m[h], l[h]);
     }
-    finish_own<bf16, D, 16>(a, p, ends);
-    end_own(a);
+    finish_own<bf16, D, 16>(a, p, ends, rows);
+    if constexpr (!SHARED) end_own(a);
 }
 
 inline bool own_tma_takes(int page_size) { return page_size >= 8 && page_size <= 128 && (page_size & (page_size - 1)) == 0; }
 
-template <int D> int launch_own_tma(const Attend& a, long long items, int pdl, cudaStream_t stream) {
+template <int D, bool SHARED> int launch_own_tma(const Attend& a, long long items, int pdl, cudaStream_t stream) {
     CUtensorMap map_k, map_v;
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.page_size, (cuuint64_t)a.num_kv, (cuuint64_t)a.pages};
     const cuuint64_t strides[3] = {D * 2, (cuuint64_t)a.page_size * D * 2, (cuuint64_t)a.num_kv * a.page_size * D * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)(a.page_size < OwnTma<D>::KEYS ? a.page_size : OwnTma<D>::KEYS), 1, 1};
     if (!tvb_make_map(&map_k, a.keys, 4, dims, strides, box) || !tvb_make_map(&map_v, a.values, 4, dims, strides, box))
         return (int)cudaErrorNotSupported;
-    auto kernel = attend_own_tma_kernel<D>;
+    auto kernel = attend_own_tma_kernel<D, SHARED>;
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, OwnTma<D>::BYTES);
     if (e != cudaSuccess) return (int)e;
     TvbLaunch at(dim3((unsigned)items), dim3(OwnTma<D>::THREADS_ALL), OwnTma<D>::BYTES, stream, pdl);

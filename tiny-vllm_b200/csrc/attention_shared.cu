@@ -12,11 +12,16 @@
 // so what that wrote is there for both), and one of its CTAs waits for the first's end, so that the third has both behind it.  Where
 // no keys are shared and no token's are cut, attend_own is all there is and stores the result itself.
 //
-// bfloat16: mma.sync m16n8k16 over tiles of 64 keys that cp.async brings two deep; a warp of a shared piece has 16 query
-// rows and every key, the warps of a token's own piece share the keys of a tile among them.  P is rounded to bfloat16 for
-// the second product, the denominator sums what was not rounded.  float32: the float32 cores.
+// bfloat16, as a rule: tcgen05.mma for the shared pieces of head sizes 64 and 128 (attention_shared_tc.cuh), mma.sync on tiles that
+// tensor-map copies bring for tokens' own keys, and for shared pieces of head size 256 (attention_own_tma.cuh).  Pages of other
+// sizes, and 64 query rows of head size 256: mma.sync m16n8k16 over tiles that cp.async brings; a warp of a shared piece has 16
+// query rows and every key, the warps of a token's own piece share the keys of a tile among them.  P is rounded to bfloat16 for the
+// second product, the denominator sums what was not rounded.  float32: the float32 cores.
 //
-// Bound by reading keys and values while a group has few query rows, by the tensor cores once it has many.
+// Bound by reading keys and values while a group has few query rows, by the shared pieces' products once it has many: 60 tokens with up
+// to 431 keys of their own behind 6,144, 32 / 8 heads of size 128, take 30 us for 93 MB, 3.1 TB/s; three groups of 13 with up to 777 behind
+// 2,896, 64 / 8 heads, 34 us for 112 MB, 3.3 TB/s.  What it is above the reading: 3 us before the first key arrives, 3 us for the join,
+// and SMs that wait for the slowest piece.  float32, two groups of 5 behind 608 keys, 16 / 8 heads: 13.5 us for 16 MB.
 #include "common.cuh"
 
 namespace {
@@ -233,14 +238,15 @@ template <typename T, int V> __device__ __forceinline__ void store_lane(T* to, c
     for (int e = 0; e < V; ++e) to[e] = from_float<T>(v[e]);
 }
 
-// Every warp has stored its share (the barrier is here): a warp a row, the warps' shares as one piece, or as the result.
+// Every warp has stored its share (the barrier is here): a warp a row, the warps' shares as one piece, or as the result; `rows`: whose.
 template <typename T, int D, int OWN>
-__device__ __forceinline__ void finish_own(const Attend& a, const Piece& p, const Ends<D, OWN>& ends) {
+__device__ __forceinline__ void finish_own(const Attend& a, const Piece& p, const Ends<D, OWN>& ends, uint32_t rows = ~0u) {
     using E = Ends<D, OWN>;
     constexpr int V = D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __syncthreads();
     for (int r = warp; warp < WARPS && r < p.rows; r += WARPS) {
+        if (!(rows >> r & 1)) continue;
         float top = -INFINITY, total = 0.0f, sum[V] = {};
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ends.ml[2 * (w * OWN + r)]);
@@ -940,17 +946,23 @@ struct Plan {
     int shared_pieces, own_pieces, own_tiles;
     int pieces() const { return shared_pieces + own_pieces; }   // of a row; with 1 there is nothing to join
     int tile_tokens;                            // tokens of a tile on the tensor cores of the fifth generation; 0: the other kernels
+    bool by_sixteen;                            // shared pieces in tiles of 16 query rows, by attend_own_tma_kernel
 };
 
 // Into how many pieces the keys are cut, none shorter than MIN_KEYS: the tokens' own for about four CTAs an SM; the shared ones, on the
 // tensor cores, for one CTA on as many SMs as are their share of the work (a block of 128 keys takes a tile 1.2 us, a token's own
-// keys come in at 47 KB a us and SM), half of them at least, so that attend_own's CTAs run on the others meanwhile (60 tokens with up
-// to 431 keys behind 6,144: 39.0 us with all 148, 35.5 with 100, 32.6 with 74; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42, 53, 87).
+// keys come in at 47 KB a us and SM), LEAST_SMS at least, so that attend_own's CTAs run on the others meanwhile (60 tokens with up to
+// 431 keys behind 6,144: 34.3 us with 100, 30.2 with 64, 32.5 with 48; three groups of 13 with up to 777 behind 2,896, 64 / 8 heads:
+// 45.3, 33.8, 33.7; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42 with 148, 53 with 100, 87 with 74).
 Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pages, int page_size, long long max_shared, long long max_own, int dtype) {
-    constexpr int MIN_KEYS = 128, SMS = 148;
+    constexpr int MIN_KEYS = 128, SMS = 148, LEAST_SMS = 64;
     const int heads = num_q / num_kv;
     Plan p;
     p.tile_tokens = dtype == TVB_BF16 && pages > 0 && tc_takes(head_dim, heads, page_size) ? TC_ROWS / heads : 0;
+    // Head size 256, whose 64 query rows leave a tile of keys no room to be ahead: 16 rows, if a group has no more as a rule (8 / 4 heads,
+    // three groups, us 16 rows / 64: 4 tokens behind 5,808 keys 22 / 32, four of 7 behind 368 11.8 / 13.4; 11 tokens, two tiles of 16,
+    // behind 4,320 33.7 / 32.3).
+    p.by_sixteen = dtype == TVB_BF16 && head_dim == 256 && pages > 0 && own_tma_takes(page_size) && (long long)tokens * heads <= 16ll * max(groups, 1);
     // CTAs' tiles: at most, and as a rule
     long long tiles = 0, usual = 1;
     // Up to so many values (32 MB of bfloat16) the tokens read the shared keys by themselves, in one launch or two: the third
@@ -960,7 +972,7 @@ Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pa
     const bool alone = (long long)tokens * num_kv * head_dim * max_shared <= FEW_VALUES;
     if (alone) max_own += max_shared;
     if (groups > 0 && max_shared > 0 && !alone) {
-        const long long in_tile = p.tile_tokens > 0 ? p.tile_tokens * heads : dtype == TVB_F32 ? 16 : 64;
+        const long long in_tile = p.tile_tokens > 0 ? p.tile_tokens * heads : dtype == TVB_F32 || p.by_sixteen ? 16 : 64;
         tiles = groups + (long long)tokens * heads / in_tile;
         usual = max((long long)groups, ceil_div((long long)tokens * heads, in_tile));
     }
@@ -971,8 +983,10 @@ Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pa
     p.own_tiles = (int)ceil_div(heads, dtype == TVB_F32 ? 4 : 16);
     const double own_us = (double)tokens * num_kv * max_own * head_dim * (dtype == TVB_F32 ? 8 : 4) / 47e3;
     const double shared_us = 1.2 * usual * num_kv * (max_shared / 128.0);
-    const int share = max(SMS / 2, (int)(SMS * shared_us / (shared_us + own_us + 1e-9)));
-    p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? share : 3 * SMS, usual * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
+    const int share = max(LEAST_SMS, (int)(SMS * shared_us / (shared_us + own_us + 1e-9)));
+    // (the other kernels: a round of their CTAs; head size 256, 33 tokens behind 4,320: 32 us in one round, 45 in three)
+    const int others = dtype == TVB_BF16 && head_dim == 256 ? SMS : 3 * SMS;
+    p.shared_pieces = tiles > 0 ? pieces_of(p.tile_tokens > 0 ? share : others, usual * num_kv, max_shared, MAX_SHARED_PIECES) : 0;
     p.own_pieces = pieces_of(4 * SMS, (long long)tokens * num_kv * p.own_tiles, max_own, MAX_OWN_PIECES);
     if (tiles == 0 && dtype == TVB_BF16 && max_own <= 2 * MIN_KEYS) p.own_pieces = 1;            // not worth the launch that joins them
     p.shared_items = tiles * num_kv * p.shared_pieces;
@@ -995,13 +1009,15 @@ template <int D> int launch_shared(const Attend& a, const Plan& p, int dtype, in
         return launch(attend_shared_f32_kernel<D>, p.shared_items, (size_t)(2 * KEYS32 * (D + 4) + 16 * D) * 4, pdl, s, a);
     if constexpr (D <= 128)
         if (p.tile_tokens > 0) return launch_shared_tc<D>(a, p.shared_items, p.tile_tokens, pdl, s);
+    if constexpr (D == 256)
+        if (p.by_sixteen) return launch_own_tma<D, true>(a, p.shared_items, pdl, s);
     return launch(attend_shared_bf16_kernel<D>, p.shared_items, Tiles<D>::bytes(64), pdl, s, a);
 }
 template <int D> int launch_all(const Attend& a, const Plan& p, int dtype, int pdl, cudaStream_t s) {
     int e = p.shared_items > 0 ? launch_shared<D>(a, p, dtype, pdl, s) : 0;
     if (e) return e;
     if (dtype == TVB_F32) e = launch(attend_own_f32_kernel<D>, p.own_items, (size_t)Ends<D, 4>::FLOATS * 4, pdl, s, a);
-    else if (a.pages > 0 && own_tma_takes(a.page_size)) e = launch_own_tma<D>(a, p.own_items, pdl, s);
+    else if (a.pages > 0 && own_tma_takes(a.page_size)) e = launch_own_tma<D, false>(a, p.own_items, pdl, s);
     else e = launch(attend_own_bf16_kernel<D>, p.own_items, OwnTiles<D>::BYTES, pdl, s, a);
     if (e || !a.part_o) return e;
     const long long joins = ceil_div((long long)a.tokens * a.num_q, WARPS);
