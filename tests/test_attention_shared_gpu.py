@@ -95,6 +95,19 @@ def test_members_that_end_before_the_shared_keys_do(dtype):
     check_both(s, sizes)
 
 
+@pytest.mark.parametrize("heads", [(8, 4), (16, 1), (2, 2)])
+@pytest.mark.parametrize("members", [1, 4, 8, 9, 20])
+def test_head_size_256_with_few_and_more_query_rows(members, heads):
+    """Up to 16 rows a group and more; a length in the middle of a page, members that end before it, padding, a page that is none."""
+    own = [[7, 40, -3, 100, 1, 2, -90, 33][i % 8] for i in range(members)]
+    s, sizes = made([(312, own), (1056, own[::-1]), (64, own[:1])], num_q=heads[0], num_kv=heads[1], dim=256, padding=(members // 2,), seed=members)
+    check_both(s, sizes)
+    s["block_tables"][:members, 5] = -1
+    s["block_tables"][-1, 1] = s["key_cache"].shape[0]
+    for hints in ({}, TOGETHER):
+        check_attention(shared(s, sizes, **hints), s, **sizes)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_several_tokens_of_a_request(dtype):
     s, sizes = made([(128, [5, 9, 40]), (16, [7])], tokens_of=5, dtype=dtype, seed=21)
