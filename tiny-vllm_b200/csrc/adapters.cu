@@ -37,11 +37,17 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// values at, .., at + 7 of a row of `size` (zeros past its end, or where the row is not there); L2: past L1
-template <bool WIDE, bool L2 = false> __device__ __forceinline__ uint4 load_8(const bf16* row, int at, int size, bool there) {
-    if constexpr (WIDE) {                       // size is a multiple of 8, the row lies on 16 bytes
+// values at, .., at + 7 of a row of `size` (zeros past its end, or where the row is not there) in loads of WIDTH, of which size is a
+// multiple and on which the row lies; L2: past L1
+template <int WIDTH, bool L2 = false> __device__ __forceinline__ uint4 load_8(const bf16* row, int at, int size, bool there) {
+    if constexpr (WIDTH == 8) {
         const uint4* from = reinterpret_cast<const uint4*>(row + at);
         return !there || at >= size ? make_uint4(0, 0, 0, 0) : L2 ? __ldcg(from) : *from;
+    } else if constexpr (WIDTH == 4) {
+        const uint2* from = reinterpret_cast<const uint2*>(row + at);
+        const uint2 lo = !there || at >= size ? make_uint2(0, 0) : L2 ? __ldcg(from) : *from;
+        const uint2 hi = !there || at + 4 >= size ? make_uint2(0, 0) : L2 ? __ldcg(from + 1) : from[1];
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
     } else {
         uint32_t h[8];
 #pragma unroll
@@ -134,11 +140,11 @@ template <bool WIDE, typename R> __device__ __forceinline__ void shrink_rows(con
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             const int b = b0 + i * WARPS, at = b * 32 + 8 * t;
-            xl[i] = load_8<WIDE>(lo, at, s.k, lo_row >= 0 && b < end);
-            xh[i] = load_8<WIDE>(hi, at, s.k, hi_row >= 0 && b < end);
+            xl[i] = load_8<WIDE ? 8 : 1>(lo, at, s.k, lo_row >= 0 && b < end);
+            xh[i] = load_8<WIDE ? 8 : 1>(hi, at, s.k, hi_row >= 0 && b < end);
 #pragma unroll
             for (int j = 0; j < NR; ++j)
-                w[i][j] = load_8<WIDE>(down + (int64_t)(8 * j + g) * s.k, at, s.k, 8 * j + g < ranks && b < end);
+                w[i][j] = load_8<WIDE ? 8 : 1>(down + (int64_t)(8 * j + g) * s.k, at, s.k, 8 * j + g < ranks && b < end);
         }
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i)
@@ -365,7 +371,7 @@ __global__ void __launch_bounds__(THREADS) shrink_many_kernel(Shrink s) {
                     const bf16* from = of_x ? s.x + (int64_t)(there ? row0 + row : 0) * s.ldx : down + (int64_t)(there ? row - 64 : 0) * s.k;
                     bf16* to = (of_x ? x_s + row * STAGE_PITCH : a_s + (row - 64) * STAGE_PITCH) + i % (STAGE_K / 8) * 8;
                     if constexpr (WIDE) cp_async_16(to, from + (at < s.k ? at : 0), there && at < s.k);
-                    else *reinterpret_cast<uint4*>(to) = load_8<false>(from, at, s.k, there);
+                    else *reinterpret_cast<uint4*>(to) = load_8<1>(from, at, s.k, there);
                 }
             }
             cp_async_commit();
@@ -439,7 +445,8 @@ struct Expand {
 //
 // All that comes from before `shrink` (whose threads wait for it before they let this kernel start) may be read before `shrink` is
 // through: ids, and where EARLY says so the first tiles of y and B, past L1.  u may not, and nothing is written before.
-template <typename Y, bool WIDE, bool EARLY>
+// B is read in loads of WIDTH, and a tile of y in 16-byte words where WIDE.
+template <typename Y, int WIDTH, bool WIDE, bool EARLY>
 __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const int (&row)[2], const bool (&there)[2], int first_tile, int end, int step) {
     constexpr int NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;                     // steps of 32 ranks held; 16-byte words of eight values of y
     const int padded = padded_rank(s.rank), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -466,10 +473,26 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
     uint4 old[2][WORDS];                        // of y
     auto load_y = [&](int tile) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            if (WIDE && there[h] && tile * 32 + 8 * t + 8 <= s.n)
+        for (int h = 0; h < 2; ++h) {
+            if (!there[h]) continue;
+            const Y* from = y[h] + tile * 32;
+            const int left = s.n - tile * 32 - 8 * t;
+            if (WIDE && left >= 8) {
 #pragma unroll
-                for (int q = 0; q < WORDS; ++q) old[h][q] = __ldcg(reinterpret_cast<const uint4*>(y[h] + tile * 32) + q);
+                for (int q = 0; q < WORDS; ++q) old[h][q] = __ldcg(reinterpret_cast<const uint4*>(from) + q);
+            } else if constexpr (sizeof(Y) == 2) {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e < left ? (uint32_t)__ldcg(reinterpret_cast<const unsigned short*>(from) + e) : 0u;
+                old[h][0] = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+            } else {
+                uint32_t v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = e < left ? __ldcg(reinterpret_cast<const uint32_t*>(from) + e) : 0u;
+                old[h][0] = make_uint4(v[0], v[1], v[2], v[3]);
+                old[h][WORDS - 1] = make_uint4(v[4], v[5], v[6], v[7]);
+            }
+        }
     };
     uint4 w[STEPS][NT];
     auto load_b = [&](int tile, int r0) {
@@ -478,7 +501,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-                w[k][j] = load_8<WIDE, EARLY>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
+                w[k][j] = load_8<WIDTH, EARLY>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
             }
     };
     load_y(first_tile);
@@ -525,33 +548,39 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
             float add[8];
 #pragma unroll
             for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
-            if (WIDE && tile * 32 + 8 * t + 8 <= s.n) {
-                if constexpr (sizeof(Y) == 2) {
-                    float v[8];
-                    unpack_bf16x8(now[h][0], v);
+            float v[8];
+            if constexpr (sizeof(Y) == 2) {
+                unpack_bf16x8(now[h][0], v);
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) add[e] += v[e];
+                for (int q = 0; q < 2; ++q) {
+                    const uint4 word = now[h][q];
+                    v[4 * q] = __uint_as_float(word.x); v[4 * q + 1] = __uint_as_float(word.y);
+                    v[4 * q + 2] = __uint_as_float(word.z); v[4 * q + 3] = __uint_as_float(word.w);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) add[e] += v[e];
+            const int left = s.n - tile * 32 - 8 * t;
+            if (WIDE && left >= 8) {
+                if constexpr (sizeof(Y) == 2) {
                     *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
                 } else {
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint4 v = now[h][q];
-                        reinterpret_cast<float4*>(to)[q] =
-                            make_float4(__uint_as_float(v.x) + add[4 * q], __uint_as_float(v.y) + add[4 * q + 1],
-                                        __uint_as_float(v.z) + add[4 * q + 2], __uint_as_float(v.w) + add[4 * q + 3]);
-                    }
+                    for (int q = 0; q < 2; ++q)
+                        reinterpret_cast<float4*>(to)[q] = make_float4(add[4 * q], add[4 * q + 1], add[4 * q + 2], add[4 * q + 3]);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (tile * 32 + 8 * t + e < s.n) to[e] = from_float<Y>(to_float<Y>(to[e]) + add[e]);
+                    if (e < left) to[e] = from_float<Y>(add[e]);
             }
         }
     }
 }
 
 // few rows: 16 rows as they lie, the blockIdx.z-th of their adapters, a tile of 32 columns a warp
-template <typename Y, bool WIDE>
+template <typename Y, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
     const int tile = blockIdx.x * WARPS + (threadIdx.x >> 5), row0 = blockIdx.y * 16, g = (threadIdx.x & 31) >> 2;
     uint32_t rows;
@@ -559,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
     if (adapter >= 0 && tile * 32 < s.n) {
         const bool there[2] = {(bool)(rows >> g & 1), (bool)(rows >> (g + 8) & 1)};
         const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
-        expand_rows<Y, WIDE, true>(s, adapter, row, there, tile, tile + 1, 1);
+        expand_rows<Y, WIDTH, WIDE, true>(s, adapter, row, there, tile, tile + 1, 1);
     } else {
         pdl_wait();                             // (a warp that has nothing to do waits too: what follows relies on this kernel's end)
         pdl_launch_dependents();
@@ -568,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
 
 // rows sorted into chunks: a chunk and a strip of its columns a CTA, as many strips as fill the GPU; the warps take every fourth tile
 // of the strip
-template <typename Y, bool WIDE>
+template <typename Y, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
     __shared__ Sorted sorted;
     const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, tiles = (s.n + 31) / 32;
@@ -580,7 +609,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
         const bool there[2] = {row[0] >= 0, row[1] >= 0};
         row[0] = max(row[0], 0);
         row[1] = max(row[1], 0);
-        if (first < end) expand_rows<Y, WIDE, true>(s, sorted.ids[chunk], row, there, first, end, WARPS);
+        if (first < end) expand_rows<Y, WIDTH, WIDE, true>(s, sorted.ids[chunk], row, there, first, end, WARPS);
     }
     pdl_wait();                                 // (see above)
     pdl_launch_dependents();
@@ -588,7 +617,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
 
 // more rows: the warps of a CTA have 16 rows each as they lie and the same columns, whose B they find in L1; one adapter of the rows
 // after another
-template <typename Y, bool WIDE>
+template <typename Y, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_many_kernel(Expand s) {
     constexpr int ROWS = 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
@@ -609,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, 4) expand_many_kernel(Expand s) {
         const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader) >> g;
         const bool there[2] = {(bool)(rows & 1), (bool)(rows >> 8 & 1)};
         const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
-        expand_rows<Y, WIDE, false>(s, __shfl_sync(0xffffffffu, id, leader), row, there, blockIdx.x, tiles, gridDim.x);
+        expand_rows<Y, WIDTH, WIDE, false>(s, __shfl_sync(0xffffffffu, id, leader), row, there, blockIdx.x, tiles, gridDim.x);
     }
 }
 
@@ -737,20 +766,22 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
                 : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-template <typename Y> int launch_expand(const Expand& a, Rows rows_are, bool wide, int pdl, cudaStream_t s) {
+template <typename Y, int WIDTH, bool WIDE> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
     const int tiles = ceil_div(a.n, 32);
-    if (rows_are == FEW) {
-        const dim3 grid(ceil_div(tiles, WARPS), ceil_div(a.m, 16), min(min(16, a.m), a.adapters));
-        return wide ? launch(expand_few_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_few_kernel<Y, false>, grid, 0, 0, pdl, s, a);
-    }
-    if (rows_are == SORTED) {
-        const dim3 grid((unsigned)min((long long)a.m * ceil_div(tiles, WARPS), 4ll * 148));       // one round of CTAs, four an SM
-        return wide ? launch(expand_sorted_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_sorted_kernel<Y, false>, grid, 0, 0, pdl, s, a);
-    }
+    if (rows_are == FEW)
+        return launch(expand_few_kernel<Y, WIDTH, WIDE>, dim3(ceil_div(tiles, WARPS), ceil_div(a.m, 16), min(min(16, a.m), a.adapters)), 0, 0, pdl, s, a);
+    if (rows_are == SORTED)                     // one round of CTAs, four an SM
+        return launch(expand_sorted_kernel<Y, WIDTH, WIDE>, dim3((unsigned)min((long long)a.m * ceil_div(tiles, WARPS), 4ll * 148)), 0, 0, pdl, s, a);
     // several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us with three CTAs an SM, 34 with six, 33 with twelve)
     const int rows = ceil_div(a.m, 16 * WARPS);
-    const dim3 grid(min(tiles, max(1, 12 * 148 / rows)), rows, min(2, a.adapters));
-    return wide ? launch(expand_many_kernel<Y, true>, grid, 0, 0, pdl, s, a) : launch(expand_many_kernel<Y, false>, grid, 0, 0, pdl, s, a);
+    return launch(expand_many_kernel<Y, WIDTH, WIDE>, dim3(min(tiles, max(1, 12 * 148 / rows)), rows, min(2, a.adapters)), 0, 0, pdl, s, a);
+}
+// by how B and y lie
+template <typename Y> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
+    const uintptr_t up = (uintptr_t)a.up, y = (uintptr_t)a.y;
+    if (a.rank % 8 == 0 && !(up & 15))
+        return !(y & 15) && a.ldy * sizeof(Y) % 16 == 0 ? launch_expand<Y, 8, true>(a, rows_are, pdl, s) : launch_expand<Y, 8, false>(a, rows_are, pdl, s);
+    return a.rank % 4 == 0 && !(up & 7) ? launch_expand<Y, 4, false>(a, rows_are, pdl, s) : launch_expand<Y, 1, false>(a, rows_are, pdl, s);
 }
 
 }  // namespace
@@ -807,11 +838,9 @@ int expand(const void* u, const void* up, const int* ids, void* y, long long ldy
                                                      : launch(expand_f32_kernel<1>, grid, shared, 0, pdl, s, a);
     }
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    const int size = y_dtype == TVB_F32 ? 4 : 2;
-    const bool wide = rank % 8 == 0 && !((uintptr_t)up & 15) && !((uintptr_t)y & 15) && ldy * size % 16 == 0;
     if (y_dtype != TVB_F32 && y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
     const Rows rows_are = rows_go(m, adapters);
-    return y_dtype == TVB_F32 ? launch_expand<float>(a, rows_are, wide, pdl, s) : launch_expand<bf16>(a, rows_are, wide, pdl, s);
+    return y_dtype == TVB_F32 ? launch_expand<float>(a, rows_are, pdl, s) : launch_expand<bf16>(a, rows_are, pdl, s);
 }
 
 }  // namespace
@@ -835,14 +864,14 @@ extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
     if (c.m <= 0 || c.n <= 0 || c.adapters <= 0) return 0;
     if (c.k <= 0 || c.rank <= 0 || c.rank > MAX_RANK || ceil_div(c.m, 16) > 65535) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
-    if (c.dtype == TVB_BF16 && rows_go(c.m, c.adapters) == MANY &&
-        adapters_tma_takes(c.x, c.ldx, c.down, c.up, c.y, c.ldy, c.k, c.n, c.rank, c.adapters, c.y_dtype)) {
-        const int e = shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0},
-                                 c.pdl, s);
-        return e ? e : expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters}, c.pdl, s);
-    }
-    const int e = shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
-    return e ? e : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);
+    const bool many = c.dtype == TVB_BF16 && rows_go(c.m, c.adapters) == MANY;
+    const int e = many && shrink_tma_takes(c.x, c.ldx, c.down, c.k, c.rank, c.adapters)
+                      ? shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0}, c.pdl, s)
+                      : shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
+    if (e) return e;
+    return many && expand_tma_takes(c.up, c.y, c.ldy, c.n, c.rank, c.adapters, c.y_dtype)
+               ? expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters}, c.pdl, s)
+               : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);
 }
 
 // 0, or which bounded wait gave up in some launch since the last call; reading clears it.  Synchronises.

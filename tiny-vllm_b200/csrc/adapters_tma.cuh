@@ -1,5 +1,5 @@
-// The adapters' two products for many rows as they lie (included by adapters.cu): bfloat16, ranks of up to 64 that are a
-// multiple of 8, operands on 16 bytes.  Tiles come in by tensor-map copies in the 128-byte swizzle that a warp of its own issues,
+// The adapters' two products for many rows as they lie (included by adapters.cu): bfloat16, ranks of up to 64, x and A on 16 bytes for
+// `shrink`, y and B (a rank that is a multiple of 8) for `expand`.  Tiles come in by tensor-map copies in the 128-byte swizzle that a warp of its own issues,
 // four warps multiply them with mma.sync; full and empty mbarriers between them, every wait bounded (tc5.cuh).
 //
 //   shrink  64 rows and up to 64 ranks a CTA, stages of 64 k; the CTAs of a cluster have a piece of k each and add up through
@@ -285,10 +285,12 @@ __global__ void __launch_bounds__(TMA_THREADS, 4) expand_tma_kernel(const __grid
     }
 }
 
-inline bool adapters_tma_takes(const void* x, long long ldx, const void* down, const void* up, const void* y, long long ldy, int k, int n, int rank,
-                               int adapters, int y_dtype) {
-    return rank <= 64 && rank % 8 == 0 && k % 8 == 0 && n >= 8 && ldx >= k && ldx % 8 == 0 && ldy >= n && ldy % 8 == 0 && y_dtype == TVB_BF16 &&
-           !(((uintptr_t)x | (uintptr_t)down | (uintptr_t)up | (uintptr_t)y) & 15) && (long long)adapters * (n > rank ? n : rank) < 0x7fffffffLL;
+inline bool shrink_tma_takes(const void* x, long long ldx, const void* down, int k, int rank, int adapters) {
+    return rank <= 64 && k % 8 == 0 && ldx >= k && ldx % 8 == 0 && !(((uintptr_t)x | (uintptr_t)down) & 15) && (long long)adapters * rank < 0x7fffffffLL;
+}
+inline bool expand_tma_takes(const void* up, const void* y, long long ldy, int n, int rank, int adapters, int y_dtype) {
+    return rank <= 64 && rank % 8 == 0 && n >= 8 && ldy >= n && ldy % 8 == 0 && y_dtype == TVB_BF16 && !(((uintptr_t)up | (uintptr_t)y) & 15) &&
+           (long long)adapters * n < 0x7fffffffLL;
 }
 inline bool matrix_map(CUtensorMap* map, const void* p, long long rows, long long columns, long long ld, int box_rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)columns, (cuuint64_t)rows};
