@@ -183,22 +183,32 @@ template <bool WIDE, typename R> __device__ __forceinline__ void shrink_rows(con
     cluster_arrive();
 }
 
-// The d-th adapter of 16 rows as they lie, in the order of the rows: its number, -1: none; `mask`: which of the rows have it.
-// A whole warp calls.
-__device__ __forceinline__ int find_adapter(const int* all, int m, int adapters, int row0, int d, uint32_t& mask) {
-    const int lane = threadIdx.x & 31;
-    int id = -1;
-    if (lane < 16 && row0 + lane < m) {
-        id = __ldcg(all + row0 + lane);
-        if ((unsigned)id >= (unsigned)adapters) id = -1;
+// The adapters of 16 rows as they lie, in the order of the rows.  A whole warp makes one.
+constexpr int BARE = -1, NO_ROW = -2;           // what a row without an adapter has, and a place without a row
+struct TileAdapters {
+    int id;                                     // of row `lane`
+    uint32_t alike, leaders;                    // lanes with the same, the first ones of each
+    // with_bare: rows without an adapter count as another one
+    __device__ __forceinline__ TileAdapters(const int* all, int m, int adapters, int row0, bool with_bare) {
+        const int lane = threadIdx.x & 31;
+        id = NO_ROW;
+        if (lane < 16 && row0 + lane < m) {
+            id = __ldcg(all + row0 + lane);
+            if ((unsigned)id >= (unsigned)adapters) id = BARE;
+        }
+        alike = __match_any_sync(0xffffffffu, id);
+        leaders = __ballot_sync(0xffffffffu, id >= (with_bare ? BARE : 0) && (alike & ((1u << lane) - 1u)) == 0);
     }
-    const uint32_t alike = __match_any_sync(0xffffffffu, id);
-    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
-    for (; d > 0; --d) leaders &= leaders - 1;
-    const int leader = leaders ? __ffs(leaders) - 1 : 31;
-    mask = __shfl_sync(0xffffffffu, alike, leader);
-    return __shfl_sync(0xffffffffu, id, leader);
-}
+    __device__ __forceinline__ void pass(int n) {
+        for (; n > 0; --n) leaders &= leaders - 1;
+    }
+    // the next one's number (NO_ROW: there is none), and which of the rows have it
+    __device__ __forceinline__ int next(uint32_t& rows) const {
+        const int leader = leaders ? __ffs(leaders) - 1 : 31;
+        rows = __shfl_sync(0xffffffffu, alike, leader);
+        return __shfl_sync(0xffffffffu, id, leader);
+    }
+};
 
 // rows as they lie, the blockIdx.z-th of their adapters
 template <bool WIDE> __global__ void __launch_bounds__(THREADS) shrink_few_kernel(Shrink s) {
@@ -207,8 +217,10 @@ template <bool WIDE> __global__ void __launch_bounds__(THREADS) shrink_few_kerne
     const int rank0 = blockIdx.x / s.splits * 16, row0 = blockIdx.y * 16;
     pdl_wait();
     pdl_launch_dependents();
+    TileAdapters tile(s.ids, s.m, s.adapters, row0, false);
+    tile.pass(blockIdx.z);
     uint32_t rows;
-    const int adapter = find_adapter(s.ids, s.m, s.adapters, row0, blockIdx.z, rows);
+    const int adapter = tile.next(rows);
     if (adapter >= 0)                           // the same for the whole cluster
         shrink_rows<WIDE>(s, adapter, rank0, [&](int i) { return rows >> i & 1 ? row0 + i : -1; }, shared);
     cluster_wait();
@@ -232,14 +244,15 @@ struct Sorted {
     unsigned short rows[MAX_SORTED_ROWS];       // sorted
     __device__ __forceinline__ int row(int chunk, int i) const { return i < starts[chunk] >> 16 ? rows[(starts[chunk] & 0xffff) + i] : -1; }
 };
-// How many chunks there are.  All threads call.  (Loops as they are: code that runs once is read as slowly as it is long.)
-__device__ __forceinline__ int sort_rows(const int* all, int m, int adapters, Sorted& c) {
+// How many chunks there are; with_bare: rows without an adapter have number `adapters`.  All threads call.  (Loops as they are: code that
+// runs once is read as slowly as it is long.)
+__device__ __forceinline__ int sort_rows(const int* all, int m, int adapters, bool with_bare, Sorted& c) {
     const int tid = threadIdx.x, lane = tid & 31, padded = (m + 31) / 32 * 32;
     const uint32_t lower = (1u << lane) - 1u;
 #pragma unroll 1
     for (int row = tid; row < padded; row += THREADS) {
         const int id = row < m ? __ldcg(all + row) : -1;
-        c.of_rows[row] = (unsigned)id < (unsigned)adapters ? id : -1;
+        c.of_rows[row] = row < m && (unsigned)id >= (unsigned)adapters && with_bare ? adapters : (unsigned)id < (unsigned)adapters ? id : -1;
     }
 #pragma unroll 1
     for (int i = tid; i < TABLE; i += THREADS) {
@@ -325,7 +338,7 @@ template <bool WIDE> __global__ void __launch_bounds__(THREADS) shrink_sorted_ke
     const int rank_chunks = (s.rank + 15) / 16;
     pdl_wait();
     pdl_launch_dependents();
-    const int items = sort_rows(s.ids, s.m, s.adapters, sorted) * rank_chunks;
+    const int items = sort_rows(s.ids, s.m, s.adapters, false, sorted) * rank_chunks;
     for (int item = blockIdx.x / s.splits; item < items; item += gridDim.x / s.splits) {          // the same for the whole cluster
         const int chunk = item / rank_chunks;
         shrink_rows<WIDE>(s, sorted.ids[chunk], item % rank_chunks * 16, [&](int i) { return sorted.row(chunk, i); }, shared);
@@ -433,8 +446,10 @@ struct Expand {
     const void* u;
     const void* up;                             // [adapters, n, rank]
     const int* ids;
-    void* y;
+    const void* y;
     int64_t ldy;
+    void* out;                                  // y itself where their types are the same
+    int64_t ldo;
     int m, n, rank, adapters;
 };
 
@@ -445,18 +460,20 @@ struct Expand {
 //
 // All that comes from before `shrink` (whose threads wait for it before they let this kernel start) may be read before `shrink` is
 // through: ids, and where EARLY says so the first tiles of y and B, past L1.  u may not, and nothing is written before.
-// B is read in loads of WIDTH, and a tile of y in 16-byte words where WIDE.
-template <typename Y, int WIDTH, bool WIDE, bool EARLY>
+// B is read in loads of WIDTH, and a tile of y in 16-byte words where WIDE.  O is Y, and y becomes the result; or y is float32, the
+// result bfloat16 elsewhere, and rows without an adapter (BARE) are rounded into it too.
+template <typename Y, typename O, int WIDTH, bool WIDE, bool EARLY>
 __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const int (&row)[2], const bool (&there)[2], int first_tile, int end, int step) {
     constexpr int NT = 4, STEPS = 2, WORDS = sizeof(Y) / 2;                     // steps of 32 ranks held; 16-byte words of eight values of y
     const int padded = padded_rank(s.rank), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)adapter * s.n * s.rank;
+    const bool has = adapter >= 0;
+    const bf16* b = reinterpret_cast<const bf16*>(s.up) + (int64_t)max(adapter, 0) * s.n * s.rank;
     const bf16* u[2];
-    Y* y[2];
+    const Y* y[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         u[h] = reinterpret_cast<const bf16*>(s.u) + (int64_t)row[h] * 2 * padded;
-        y[h] = reinterpret_cast<Y*>(s.y) + row[h] * s.ldy + 8 * t;
+        y[h] = reinterpret_cast<const Y*>(s.y) + row[h] * s.ldy + 8 * t;
     }
     uint4 held[STEPS][2][2];                    // u of rows g + 8 h, its heads and its rests
     auto load_u = [&](int r0) {
@@ -467,7 +484,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
                     const int at = r0 + 32 * k + 8 * t;
-                    held[k][h][q] = there[h] && at < padded ? *reinterpret_cast<const uint4*>(u[h] + q * padded + at) : make_uint4(0, 0, 0, 0);
+                    held[k][h][q] = has && there[h] && at < padded ? *reinterpret_cast<const uint4*>(u[h] + q * padded + at) : make_uint4(0, 0, 0, 0);
                 }
     };
     uint4 old[2][WORDS];                        // of y
@@ -501,7 +518,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const int at = tile * 32 + (g >> 1) * 8 + 2 * j + (g & 1);
-                w[k][j] = load_8<WIDTH, EARLY>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, at < s.n);
+                w[k][j] = load_8<WIDTH, EARLY>(b + (int64_t)at * s.rank, r0 + 32 * k + 8 * t, s.rank, has && at < s.n);
             }
     };
     load_y(first_tile);
@@ -544,7 +561,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (!there[h]) continue;
-            Y* to = y[h] + tile * 32;
+            O* to = reinterpret_cast<O*>(s.out) + row[h] * s.ldo + 8 * t + tile * 32;
             float add[8];
 #pragma unroll
             for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
@@ -563,7 +580,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
             for (int e = 0; e < 8; ++e) add[e] += v[e];
             const int left = s.n - tile * 32 - 8 * t;
             if (WIDE && left >= 8) {
-                if constexpr (sizeof(Y) == 2) {
+                if constexpr (sizeof(O) == 2) {
                     *reinterpret_cast<uint4*>(to) = pack_bf16x8(add);
                 } else {
 #pragma unroll
@@ -573,22 +590,24 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                    if (e < left) to[e] = from_float<Y>(add[e]);
+                    if (e < left) to[e] = from_float<O>(add[e]);
             }
         }
     }
 }
 
 // few rows: 16 rows as they lie, the blockIdx.z-th of their adapters, a tile of 32 columns a warp
-template <typename Y, int WIDTH, bool WIDE>
+template <typename Y, typename O, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
     const int tile = blockIdx.x * WARPS + (threadIdx.x >> 5), row0 = blockIdx.y * 16, g = (threadIdx.x & 31) >> 2;
+    TileAdapters of_tile(s.ids, s.m, s.adapters, row0, sizeof(Y) != sizeof(O));
+    of_tile.pass(blockIdx.z);
     uint32_t rows;
-    const int adapter = find_adapter(s.ids, s.m, s.adapters, row0, blockIdx.z, rows);
-    if (adapter >= 0 && tile * 32 < s.n) {
+    const int adapter = of_tile.next(rows);
+    if (adapter != NO_ROW && tile * 32 < s.n && (sizeof(Y) != sizeof(O) || adapter >= 0)) {
         const bool there[2] = {(bool)(rows >> g & 1), (bool)(rows >> (g + 8) & 1)};
         const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
-        expand_rows<Y, WIDTH, WIDE, true>(s, adapter, row, there, tile, tile + 1, 1);
+        expand_rows<Y, O, WIDTH, WIDE, true>(s, adapter, row, there, tile, tile + 1, 1);
     } else {
         pdl_wait();                             // (a warp that has nothing to do waits too: what follows relies on this kernel's end)
         pdl_launch_dependents();
@@ -597,11 +616,11 @@ __global__ void __launch_bounds__(THREADS, 4) expand_few_kernel(Expand s) {
 
 // rows sorted into chunks: a chunk and a strip of its columns a CTA, as many strips as fill the GPU; the warps take every fourth tile
 // of the strip
-template <typename Y, int WIDTH, bool WIDE>
+template <typename Y, typename O, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
     __shared__ Sorted sorted;
     const int warp = threadIdx.x >> 5, g = (threadIdx.x & 31) >> 2, tiles = (s.n + 31) / 32;
-    const int count = sort_rows(s.ids, s.m, s.adapters, sorted);
+    const int count = sort_rows(s.ids, s.m, s.adapters, sizeof(Y) != sizeof(O), sorted);
     const int strips = max(1, min((tiles + WARPS - 1) / WARPS, (int)gridDim.x / max(count, 1))), per = (tiles + strips - 1) / strips;
     for (int item = blockIdx.x; item < count * strips; item += gridDim.x) {
         const int chunk = item % count, first = item / count * per + warp, end = min(tiles, (item / count + 1) * per);
@@ -609,7 +628,8 @@ __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
         const bool there[2] = {row[0] >= 0, row[1] >= 0};
         row[0] = max(row[0], 0);
         row[1] = max(row[1], 0);
-        if (first < end) expand_rows<Y, WIDTH, WIDE, true>(s, sorted.ids[chunk], row, there, first, end, WARPS);
+        const int adapter = sorted.ids[chunk] < s.adapters ? sorted.ids[chunk] : BARE;
+        if (first < end) expand_rows<Y, O, WIDTH, WIDE, true>(s, adapter, row, there, first, end, WARPS);
     }
     pdl_wait();                                 // (see above)
     pdl_launch_dependents();
@@ -617,28 +637,21 @@ __global__ void __launch_bounds__(THREADS, 4) expand_sorted_kernel(Expand s) {
 
 // more rows: the warps of a CTA have 16 rows each as they lie and the same columns, whose B they find in L1; one adapter of the rows
 // after another
-template <typename Y, int WIDTH, bool WIDE>
+template <typename Y, typename O, int WIDTH, bool WIDE>
 __global__ void __launch_bounds__(THREADS, 4) expand_many_kernel(Expand s) {
     constexpr int ROWS = 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int row0 = (blockIdx.y * WARPS + warp) * ROWS, tiles = (s.n + 31) / 32;
-    int id = -1;
-    if (lane < ROWS && row0 + lane < s.m) {
-        id = __ldcg(s.ids + row0 + lane);
-        if ((unsigned)id >= (unsigned)s.adapters) id = -1;
-    }
-    const uint32_t alike = __match_any_sync(0xffffffffu, id);
-    uint32_t leaders = __ballot_sync(0xffffffffu, id >= 0 && (alike & ((1u << lane) - 1u)) == 0);
-    for (int d = 0; d < (int)blockIdx.z; ++d) leaders &= leaders - 1;
+    TileAdapters of_tile(s.ids, s.m, s.adapters, row0, sizeof(Y) != sizeof(O));
+    of_tile.pass(blockIdx.z);
     pdl_wait();
     pdl_launch_dependents();
-    while (leaders) {
-        const int leader = __ffs(leaders) - 1;
-        for (int d = 0; d < (int)gridDim.z; ++d) leaders &= leaders - 1;
-        const uint32_t rows = __shfl_sync(0xffffffffu, alike, leader) >> g;
-        const bool there[2] = {(bool)(rows & 1), (bool)(rows >> 8 & 1)};
+    for (; of_tile.leaders; of_tile.pass(gridDim.z)) {
+        uint32_t rows;
+        const int adapter = of_tile.next(rows);
+        const bool there[2] = {(bool)(rows >> g & 1), (bool)(rows >> (g + 8) & 1)};
         const int row[2] = {there[0] ? row0 + g : 0, there[1] ? row0 + g + 8 : 0};
-        expand_rows<Y, WIDTH, WIDE, false>(s, __shfl_sync(0xffffffffu, id, leader), row, there, blockIdx.x, tiles, gridDim.x);
+        expand_rows<Y, O, WIDTH, WIDE, false>(s, adapter, row, there, blockIdx.x, tiles, gridDim.x);
     }
 }
 
@@ -704,10 +717,10 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
     const int row0 = blockIdx.y * ROWS, rows = min(ROWS, s.m - row0), column = blockIdx.x * THREADS + threadIdx.x;
     // before `shrink` is through (see expand_kernel): the adapters, y, and B on its way into L2
     const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
-    float* y = reinterpret_cast<float*>(s.y) + (int64_t)row0 * s.ldy + column;
+    float* y = reinterpret_cast<float*>(s.out) + (int64_t)row0 * s.ldo + column;
     float old[ROWS];
 #pragma unroll
-    for (int row = 0; row < ROWS; ++row) old[row] = column < s.n && ids[row] >= 0 ? __ldcg(y + row * s.ldy) : 0.0f;
+    for (int row = 0; row < ROWS; ++row) old[row] = column < s.n && ids[row] >= 0 ? __ldcg(y + row * s.ldo) : 0.0f;
     if (column < s.n)
         for (int d = 0; d < count; ++d)
             asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const float*>(s.up) + ((int64_t)distinct[d] * s.n + column) * s.rank));
@@ -732,7 +745,7 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
         }
 #pragma unroll
         for (int row = 0; row < ROWS; ++row)
-            if (ids[row] == adapter) y[row * s.ldy] = old[row] + total[row];
+            if (ids[row] == adapter) y[row * s.ldo] = old[row] + total[row];
     }
 }
 
@@ -766,22 +779,25 @@ template <int RANKS> int launch_many(const Shrink& a, int chunks, bool wide, int
                 : launch(shrink_many_kernel<RANKS, false>, grid, ManyShared<RANKS>::BYTES, a.splits, pdl, s, a);
 }
 
-template <typename Y, int WIDTH, bool WIDE> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
-    const int tiles = ceil_div(a.n, 32);
+template <typename Y, typename O, int WIDTH, bool WIDE> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
+    const int tiles = ceil_div(a.n, 32), each = min(a.adapters, 16) + (sizeof(Y) != sizeof(O));   // (what 16 rows have, at most)
     if (rows_are == FEW)
-        return launch(expand_few_kernel<Y, WIDTH, WIDE>, dim3(ceil_div(tiles, WARPS), ceil_div(a.m, 16), min(min(16, a.m), a.adapters)), 0, 0, pdl, s, a);
+        return launch(expand_few_kernel<Y, O, WIDTH, WIDE>, dim3(ceil_div(tiles, WARPS), ceil_div(a.m, 16), min(min(16, a.m), each)), 0, 0, pdl, s, a);
     if (rows_are == SORTED)                     // one round of CTAs, four an SM
-        return launch(expand_sorted_kernel<Y, WIDTH, WIDE>, dim3((unsigned)min((long long)a.m * ceil_div(tiles, WARPS), 4ll * 148)), 0, 0, pdl, s, a);
+        return launch(expand_sorted_kernel<Y, O, WIDTH, WIDE>, dim3((unsigned)min((long long)a.m * ceil_div(tiles, WARPS), 4ll * 148)), 0, 0, pdl, s, a);
     // several rounds of CTAs, which walk over the columns (4,099 rows x 4,096 of rank 64: 41 us with three CTAs an SM, 34 with six, 33 with twelve)
     const int rows = ceil_div(a.m, 16 * WARPS);
-    return launch(expand_many_kernel<Y, WIDTH, WIDE>, dim3(min(tiles, max(1, 12 * 148 / rows)), rows, min(2, a.adapters)), 0, 0, pdl, s, a);
+    return launch(expand_many_kernel<Y, O, WIDTH, WIDE>, dim3(min(tiles, max(1, 12 * 148 / rows)), rows, min(2, each)), 0, 0, pdl, s, a);
 }
 // by how B and y lie
-template <typename Y> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
+template <typename Y, typename O> int launch_expand(const Expand& a, Rows rows_are, int pdl, cudaStream_t s) {
     const uintptr_t up = (uintptr_t)a.up, y = (uintptr_t)a.y;
-    if (a.rank % 8 == 0 && !(up & 15))
-        return !(y & 15) && a.ldy * sizeof(Y) % 16 == 0 ? launch_expand<Y, 8, true>(a, rows_are, pdl, s) : launch_expand<Y, 8, false>(a, rows_are, pdl, s);
-    return a.rank % 4 == 0 && !(up & 7) ? launch_expand<Y, 4, false>(a, rows_are, pdl, s) : launch_expand<Y, 1, false>(a, rows_are, pdl, s);
+    if (a.rank % 8 == 0 && !(up & 15)) {
+        if constexpr (sizeof(Y) == sizeof(O))
+            if (!(y & 15) && a.ldy * sizeof(Y) % 16 == 0) return launch_expand<Y, O, 8, true>(a, rows_are, pdl, s);
+        return launch_expand<Y, O, 8, false>(a, rows_are, pdl, s);
+    }
+    return a.rank % 4 == 0 && !(up & 7) ? launch_expand<Y, O, 4, false>(a, rows_are, pdl, s) : launch_expand<Y, O, 1, false>(a, rows_are, pdl, s);
 }
 
 }  // namespace
@@ -826,21 +842,21 @@ int shrink(const void* x, long long ldx, const void* down, const int* ids, const
     return rank <= 16 ? launch_many<16>(a, chunks, wide, pdl, s) : launch_many<64>(a, chunks, wide, pdl, s);
 }
 
-// dtype: of x, A and B; y_dtype: of y (float32 with either, bfloat16 with bfloat16)
-int expand(const void* u, const void* up, const int* ids, void* y, long long ldy, int m, int n, int rank, int adapters, int dtype, int y_dtype,
-           int pdl, cudaStream_t s) {
-    const Expand a{u, up, ids, y, ldy, m, n, rank, adapters};
+// dtype: of x, A and B; y_dtype and out_dtype: both float32, both bfloat16 with bfloat16, or float32 and bfloat16 with it
+int expand(const Expand& a, int dtype, int y_dtype, int out_dtype, int pdl, cudaStream_t s) {
     if (dtype == TVB_F32) {
-        if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
-        const dim3 grid(ceil_div(n, THREADS), ceil_div(m, 16));
-        const size_t shared = 16 * (size_t)rank * 4;
-        return rank % 4 == 0 && !((uintptr_t)up & 15) ? launch(expand_f32_kernel<4>, grid, shared, 0, pdl, s, a)
-                                                     : launch(expand_f32_kernel<1>, grid, shared, 0, pdl, s, a);
+        if (y_dtype != TVB_F32 || out_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
+        const dim3 grid(ceil_div(a.n, THREADS), ceil_div(a.m, 16));
+        const size_t shared = 16 * (size_t)a.rank * 4;
+        return a.rank % 4 == 0 && !((uintptr_t)a.up & 15) ? launch(expand_f32_kernel<4>, grid, shared, 0, pdl, s, a)
+                                                         : launch(expand_f32_kernel<1>, grid, shared, 0, pdl, s, a);
     }
     if (dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    if (y_dtype != TVB_F32 && y_dtype != TVB_BF16) return TVB_BAD_ARGUMENT;
-    const Rows rows_are = rows_go(m, adapters);
-    return y_dtype == TVB_F32 ? launch_expand<float>(a, rows_are, pdl, s) : launch_expand<bf16>(a, rows_are, pdl, s);
+    const Rows rows_are = rows_go(a.m, a.adapters);
+    if (y_dtype == TVB_BF16 && out_dtype == TVB_BF16) return launch_expand<bf16, bf16>(a, rows_are, pdl, s);
+    if (y_dtype != TVB_F32) return TVB_BAD_ARGUMENT;
+    if (out_dtype == TVB_F32) return launch_expand<float, float>(a, rows_are, pdl, s);
+    return out_dtype == TVB_BF16 ? launch_expand<float, bf16>(a, rows_are, pdl, s) : TVB_BAD_ARGUMENT;
 }
 
 }  // namespace
@@ -854,24 +870,28 @@ struct AdaptersCall {
     const int* ids;
     const float* scales;
     void* u;                                    // scratch: m rows of rank float32, for bfloat16 of the rank filled up to sixteens
-    void* y;
+    const void* y;
     long long ldy;
-    int m, n, k, rank, adapters, dtype, y_dtype, pdl;
+    void* out;                                  // y itself, or a bfloat16 result of a float32 y
+    long long ldo;
+    int m, n, k, rank, adapters, dtype, y_dtype, out_dtype, pdl;
 };
 
 extern "C" int tvb_add_adapters(const AdaptersCall* call, void* stream) {
     const AdaptersCall& c = *call;
     if (c.m <= 0 || c.n <= 0 || c.adapters <= 0) return 0;
     if (c.k <= 0 || c.rank <= 0 || c.rank > MAX_RANK || ceil_div(c.m, 16) > 65535) return TVB_BAD_ARGUMENT;
+    if (c.y_dtype == c.out_dtype && (c.out != c.y || c.ldo != c.ldy)) return TVB_BAD_ARGUMENT;
     cudaStream_t s = (cudaStream_t)stream;
     const bool many = c.dtype == TVB_BF16 && rows_go(c.m, c.adapters) == MANY;
     const int e = many && shrink_tma_takes(c.x, c.ldx, c.down, c.k, c.rank, c.adapters)
                       ? shrink_tma(Shrink{(const bf16*)c.x, c.ldx, (const bf16*)c.down, c.ids, c.scales, (bf16*)c.u, c.m, c.k, c.rank, c.adapters, 1, 0}, c.pdl, s)
                       : shrink(c.x, c.ldx, c.down, c.ids, c.scales, c.u, c.m, c.k, c.rank, c.adapters, c.dtype, c.pdl, s);
     if (e) return e;
-    return many && expand_tma_takes(c.up, c.y, c.ldy, c.n, c.rank, c.adapters, c.y_dtype)
-               ? expand_tma(Expand{c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters}, c.pdl, s)
-               : expand(c.u, c.up, c.ids, c.y, c.ldy, c.m, c.n, c.rank, c.adapters, c.dtype, c.y_dtype, c.pdl, s);
+    const Expand a{c.u, c.up, c.ids, c.y, c.ldy, c.out, c.ldo, c.m, c.n, c.rank, c.adapters};
+    return many && c.out_dtype == TVB_BF16 && expand_tma_takes(c.up, c.y, c.ldy, c.n, c.rank, c.adapters, c.y_dtype)
+               ? expand_tma(a, c.pdl, s)
+               : expand(a, c.dtype, c.y_dtype, c.out_dtype, c.pdl, s);
 }
 
 // 0, or which bounded wait gave up in some launch since the last call; reading clears it.  Synchronises.

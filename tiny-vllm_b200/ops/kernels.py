@@ -2110,20 +2110,21 @@ ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
 ADAPTERS_FEW_ROWS = 192            # more rows may go through the kernels with bounded waits there
 
 
-_ADAPTERS_CALL = struct.Struct("@PqPPPPPPqiiiiiiii")
+_ADAPTERS_CALL = struct.Struct("@PqPPPPPPqPqiiiiiiiii")
 
 
 def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch.Tensor, ids: torch.Tensor,
-                 scales: torch.Tensor | None, stream: int) -> None:
-    """y[t] += scale * (x[t] . A^T) . B^T in place, rounded once more to the type of y; arguments as
-    :func:`tinyvllm_b200.ops.linear_adapted` has checked them."""
+                 scales: torch.Tensor | None, out: torch.Tensor, stream: int) -> None:
+    """out[t] = y[t] + scale * (x[t] . A^T) . B^T, rounded to the type of ``out``: y itself, or a bfloat16 tensor where y is float32;
+    arguments as :func:`tinyvllm_b200.ops.linear_adapted` has checked them."""
     (m, n), (adapters, rank, k) = y.shape, down.shape
     tag = dtype_tag(x.dtype)
     # u: float32, or two bfloat16 a value with the rank filled up to sixteens
     u = torch.empty(m * (rank if tag == F32 else -(-rank // 16) * 16), dtype=torch.float32, device=x.device)
     call = _ADAPTERS_CALL.pack(
         x.data_ptr(), x.stride()[0], down.data_ptr(), up.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
-        u.data_ptr(), y.data_ptr(), y.stride()[0], m, n, k, rank, adapters, tag, dtype_tag(y.dtype), _pdl("gemm"))
+        u.data_ptr(), y.data_ptr(), y.stride()[0], out.data_ptr(), out.stride()[0], m, n, k, rank, adapters, tag, dtype_tag(y.dtype),
+        dtype_tag(out.dtype), _pdl("gemm"))
     _check(_fn("adapters", "tvb_add_adapters", _PACKED)(call, stream), "add_adapters", 2)
     global _adapters_unchecked
     _adapters_unchecked = _adapters_unchecked or (tag == BF16 and m > ADAPTERS_FEW_ROWS)
