@@ -6,10 +6,10 @@
 // Tiles are those of the positions (32 from 0 on), so that boxes lie on the 1024 bytes of the 128-byte swizzle; keys of a tile that
 // are not the piece's get no weight, and their values are zeroed in the fragments (what lies there is of no account).
 //
-// Bound by reading keys and values, of which the 96 KB of the four CTAs' rings are in flight on an SM: whole calls, us with this kernel /
-// with attend_own_bf16_kernel: 60 tokens with up to 431 keys behind 6,144, 32 / 8 heads of size 128, 30.1 / 33.0; three groups of 13 with
-// up to 777 behind 2,896, 64 / 8 heads, 33.8 / 38.9; 2 tokens with 231 keys, 16 / 8 heads, alone 7.6 / 9.8, which is the chain of
-// position, page number, eight tiles one after another and the meeting of the warps.
+// Bound by reading keys and values, and by the tiles of the longest piece, one after another.  Whole calls, us with this kernel / with
+// attend_own_bf16_kernel: 60 tokens with up to 431 keys behind 6,144, 32 / 8 heads of size 128, 28.2 / 33.0; three groups of 13 with up
+// to 777 behind 2,896, 64 / 8 heads, 31.3 / 38.9; 2 tokens with 231 keys, 16 / 8 heads, alone 6.9 / 9.8, which is the chain of
+// position, page number, eight tiles and the meeting of the warps.  Rings of four and six tiles in as many CTAs as then fit: 28.7, 33.0.
 #pragma once
 
 template <int D> struct OwnTma {
@@ -18,8 +18,8 @@ template <int D> struct OwnTma {
     static constexpr int Q_PITCH = D + 8, Q_BYTES = 16 * Q_PITCH * 2;
     static constexpr int RING_BYTES = 2 * RING * TILE, END_BYTES = Ends<D, 16>::FLOATS * 4;
     static constexpr int BYTES = 1024 + (RING_BYTES > END_BYTES ? RING_BYTES : END_BYTES) + Q_BYTES + 2 * RING * 8 + 16;
-    static constexpr int CTAS = D == 64 ? 5 : D == 128 ? 4 : 1;                 // on an SM, by its registers and shared memory
-    static constexpr bool Q_HELD = D == 64;                                     // q fragments in registers (else read again a tile)
+    static constexpr int CTAS = D == 64 ? 4 : D == 128 ? 3 : 1;                 // on an SM (one more: 1 us slower, with fewer registers)
+    static constexpr bool Q_HELD = D <= 128;                                    // q fragments in registers (else read again a tile)
     static constexpr int THREADS_ALL = THREADS + 32;                            // four warps of products, one of copies
 };
 

@@ -19,8 +19,8 @@
 // second product, the denominator sums what was not rounded.  float32: the float32 cores.
 //
 // Bound by reading keys and values while a group has few query rows, by the shared pieces' products once it has many: 60 tokens with up
-// to 431 keys of their own behind 6,144, 32 / 8 heads of size 128, take 30 us for 93 MB, 3.1 TB/s; three groups of 13 with up to 777 behind
-// 2,896, 64 / 8 heads, 34 us for 112 MB, 3.3 TB/s.  What it is above the reading: 3 us before the first key arrives, 3 us for the join,
+// to 431 keys of their own behind 6,144, 32 / 8 heads of size 128, take 28 us for 93 MB, 3.3 TB/s; three groups of 13 with up to 777 behind
+// 2,896, 64 / 8 heads, 31 us for 112 MB, 3.6 TB/s.  What it is above the reading: 3 us before the first key arrives, 3 us for the join,
 // and SMs that wait for the slowest piece.  float32, two groups of 5 behind 608 keys, 16 / 8 heads: 13.5 us for 16 MB.
 #include "common.cuh"
 
@@ -952,8 +952,8 @@ struct Plan {
 // Into how many pieces the keys are cut, none shorter than MIN_KEYS: the tokens' own for about four CTAs an SM; the shared ones, on the
 // tensor cores, for one CTA on as many SMs as are their share of the work (a block of 128 keys takes a tile 1.2 us, a token's own
 // keys come in at 47 KB a us and SM), LEAST_SMS at least, so that attend_own's CTAs run on the others meanwhile (60 tokens with up to
-// 431 keys behind 6,144: 34.3 us with 100, 30.2 with 64, 32.5 with 48; three groups of 13 with up to 777 behind 2,896, 64 / 8 heads:
-// 45.3, 33.8, 33.7; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42 with 148, 53 with 100, 87 with 74).
+// 431 keys behind 6,144: 31.1 us with 96, 28.2 with 64, 31.2 with 48; three groups of 13 with up to 777 behind 2,896, 64 / 8 heads:
+// 39.7, 31.3, 31.3; 64 tokens with up to 64 behind 8,192, 64 / 8 heads: 42 with 148, 53 with 100, 87 with 74).
 Plan plan_of(int tokens, int groups, int num_q, int num_kv, int head_dim, int pages, int page_size, long long max_shared, long long max_own, int dtype) {
     constexpr int MIN_KEYS = 128, SMS = 148, LEAST_SMS = 64;
     const int heads = num_q / num_kv;

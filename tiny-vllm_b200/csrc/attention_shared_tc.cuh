@@ -15,8 +15,8 @@
 //
 // Bound by a block's chain (a tile's arrival, S, the softmax, P V) of 1.2 us, of which two run side by side: 16 tiles of 120 rows over
 // 6,144 keys on 64 SMs take 21 us beside attend_own's reading; whole calls, us with this kernel / with
-// attend_shared_bf16_kernel: 60 tokens behind 6,144 keys, 32 / 8 heads of size 128, 30.1 / 68.6; three groups of 13 behind 2,896, 64 / 8
-// heads, 33.8 / 59.9.
+// attend_shared_bf16_kernel: 60 tokens behind 6,144 keys, 32 / 8 heads of size 128, 28.2 / 68.6; three groups of 13 behind 2,896, 64 / 8
+// heads, 31.3 / 59.9.
 #pragma once
 
 #include "tc5.cuh"
