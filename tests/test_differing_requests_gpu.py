@@ -134,7 +134,9 @@ def test_decode_steps(dtype, hints):
             for r, (g, tokens) in enumerate(requests):
                 logits = plain_logits(w, texts[r], g, OUT_ADAPTERS[r])
                 off = (logits_seen[r].double() - logits[0]).abs().max().item() / logits.abs().max().item()
-                # float32: sums of 256 products over logits of some units; bfloat16: eight roundings on the way, 2^-8 each at the most
+                # float32: five products in line of up to 256 terms, whose sums are off by some 2^-23 sqrt(256) of what is added up, so
+                # 1e-5 in all, and twice that is allowed.  bfloat16: eight roundings on the way (each projection's two, the softmax's
+                # weights, the heads, x + out and the rest of its own), 2^-8 each at the most, all of them at once.
                 assert off < (2e-5 if dtype == torch.float32 else 8 * 2.0**-8)
                 p = params[r]
                 held = dict(slots=torch.zeros(1, dtype=torch.int32), history=torch.tensor([texts[r]], dtype=torch.int32),
