@@ -15,8 +15,8 @@
 // alone: what other adapters hold, infinities among them, does not reach it.
 // float32: the float32 cores.
 //
-// Bound by the latency of their chains of loads (ids, A and x, u, B and y) for few rows: one row 1024 -> 4096 of rank 16 takes 4.1 us
-// beside a projection of 2.8, 48 rows 4096 -> 6144 with 13 adapters of rank 16 9.9 us beside 11.6 (7 MB, 1 us at the speed of HBM).
+// Bound by the latency of their chains of loads (ids, A and x, u, B and y) for few rows: one row 1024 -> 4096 of rank 16 takes 4.4 us
+// beside a projection of 2.7, 48 rows 4096 -> 6144 with 13 adapters of rank 16 10 us beside 11.5 (7 MB, 1 us at the speed of HBM).
 // Bound by the traffic of x and y and the instructions between it for many: adapters_tma.cuh.  float32, 301 rows 1024 -> 2048 of
 // rank 8: 8 to 10 us beside 25 to 28.
 #include <cooperative_groups.h>
