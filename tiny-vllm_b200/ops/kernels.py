@@ -2180,27 +2180,30 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     them beyond rounding (default: what the tables hold).  A key
     whose page is no page of the cache is not seen.  bfloat16 and float32, head sizes 64, 128 and 256.  (The bfloat16 kernels
     have bounded waits: :func:`check_finished_launches` says whether one ran out.)"""
+    dtype, cache_shape, table_shape = q.dtype, key_cache.shape, block_tables.shape
     tokens = positions.shape[0] if positions.dim() == 1 else -1
-    tag = dtype_tag(q.dtype)
+    tag = dtype_tag(dtype)
     if head_dim not in DECODE_HEAD_DIMS or num_kv < 1 or num_q < 1 or num_q % num_kv:
         raise KernelError(f"attention_shared takes head sizes {DECODE_HEAD_DIMS} and whole groups of q heads "
                           f"(head_dim {head_dim}, {num_q} / {num_kv} heads)")
-    pages, _, page_size, _ = key_cache.shape if key_cache.dim() == 4 else (0, 0, 0, 0)
-    if page_size < 1 or not _is(key_cache, q.dtype, pages, num_kv, page_size, head_dim) \
-            or not _is(value_cache, q.dtype, pages, num_kv, page_size, head_dim):
+    pages, _, page_size, _ = cache_shape if len(cache_shape) == 4 else (0, 0, 0, 0)
+    if page_size < 1 or not _is(key_cache, dtype, pages, num_kv, page_size, head_dim) \
+            or value_cache.dtype is not dtype or value_cache.shape != cache_shape or not value_cache.is_contiguous():
         raise KernelError("attention_shared: caches must be contiguous [pages, num_kv, page_size, head_dim] of the type of q")
     if tokens < 0 or not _is(positions, torch.int32, tokens) or not _is(token_row, torch.int32, tokens):
         raise KernelError("attention_shared: token_row and positions must be contiguous int32 [tokens]")
-    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or not block_tables.is_contiguous():
+    if len(table_shape) != 2 or block_tables.dtype is not torch.int32 or not block_tables.is_contiguous():
         raise KernelError("attention_shared: block_tables must be contiguous int32 [requests, blocks]")
     groups = shared_lens.shape[0] if shared_lens.dim() == 1 else -1
     if groups < 0 or not _is(shared_lens, torch.int32, groups) or not _is(group_starts, torch.int32, groups + 1):
         raise KernelError("attention_shared: shared_lens must be contiguous int32 [groups], group_starts int32 [groups + 1]")
-    size, width = q.element_size(), num_q * head_dim
-    if not q.dim() or q.stride()[-1] != 1 or q_token_stride < width or q_token_stride * size % 16 or q.data_ptr() % 16 \
-            or tokens > 0 and q.untyped_storage().nbytes() < (q.storage_offset() + (tokens - 1) * q_token_stride + width) * size:
+    size, width, q_shape, strides, q_at = 4 if tag == F32 else 2, num_q * head_dim, q.shape, q.stride(), q.data_ptr()
+    # (a tensor [tokens or more, heads or more] with these rows holds them; of others the memory is asked)
+    holds = len(strides) == 2 and strides[0] == q_token_stride and q_shape[0] >= tokens and q_shape[1] >= width
+    if not strides or strides[-1] != 1 or q_token_stride < width or q_token_stride * size % 16 or q_at % 16 or not holds and tokens > 0 \
+            and q.untyped_storage().nbytes() < (q.storage_offset() + (tokens - 1) * q_token_stride + width) * size:
         raise KernelError("attention_shared: the heads of token t stand at q + t * q_token_stride, on 16 bytes, inside its memory")
-    held = block_tables.shape[1] * page_size
+    held = table_shape[1] * page_size
     max_shared = held if max_shared is None else max_shared
     max_own = held if max_own is None else max_own
     if not 0 <= max_shared < 2**31 or not 0 <= max_own < 2**31:
@@ -2209,7 +2212,7 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         raise KernelError("attention_shared: the scale is positive and finite")
     if out is None:
         stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
-        out = torch.empty((tokens, width), dtype=q.dtype, device=q.device)
+        out = torch.empty((tokens, width), dtype=dtype, device=q.device)
     else:
         if out.shape != (tokens, width) or out.dtype != q.dtype or out.stride(1) != 1 or tokens > 1 and out.stride(0) < width \
                 or any(_overlaps(out, t) for t in (q, key_cache, value_cache)):
@@ -2221,9 +2224,9 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, pages, page_size, max_shared, max_own, tag)
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     call = _SHARED_CALL.pack(
-        q.data_ptr(), q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_row.data_ptr(),
+        q_at, q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_row.data_ptr(),
         positions.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
-        out.data_ptr(), out.stride()[0], block_tables.shape[0], block_tables.shape[1], groups, tokens, pages, page_size, num_q,
+        out.data_ptr(), out.stride()[0], table_shape[0], table_shape[1], groups, tokens, pages, page_size, num_q,
         num_kv, head_dim, max_shared, max_own, tag, _pdl("attention_shared"), scale)
     _check(_fn("attention_shared", "tvb_attention_shared", _PACKED)(call, stream), "attention_shared", launches)
     global _attention_shared_unchecked

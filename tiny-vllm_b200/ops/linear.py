@@ -76,12 +76,13 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     result's type; the projection stays float32 in between where the result is, and where n is no multiple of 8.
 
     Rows whose adapters lie together go fastest; up to 512 they may as well come in any order."""
-    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1] or weight.dtype != x.dtype or x.shape[1] < 1:
+    x_shape, weight_shape, down_shape, dtype = x.shape, weight.shape, down.shape, x.dtype
+    if len(x_shape) != 2 or len(weight_shape) != 2 or x_shape[1] != weight_shape[1] or weight.dtype != dtype or x_shape[1] < 1:
         raise kernels.KernelError("linear_adapted wants x [m, k] and a weight [n, k] of its type")
-    (m, k), n = x.shape, weight.shape[0]
-    kernels.dtype_tag(x.dtype)
-    adapters, rank = down.shape[:2] if down.dim() == 3 else (0, 0)
-    if not kernels._is(down, x.dtype, adapters, rank, k) or not kernels._is(up, x.dtype, adapters, n, rank) or adapters < 1 \
+    (m, k), n = x_shape, weight_shape[0]
+    kernels.dtype_tag(dtype)
+    adapters, rank = (down_shape[0], down_shape[1]) if len(down_shape) == 3 else (0, 0)
+    if not kernels._is(down, dtype, adapters, rank, k) or not kernels._is(up, dtype, adapters, n, rank) or adapters < 1 \
             or not 1 <= rank <= kernels.ADAPTERS_MAX_RANK:
         raise kernels.KernelError(f"linear_adapted: down and up must be contiguous [adapters, rank, {k}] and [adapters, {n}, rank] "
                                   f"of the type of x, at least one adapter, ranks from 1 to {kernels.ADAPTERS_MAX_RANK}")
@@ -91,8 +92,8 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
         raise kernels.KernelError(f"linear_adapted: scales must be contiguous float32 [{adapters}]")
     if x.stride()[1] != 1 and k > 1:
         raise kernels.KernelError("linear_adapted: the rows of x must be contiguous")
-    out_dtype = out_dtype or (x.dtype if out is None else out.dtype)
-    if out_dtype not in (x.dtype, torch.float32):
+    out_dtype = out_dtype or (dtype if out is None else out.dtype)
+    if out_dtype != dtype and out_dtype != torch.float32:
         raise kernels.KernelError("linear_adapted: the result has the type of x, or float32")
     if out is not None and (out.shape != (m, n) or out.dtype != out_dtype or out.stride(1) != 1 and n > 1
                             or m > 1 and out.stride(0) < n or any(kernels._overlaps(out, t) for t in (x, weight, down, up))):
