@@ -33,6 +33,13 @@ def test_bad_rules_are_refused(rule):
         SamplingParams(**rule)
 
 
+@pytest.mark.parametrize("rule", [dict(repetition_penalty=1e300), dict(repetition_penalty=1e-300), dict(presence_penalty=-1e39),
+                                  dict(frequency_penalty=10**400), dict(logit_bias={1: 3.5e38})])
+def test_numbers_that_float32_does_not_have_are_refused(rule):
+    with pytest.raises(ValueError, match="float32"):
+        SamplingParams(**rule)
+
+
 @pytest.mark.parametrize("rule", [dict(repetition_penalty="1"), dict(presence_penalty=None), dict(frequency_penalty=True)])
 def test_rules_of_another_type_are_refused(rule):
     with pytest.raises(TypeError):

@@ -8,6 +8,7 @@ from dataclasses import dataclass
 
 _MAX_SEED = (1 << 64) - 1
 _MAX_BIASES = 1024
+_MIN_FLOAT32, _MAX_FLOAT32 = 2.0**-126, (2.0 - 2.0**-23) * 2.0**127          # the device keeps rules in float32
 
 
 @dataclass(frozen=True)
@@ -50,15 +51,15 @@ class SamplingParams:
             value = getattr(self, name)
             if type(value) not in (int, float):
                 raise TypeError(f"{name} must be a number")
-            if not math.isfinite(value) or (name == "repetition_penalty" and value <= 0.0):
-                raise ValueError(f"{name} must be finite" + (" and positive" if name == "repetition_penalty" else ""))
+            if not abs(value) <= _MAX_FLOAT32 or (name == "repetition_penalty" and value < _MIN_FLOAT32):
+                raise ValueError(f"{name} must be finite" + (" and positive" if name == "repetition_penalty" else "") + " in float32")
             object.__setattr__(self, name, float(value))
         pairs = self.logit_bias.items() if hasattr(self.logit_bias, "items") else self.logit_bias
         pairs = tuple(tuple(pair) for pair in pairs)
         for pair in pairs:
             if len(pair) != 2 or type(pair[0]) is not int or pair[0] < 0 or type(pair[1]) not in (int, float) \
-                    or not math.isfinite(pair[1]):
-                raise ValueError("logit_bias holds pairs of a token id and a finite number")
+                    or not abs(pair[1]) <= _MAX_FLOAT32:
+                raise ValueError("logit_bias holds pairs of a token id and a number that is finite in float32")
         if len(pairs) > _MAX_BIASES:
             raise ValueError(f"logit_bias holds up to {_MAX_BIASES} pairs")
         object.__setattr__(self, "logit_bias", pairs)
