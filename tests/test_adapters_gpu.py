@@ -203,3 +203,13 @@ def test_captured_twice_and_on_another_stream(m):
             graph.replay()
         eager = adapted(**(s | dict(x=x)))
         assert torch.equal(outs[0], wants[seed]) and torch.equal(outs[1], wants[seed]) and torch.equal(eager, wants[seed])
+
+
+def test_waits_of_many_rows_are_recorded():
+    from tinyvllm_b200.ops import kernels
+
+    s = made(700, 512, 264, 16, 3)
+    adapted(**s)
+    assert kernels._adapters_unchecked
+    kernels.check_finished_launches()                                  # none ran out
+    assert not kernels._adapters_unchecked and kernels.adapters_status() == 0

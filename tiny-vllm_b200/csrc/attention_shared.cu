@@ -1070,7 +1070,9 @@ extern "C" int tvb_attention_shared(const SharedCall* call, void* stream) {
         (long long)c.pages * c.num_kv * c.page_size > 0x7fffffffLL)
         return TVB_BAD_ARGUMENT;
     const Plan p = plan_of(c.tokens, c.groups, c.num_q, c.num_kv, c.head_dim, c.pages, c.page_size, c.max_shared, c.max_own, c.dtype);
-    if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL || (p.pieces() > 1 && !c.scratch)) return TVB_BAD_ARGUMENT;
+    if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL || (long long)c.tokens * c.num_q * p.pieces() > 0x7fffffffLL ||
+        (p.pieces() > 1 && !c.scratch))
+        return TVB_BAD_ARGUMENT;
     Attend a{c.q, c.q_stride, c.keys, c.values, c.tables, c.token_row, c.positions, c.group_starts, c.shared_lens,
              p.pieces() > 1 ? c.scratch : nullptr, nullptr, c.out, c.out_stride, c.tokens, c.rows, c.width, c.groups, c.pages, c.page_size,
              c.num_q, c.num_kv, p.shared_pieces, p.own_pieces, p.own_tiles, c.scale * LOG2E};

@@ -190,6 +190,13 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(barrier));
         };
+        // where the row's result goes (-1: nowhere); asked for here, while the first tiles come in
+        int place = -1;
+        if (group == 0 && row < p.rows) {
+            int head;
+            const int token = token_of(a, p, row, head);
+            if (takes_part(a, p, token)) place = (int)part_of(a, token, head, p.slot);
+        }
         float reference = -INFINITY, l = 0.0f;  // what the exponentials of this row subtract (log2); the group's denominator
         bool alive = true;
         int next_page = page_of(group);
@@ -271,7 +278,7 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
         // warp stores whole rows; 16-byte word w of row r lies in place w ^ (r % 32, or % 16 for 64 values).
         constexpr int WORDS = HD / 4;
         const bool second = blocks > 1;         // else the second group had no block, and its O holds nothing
-        int64_t* places = reinterpret_cast<int64_t*>(exchange + TC_ROWS * 2);
+        int* places = reinterpret_cast<int*>(exchange + TC_ROWS * 2);
         uint4* staged = reinterpret_cast<uint4*>(aligned + T::TILE);
         static_assert(TC_ROWS * HD * 4 <= (T::K_RING + T::V_RING) * T::TILE, "room for the results");
         if (alive) alive = warp_wait(T::O_LAST, 0, 13);
@@ -288,13 +295,8 @@ attend_shared_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_
             const float top = fmaxf(reference, other);
             const float mine = reference == -INFINITY ? 0.0f : exp2_unit(reference - top);
             const float theirs = other == -INFINITY ? 0.0f : exp2_unit(other - top);
-            const bool here = alive && row < p.rows;
-            int head = 0;
-            const int token = here ? token_of(a, p, row, head) : 0;
-            const bool takes = here && takes_part(a, p, token);
-            const int64_t at = takes ? part_of(a, token, head, p.slot) : -1;
-            places[row] = at;
-            if (takes) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(top, l * mine + other_l * theirs);
+            places[row] = alive ? place : -1;
+            if (alive && place >= 0) *reinterpret_cast<float2*>(a.part_ml + (int64_t)place * 2) = make_float2(top, l * mine + other_l * theirs);
             if (alive)
 #pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
