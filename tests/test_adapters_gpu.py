@@ -102,6 +102,29 @@ def test_rows_in_any_order(m, adapters, rank):
     check(adapted(**other, out_dtype=torch.float32), other)
 
 
+@pytest.mark.parametrize("rank", [4, 5, 16])
+@pytest.mark.parametrize("adapters", [3, 40])
+@pytest.mark.parametrize("m", [5, 100, 192, 193, 512, 600])
+def test_widths_that_are_no_multiple_of_8_are_rounded_once(m, adapters, rank):
+    """Every way the rows go, and rows without an adapter among them; the bound has one rounding to bfloat16."""
+    s = made(m, 136, 171, rank, adapters)
+    memory = torch.full((m, 180), 3.0, dtype=BF16, device=DEV)
+    got = adapted(**s, out=memory[:, 5:176])
+    check(got, s)
+    wide = {name: t.double() for name, t in s.items() if name not in ("ids", "scales")}
+    has = (s["ids"] >= 0)[:, None]
+    rows = s["ids"].long().clamp(min=0)
+    narrow = torch.einsum("tk,trk->tr", wide["x"], wide["down"][rows]) * s["scales"].double()[rows][:, None]
+    want = wide["x"] @ wide["weight"].t() + torch.where(has, torch.einsum("tr,tnr->tn", narrow, wide["up"][rows]), 0.0)
+    # sums of 136 products, then of up to 16: 2^-23 of some 12 + 4 times their size each, u in two parts; one rounding, 2^-8 of the result
+    sizes = wide["x"].abs() @ wide["weight"].abs().t() + torch.where(has, torch.einsum(
+        "tr,tnr->tn", torch.einsum("tk,trk->tr", wide["x"].abs(), wide["down"][rows].abs()) * s["scales"].double().abs()[rows][:, None],
+        wide["up"][rows].abs()), 0.0)
+    bound = ((136 + rank + 24) * 2.0**-23 + 2.0**-16) * sizes
+    assert ((got.double() - want).abs() <= bound + 2.0**-8 * (want.abs() + bound)).all()
+    assert (memory[:, :5] == 3).all() and (memory[:, 176:] == 3).all()
+
+
 @pytest.mark.parametrize("kind", ["one", "none", "spans"])
 @pytest.mark.parametrize("m", [20, 333])
 def test_which_rows_have_which(kind, m):
