@@ -1067,8 +1067,9 @@ extern "C" int tvb_attention_shared(const SharedCall* call, void* stream) {
     if (c.tokens <= 0) return 0;
     if ((c.dtype != TVB_F32 && c.dtype != TVB_BF16) || c.num_kv <= 0 || c.num_q <= 0 || c.num_q % c.num_kv || c.page_size <= 0 || c.groups < 0 ||
         c.rows < 0 || c.width < 0 || c.max_shared < 0 || c.max_own < 0 || (long long)c.width * c.page_size > 0x7fffffffLL - 4096 ||
-        (long long)c.pages * c.num_kv * c.page_size > 0x7fffffffLL)
-        return TVB_BAD_ARGUMENT;
+        (long long)c.pages * c.num_kv * c.page_size > 0x7fffffffLL || (((uintptr_t)c.q | (uintptr_t)c.keys | (uintptr_t)c.values) & 15) ||
+        c.q_stride * (c.dtype == TVB_F32 ? 4 : 2) % 16)
+        return TVB_BAD_ARGUMENT;                // (loads of 16 bytes)
     const Plan p = plan_of(c.tokens, c.groups, c.num_q, c.num_kv, c.head_dim, c.pages, c.page_size, c.max_shared, c.max_own, c.dtype);
     if (p.shared_items > 0x7fffffffLL || p.own_items > 0x7fffffffLL || (long long)c.tokens * c.num_q * p.pieces() > 0x7fffffffLL ||
         (p.pieces() > 1 && !c.scratch))

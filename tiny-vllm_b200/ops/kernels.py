@@ -2190,6 +2190,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     if page_size < 1 or not _is(key_cache, dtype, pages, num_kv, page_size, head_dim) \
             or value_cache.dtype is not dtype or value_cache.shape != cache_shape or not value_cache.is_contiguous():
         raise KernelError("attention_shared: caches must be contiguous [pages, num_kv, page_size, head_dim] of the type of q")
+    if (key_cache.data_ptr() | value_cache.data_ptr()) % 16:
+        raise KernelError("attention_shared: the caches must start on 16 bytes")
     if tokens < 0 or not _is(positions, torch.int32, tokens) or not _is(token_row, torch.int32, tokens):
         raise KernelError("attention_shared: token_row and positions must be contiguous int32 [tokens]")
     if len(table_shape) != 2 or block_tables.dtype is not torch.int32 or not block_tables.is_contiguous():
