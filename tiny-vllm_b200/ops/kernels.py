@@ -2126,11 +2126,19 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch
         u.data_ptr(), y.data_ptr(), y.stride()[0], out.data_ptr(), out.stride()[0], m, n, k, rank, adapters, tag, dtype_tag(y.dtype),
         dtype_tag(out.dtype), _pdl("gemm"))
     _check(_fn("adapters", "tvb_add_adapters", _PACKED)(call, stream), "add_adapters", 2)
-    global _adapters_unchecked
-    _adapters_unchecked = _adapters_unchecked or (tag == BF16 and m > ADAPTERS_FEW_ROWS)
+    if tag == BF16 and m > ADAPTERS_FEW_ROWS:
+        _note_adapters_launch()
 
 
-_adapters_unchecked = False
+_adapters_unchecked = _adapters_captured = False
+
+
+def _note_adapters_launch() -> None:
+    """Kernels with bounded waits were launched, or recorded: a graph's replays are not seen here, so from then on every check reads
+    their status word."""
+    global _adapters_unchecked, _adapters_captured
+    _adapters_unchecked = True
+    _adapters_captured = _adapters_captured or torch.cuda.is_current_stream_capturing()
 
 
 def adapters_status() -> int:
@@ -2152,7 +2160,14 @@ def _shared_plan(*sizes: int) -> tuple[int, int]:
 
 
 _SHARED_CALL = struct.Struct("@PqPPPPPPPPPqiiiiiiiiiiiiif")
-_attention_shared_unchecked = False
+_attention_shared_unchecked = _attention_shared_captured = False
+
+
+def _note_attention_shared_launch() -> None:
+    """As :func:`_note_adapters_launch`."""
+    global _attention_shared_unchecked, _attention_shared_captured
+    _attention_shared_unchecked = True
+    _attention_shared_captured = _attention_shared_captured or torch.cuda.is_current_stream_capturing()
 
 
 def attention_shared_status() -> int:
@@ -2231,8 +2246,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         out.data_ptr(), out.stride()[0], table_shape[0], table_shape[1], groups, tokens, pages, page_size, num_q,
         num_kv, head_dim, max_shared, max_own, tag, _pdl("attention_shared"), scale)
     _check(_fn("attention_shared", "tvb_attention_shared", _PACKED)(call, stream), "attention_shared", launches)
-    global _attention_shared_unchecked
-    _attention_shared_unchecked = _attention_shared_unchecked or tag == BF16
+    if tag == BF16:
+        _note_attention_shared_launch()
     return out
 
 
@@ -2794,7 +2809,8 @@ def guarded_launch_counts() -> tuple[int, int]:
     """How often (gemm_tc, gemm_stream or gemm_f32_tc, attention_prefill_tc), the kernels with bounded waits, were launched
     through this module so far.  A caller that records a step into a CUDA graph compares the
     counts around one pass of the step and hands what it finds to :func:`note_guarded_launches`
-    at every replay: a replay launches the kernels without passing through this module."""
+    at every replay: a replay launches the kernels without passing through this module.  (Of :func:`attention_shared` and the
+    adapters nothing has to be handed over: once they have been recorded, every check reads their status words.)"""
     return _guarded_counts[0], _guarded_counts[1]
 
 
@@ -2808,7 +2824,8 @@ def note_guarded_launches(gemm: bool, attention: bool) -> None:
 
 def check_finished_launches() -> None:
     """Call after a step's results have reached the host: raises if a kernel with bounded waits
-    gave up in a launch since the last call.  Costs nothing when no such kernel was launched."""
+    gave up in a launch since the last call.  Costs nothing when no such kernel was launched (and none of
+    :func:`attention_shared` or the adapters ever recorded into a graph: that costs a read at every call)."""
     if _gemm_tc_unchecked:
         status = gemm_tc_status()
         if status:
@@ -2829,12 +2846,12 @@ def check_finished_launches() -> None:
         if status:
             raise KernelError(f"attention_prefill_tc: a wait inside the kernel ran out (code {status}); "
                               "the results of this step are not valid")
-    if _attention_shared_unchecked:
+    if _attention_shared_unchecked or _attention_shared_captured:
         status = attention_shared_status()
         if status:
             raise KernelError(f"attention_shared: a wait inside the kernel ran out (code {status}); "
                               "the results of this step are not valid")
-    if _adapters_unchecked:
+    if _adapters_unchecked or _adapters_captured:
         status = adapters_status()
         if status:
             raise KernelError(f"add_adapters: a wait inside the kernel ran out (code {status}); "
