@@ -75,20 +75,37 @@ __device__ __forceinline__ int shared_piece_keys(int n, int pieces) { return max
 __device__ __forceinline__ int shared_of_group(const Attend& a, int group) {
     return (int)min((int64_t)max(__ldcg(a.shared_lens + group), 0), (int64_t)a.width * a.page_size);
 }
+// The groups of a warp's lanes, 32 at a time: where the starts fall, a group begins (and ends) no earlier than the largest before it, so
+// that no token stands in two groups, whatever the starts are, and no row has two writers.  `upto`: the end of the groups before.
+__device__ __forceinline__ void keep_ascending(int& start, int& end, int& upto) {
+    if (__any_sync(0xffffffffu, start > end || start < upto)) {
+        int top = start;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, top, d);
+            if ((int)(threadIdx.x & 31) >= d) top = max(top, other);
+        }
+        start = max(top, upto);
+        end = max(start, end);
+    }
+    upto = __shfl_sync(0xffffffffu, end, 31);
+}
 // What a token reads: the row of its table (-1: it is none), its keys, and how many of them its group reads for it (those it
 // shares if it reads them all, else none).  A whole warp asks, 32 groups at a time, all loads side by side.
 struct Facts { int row, keys, shared; };
 __device__ __forceinline__ Facts facts_of(const Attend& a, int token) {
     const int lane = threadIdx.x & 31;
     Facts f{__ldcg(a.token_row + token), __ldcg(a.positions + token), 0};
+    int upto = 0;
     if (a.shared_pieces > 0)
         for (int g0 = 0; g0 < a.groups; g0 += 32) {
-            int start = 0x7fffffff, end = 0, shared = 0;
+            int start = 0x7fffffff, end = 0x7fffffff, shared = 0;
             if (g0 + lane < a.groups) {
-                start = __ldcg(a.group_starts + g0 + lane);
-                end = __ldcg(a.group_starts + g0 + lane + 1);
+                start = max(__ldcg(a.group_starts + g0 + lane), 0);
+                end = max(__ldcg(a.group_starts + g0 + lane + 1), 0);
                 shared = shared_of_group(a, g0 + lane);
             }
+            keep_ascending(start, end, upto);
             const uint32_t found = __ballot_sync(0xffffffffu, start <= token && token < end);
             if (found) {
                 f.shared = __shfl_sync(0xffffffffu, shared, __ffs(found) - 1);
@@ -135,15 +152,15 @@ __device__ __forceinline__ bool find_shared_piece(const Attend& a, int tile_rows
     p.kv_head = item % a.num_kv;
     int tile = item / a.num_kv;
     // the group that has the tile: 32 groups at a time
+    int groups_upto = 0;
     for (int g0 = 0; g0 < a.groups; g0 += 32) {
-        int start = 0, end = 0, shared = 0;
+        int start = a.tokens, end = a.tokens, shared = 0;
         if (g0 + lane < a.groups) {
-            start = __ldcg(a.group_starts + g0 + lane);
-            end = __ldcg(a.group_starts + g0 + lane + 1);
+            start = min(max(__ldcg(a.group_starts + g0 + lane), 0), a.tokens);
+            end = min(max(__ldcg(a.group_starts + g0 + lane + 1), 0), a.tokens);
             shared = shared_of_group(a, g0 + lane);
-            start = min(max(start, 0), a.tokens);
-            end = min(max(end, start), a.tokens);
         }
+        keep_ascending(start, end, groups_upto);
         const int count = shared > 0 ? ((end - start) * heads + tile_rows - 1) / tile_rows : 0;
         int upto = count;
 #pragma unroll

@@ -2187,7 +2187,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     [pages, num_kv, page_size, head_dim]; int32 tables, rows and positions; a token whose row or position is negative is
     padding and gets zeros), for tokens of which groups share their first keys.
 
-    Group g is the tokens ``group_starts[g]`` to ``group_starts[g + 1]`` - 1 (int32 [groups + 1], ascending); its first
+    Group g is the tokens ``group_starts[g]`` to ``group_starts[g + 1]`` - 1 (int32 [groups + 1], ascending; a start
+    below an earlier one counts as that one); its first
     ``shared_lens[g]`` (int32 [groups]) positions hold the same keys and values for all of them, which are read once, through
     the table of the group's first token that reaches them all.  A token that ends before them, or stands in no group, reads
     its keys by itself.  ``max_shared`` and ``max_own``: no group shares more, no token has more keys behind its group's;
