@@ -66,11 +66,35 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t* r, const bf16* p) {
 // What both kernels agree on: u as `hi` and `lo` rows [m][2][padded rank] (bfloat16), or [m][rank] (float32).
 __device__ __forceinline__ int padded_rank(int rank) { return (rank + 15) / 16 * 16; }
 
-// u of a row and rank: scaled, in two parts; places behind the rank are zeros
+// u of a row and rank: scaled, in two parts; places behind the rank are zeros.  The head of a number that bfloat16 would round to
+// infinity is the largest one it has, and an infinite u has no rest (infinity - infinity).
+constexpr float BF16_MOST = 3.3895313892515355e38f;
 __device__ __forceinline__ void store_u(bf16* u, int row, int rank, int padded, float value) {
-    const bf16 hi = from_float<bf16>(value);
+    const bool infinite = isinf(value);
+    const bf16 hi = from_float<bf16>(infinite ? value : value > BF16_MOST ? BF16_MOST : value < -BF16_MOST ? -BF16_MOST : value);
     u[((int64_t)row * 2) * padded + rank] = hi;
-    u[((int64_t)row * 2 + 1) * padded + rank] = from_float<bf16>(value - to_float<bf16>(hi));
+    u[((int64_t)row * 2 + 1) * padded + rank] = from_float<bf16>(infinite ? 0.0f : value - to_float<bf16>(hi));
+}
+// Sums of products of u's two parts with a B that is infinite, or of an infinite u, hold infinity - infinity or 0 * infinity where the
+// definition has infinity.  So a thread whose sums are not all finite makes them again from u itself: `columns` of them, the i-th of
+// column column_of(i), `row`s u, the adapter's B.
+__device__ __forceinline__ bool all_finite(const float* v, int count) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < count; ++i) zero = fmaf(v[i], 0.0f, zero);
+    return zero == 0.0f;
+}
+template <int COLUMNS, typename F>
+__device__ __forceinline__ void sums_again(float (&sums)[COLUMNS], const bf16* u, int padded, const bf16* b, int rank, int n, const F& column_of) {
+#pragma unroll
+    for (int i = 0; i < COLUMNS; ++i) sums[i] = 0.0f;
+#pragma unroll 1
+    for (int r = 0; r < rank; ++r) {
+        const float value = to_float<bf16>(u[r]) + to_float<bf16>(u[padded + r]);
+#pragma unroll
+        for (int i = 0; i < COLUMNS; ++i)
+            if (column_of(i) < n) sums[i] = fmaf(value, to_float<bf16>(b[(int64_t)column_of(i) * rank + r]), sums[i]);
+    }
 }
 
 struct Shrink {
@@ -565,6 +589,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
             float add[8];
 #pragma unroll
             for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
+            if (!all_finite(add, 8)) sums_again(add, u[h], padded, b, s.rank, s.n, [&](int i) { return tile * 32 + 8 * t + i; });
             float v[8];
             if constexpr (sizeof(Y) == 2) {
                 unpack_bf16x8(now[h][0], v);

@@ -254,13 +254,21 @@ __global__ void __launch_bounds__(TMA_THREADS, 4) expand_tma_kernel(const __grid
                     }
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        if (mine[h])
+                        if (mine[h]) {
+                            float add[16];
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
+                            if (!all_finite(add, 16))
+                                sums_again(add, reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + rows[h]) * 2 * padded, padded,
+                                           reinterpret_cast<const bf16*>(s.up) + (int64_t)distinct[d] * s.n * s.rank, s.rank, s.n,
+                                           [&](int c) { return (tile0 + i) * S::COLUMNS + c / 2 * 8 + 2 * t + c % 2; });
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t to = swizzled(y_s, rows[h], j) + 4 * t, v = load_shared_32(to);
-                                store_shared_32(to, pack_bf16x2(__uint_as_float(v << 16) + sums[j][2 * h],
-                                                                __uint_as_float(v & 0xffff0000u) + sums[j][2 * h + 1]));
+                                store_shared_32(to, pack_bf16x2(__uint_as_float(v << 16) + add[2 * j],
+                                                                __uint_as_float(v & 0xffff0000u) + add[2 * j + 1]));
                             }
+                        }
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(b_empty(at));
