@@ -23,3 +23,16 @@ def test_caches_off_the_16_bytes(offset, dtype, name, page):
     aligned = offset * buffer.element_size() % 16 == 0
     with pytest.raises(kernels.KernelError, match="CUDA tensors only" if aligned else "16 bytes"):
         call(arguments)
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, 2.4e38, 3.4e38, 1e39, 1e300])
+def test_scales_that_float32_does_not_have(scale):
+    """1e-46 would be 0 (times -inf for a masked score: NaN), 2.4e38 infinite times log2(e), 1e39 infinite."""
+    with pytest.raises(kernels.KernelError, match="scale"):
+        call(good() | dict(scale=scale))
+
+
+@pytest.mark.parametrize("scale", [2.0**-126, 1e-30, 1.0, 2.0**127])
+def test_scales_that_it_has(scale):
+    with pytest.raises(kernels.KernelError, match="CUDA tensors only"):
+        call(good() | dict(scale=scale))

@@ -2159,6 +2159,7 @@ def _shared_plan(*sizes: int) -> tuple[int, int]:
     return floats, launches.value
 
 
+_SCALE_LEAST, _SCALE_MOST = 2.0**-126, 2.0**127     # the kernel has scale * log2(e) in float32 (and 0 * -inf for a masked key's score)
 _SHARED_CALL = struct.Struct("@PqPPPPPPPPPqiiiiiiiiiiiiif")
 _attention_shared_unchecked = _attention_shared_captured = False
 
@@ -2226,8 +2227,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     max_own = held if max_own is None else max_own
     if not 0 <= max_shared < 2**31 or not 0 <= max_own < 2**31:
         raise KernelError("attention_shared: max_shared and max_own are not negative and have 31 bits")
-    if not 0.0 < scale < float("inf"):
-        raise KernelError("attention_shared: the scale is positive and finite")
+    if not _SCALE_LEAST <= scale <= _SCALE_MOST:
+        raise KernelError("attention_shared: the scale is positive and finite, in float32 and times log2(e)")
     if out is None:
         stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
         out = torch.empty((tokens, width), dtype=dtype, device=q.device)
