@@ -1,0 +1,25 @@
+"""Results in memory that the same call reads are refused on the host, whatever the types of the two are."""
+
+import pytest
+import torch
+
+import test_logit_rules
+from tinyvllm_b200.ops import kernels
+
+
+def over(other, like):
+    """``like``'s shape and type in memory that begins with the last four bytes of ``other`` (which moves there)."""
+    size = other.numel() * other.element_size()
+    memory = torch.zeros(size + like.numel() * like.element_size() + 64, dtype=torch.uint8)
+    moved = memory[:size].view(other.dtype).view(other.shape).copy_(other)
+    start = size - 4
+    return moved, memory[start:start + like.numel() * like.element_size()].view(like.dtype).view(like.shape)
+
+
+@pytest.mark.parametrize("name", ["slots", "penalties", "lengths", "history", "bias_tokens", "bias_values", "masks", "mask_rows"])
+def test_rules(name):
+    arguments = test_logit_rules.good()
+    arguments[name], out = over(arguments[name], arguments["logits"])
+    for logits in (arguments["logits"], out):              # elsewhere, and in place
+        with pytest.raises(kernels.KernelError, match="memory of its own"):
+            test_logit_rules.call(dict(arguments, logits=logits, out=out))

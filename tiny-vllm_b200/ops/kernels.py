@@ -2004,16 +2004,21 @@ def _here(who: str, *tensors: torch.Tensor | None) -> int:
 _PACKED = [ctypes.c_char_p, c_void_p]
 
 
-def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the memory from the first to the last element of two tensors has bytes in common."""
+def _overlaps(written: torch.Tensor, *others: torch.Tensor | None) -> bool:
+    """Whether the memory from the first to the last element of a tensor has bytes in common with that of one of the others."""
     def span(t):
-        last = sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+        at, count = t.data_ptr(), t.numel()
+        if count and not t.is_contiguous():
+            count = 1 + sum((size - 1) * stride for size, stride in zip(t.shape, t.stride()))
+        return at, at + count * t.element_size()
 
-    if a.numel() == 0 or b.numel() == 0:
-        return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    first, end = span(written)
+    for other in others:
+        if other is not None:
+            at, past = span(other)
+            if max(first, at) < min(end, past):
+                return True
+    return False
 
 
 # ------------------------------------------------------------ rules on logits
@@ -2078,7 +2083,8 @@ def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.T
         if out.shape != logits.shape or out.dtype != logits.dtype or out.stride(1) != 1 and vocab > 1 \
                 or rows > 1 and out.stride(0) < vocab:
             raise KernelError("logit_rules: out must be [rows, vocab] of the type of the logits with contiguous rows of its own")
-        if (out.data_ptr() != logits.data_ptr() or out.stride(0) != logits.stride(0)) and _overlaps(out, logits):
+        if (out.data_ptr() != logits.data_ptr() or out.stride(0) != logits.stride(0)) and _overlaps(out, logits) \
+                or _overlaps(out, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows):
             raise KernelError("logit_rules: out is the logits themselves, or memory of its own")
         stream = _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows, out)
     call = _RULES_CALL.pack(
