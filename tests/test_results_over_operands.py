@@ -23,3 +23,13 @@ def test_rules(name):
     for logits in (arguments["logits"], out):              # elsewhere, and in place
         with pytest.raises(kernels.KernelError, match="memory of its own"):
             test_logit_rules.call(dict(arguments, logits=logits, out=out))
+
+
+@pytest.mark.parametrize("written, read", [("history", "tokens"), ("history", "slots"), ("lengths", "tokens"), ("lengths", "slots"),
+                                           ("history", "lengths")])
+def test_appended_tokens(written, read):
+    arguments = dict(tokens=torch.zeros(2, dtype=torch.int32), slots=torch.zeros(2, dtype=torch.int32),
+                     lengths=torch.zeros(3, 2, dtype=torch.int32), history=torch.zeros(3, 5, dtype=torch.int32))
+    arguments[read], arguments[written] = over(arguments[read], arguments[written])
+    with pytest.raises(kernels.KernelError, match="memory of their own"):
+        kernels.append_tokens(arguments.pop("tokens"), **arguments)

@@ -2105,6 +2105,8 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
     if history.dim() != 2 or history.dtype != torch.int32 or not history.is_contiguous() \
             or not _is(lengths, torch.int32, history.shape[0], 2):
         raise KernelError("append_tokens: history must be contiguous int32 [slots, room], lengths int32 [slots, 2]")
+    if _overlaps(lengths, tokens, slots, history) or _overlaps(history, tokens, slots):
+        raise KernelError("append_tokens: lengths and history are memory of their own")
     _here("append_tokens", tokens, slots, lengths, history)
     fn = _fn("logit_rules", "tvb_append_tokens", [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_void_p])
     _check(fn(slots.data_ptr(), tokens.data_ptr(), tokens.shape[0], lengths.data_ptr(), history.data_ptr(), history.shape[0],
