@@ -33,3 +33,13 @@ def test_appended_tokens(written, read):
     arguments[read], arguments[written] = over(arguments[read], arguments[written])
     with pytest.raises(kernels.KernelError, match="memory of their own"):
         kernels.append_tokens(arguments.pop("tokens"), **arguments)
+
+
+@pytest.mark.parametrize("name", ["x", "weight", "down", "up", "ids", "scales"])
+def test_adapters(name):
+    import test_adapters as adapters
+
+    arguments = adapters.good()
+    arguments[name], out = over(arguments[name], torch.zeros(3, 24, dtype=torch.bfloat16))
+    with pytest.raises(kernels.KernelError, match="memory of its own"):
+        adapters.linear_adapted(**arguments, out=out)

@@ -110,7 +110,7 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
     if out_dtype != dtype and out_dtype != torch.float32:
         raise kernels.KernelError("linear_adapted: the result has the type of x, or float32")
     if out is not None and (out.shape != (m, n) or out.dtype != out_dtype or out.stride(1) != 1 and n > 1
-                            or m > 1 and out.stride(0) < n or any(kernels._overlaps(out, t) for t in (x, weight, down, up))):
+                            or m > 1 and out.stride(0) < n or kernels._overlaps(out, x, weight, down, up, ids, scales)):
         raise kernels.KernelError(f"linear_adapted: out must be {out_dtype} [{m}, {n}] with contiguous rows, in memory of its own")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or down.requires_grad or up.requires_grad
                                     or scales is not None and scales.requires_grad or out is not None and out.requires_grad):
