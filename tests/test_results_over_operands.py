@@ -43,3 +43,13 @@ def test_adapters(name):
     arguments[name], out = over(arguments[name], torch.zeros(3, 24, dtype=torch.bfloat16))
     with pytest.raises(kernels.KernelError, match="memory of its own"):
         adapters.linear_adapted(**arguments, out=out)
+
+
+@pytest.mark.parametrize("name", ["q", "key_cache", "value_cache", "block_tables", "token_row", "positions", "group_starts", "shared_lens"])
+def test_attention_over_keys_in_common(name):
+    import test_attention_shared as shared
+
+    arguments = shared.good()
+    arguments[name], out = over(arguments[name], torch.zeros(3, 256, dtype=torch.bfloat16))
+    with pytest.raises(kernels.KernelError, match="memory of its own"):
+        shared.call(arguments | dict(out=out))

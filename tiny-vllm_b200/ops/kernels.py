@@ -2242,7 +2242,7 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         out = torch.empty((tokens, width), dtype=dtype, device=q.device)
     else:
         if out.shape != (tokens, width) or out.dtype != q.dtype or out.stride(1) != 1 or tokens > 1 and out.stride(0) < width \
-                or any(_overlaps(out, t) for t in (q, key_cache, value_cache)):
+                or _overlaps(out, q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens):
             raise KernelError("attention_shared: out must be [tokens, num_q * head_dim] of the type of q with contiguous rows, in memory "
                               "of its own")
         stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens, out)
