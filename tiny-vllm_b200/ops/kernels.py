@@ -2115,6 +2115,7 @@ def append_tokens(tokens: torch.Tensor, *, slots: torch.Tensor, lengths: torch.T
 
 # ------------------------------------------------------------- low-rank adapters
 ADAPTERS_MAX_RANK = 256            # MAX_RANK of adapters.cu
+ADAPTERS_MAX_ROWS = 16 * 65535     # tiles of 16 rows along a grid's y
 ADAPTERS_FEW_ROWS = 192            # more rows may go through the kernels with bounded waits there
 
 

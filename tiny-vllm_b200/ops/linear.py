@@ -106,6 +106,8 @@ def linear_adapted(x: torch.Tensor, weight: torch.Tensor, down: torch.Tensor, up
         raise kernels.KernelError(f"linear_adapted: scales must be contiguous float32 [{adapters}]")
     if x.stride()[1] != 1 and k > 1:
         raise kernels.KernelError("linear_adapted: the rows of x must be contiguous")
+    if m > kernels.ADAPTERS_MAX_ROWS:
+        raise kernels.KernelError(f"linear_adapted takes up to {kernels.ADAPTERS_MAX_ROWS} rows")
     out_dtype = out_dtype or (dtype if out is None else out.dtype)
     if out_dtype != dtype and out_dtype != torch.float32:
         raise kernels.KernelError("linear_adapted: the result has the type of x, or float32")
