@@ -2004,6 +2004,12 @@ def _here(who: str, *tensors: torch.Tensor | None) -> int:
 _PACKED = [ctypes.c_char_p, c_void_p]
 
 
+def _no_gradients(who: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse operands whose gradients are wanted: there is no backward pass, and the result would be cut off without a word."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise KernelError(f"{who} has no backward pass: call it under torch.no_grad() or torch.inference_mode()")
+
+
 def _overlaps(written: torch.Tensor, *others: torch.Tensor | None) -> bool:
     """Whether the memory from the first to the last element of a tensor has bytes in common with that of one of the others."""
     def span(t):
@@ -2076,6 +2082,7 @@ def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.T
                 or not _is(mask_rows, torch.int32, count):
             raise KernelError(f"logit_rules: masks must be contiguous int32 [masks, at least {-(-vocab // 32)}], "
                               f"mask_rows int32 [{count}]")
+    _no_gradients("logit_rules", logits, penalties, bias_values, out)
     if out is None:
         stream = _here("logit_rules", logits, slots, penalties, lengths, history, bias_tokens, bias_values, masks, mask_rows)
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
