@@ -36,3 +36,13 @@ def test_scales_that_float32_does_not_have(scale):
 def test_scales_that_it_has(scale):
     with pytest.raises(kernels.KernelError, match="CUDA tensors only"):
         call(good() | dict(scale=scale))
+
+
+@pytest.mark.parametrize("name", ["q", "key_cache", "value_cache", "out"])
+def test_operands_that_want_gradients(name):
+    arguments = good() | dict(out=torch.zeros(3, 256, dtype=BF16))
+    arguments[name].requires_grad_(True)
+    with pytest.raises(kernels.KernelError, match="backward"):
+        call(arguments)
+    with torch.no_grad(), pytest.raises(kernels.KernelError, match="CUDA tensors only"):
+        call(arguments)

@@ -2245,6 +2245,7 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
         raise KernelError("attention_shared: max_shared and max_own are not negative and have 31 bits")
     if not _SCALE_LEAST <= scale <= _SCALE_MOST:
         raise KernelError("attention_shared: the scale is positive and finite, in float32 and times log2(e)")
+    _no_gradients("attention_shared", q, key_cache, value_cache, out)
     if out is None:
         stream = _here("attention_shared", q, key_cache, value_cache, block_tables, token_row, positions, group_starts, shared_lens)
         out = torch.empty((tokens, width), dtype=dtype, device=q.device)
