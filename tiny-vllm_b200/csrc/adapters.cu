@@ -76,24 +76,28 @@ __device__ __forceinline__ void store_u(bf16* u, int row, int rank, int padded, 
     u[((int64_t)row * 2 + 1) * padded + rank] = from_float<bf16>(infinite ? 0.0f : value - to_float<bf16>(hi));
 }
 // Sums of products of u's two parts with a B that is infinite, or of an infinite u, hold infinity - infinity or 0 * infinity where the
-// definition has infinity.  So a thread whose sums are not all finite makes them again from u itself: `columns` of them, the i-th of
-// column column_of(i), `row`s u, the adapter's B.
-__device__ __forceinline__ bool all_finite(const float* v, int count) {
+// definition has infinity.  So a thread makes those of its sums that are not finite (the i-th is of column column_of(i), of which there
+// are n) again from u itself and the adapter's B.
+template <int COLUMNS, typename F>
+__device__ __forceinline__ void mend_sums(float (&sums)[COLUMNS], const bf16* u, int padded, const bf16* b, int rank, int n, const F& column_of) {
     float zero = 0.0f;
 #pragma unroll
-    for (int i = 0; i < count; ++i) zero = fmaf(v[i], 0.0f, zero);
-    return zero == 0.0f;
-}
-template <int COLUMNS, typename F>
-__device__ __forceinline__ void sums_again(float (&sums)[COLUMNS], const bf16* u, int padded, const bf16* b, int rank, int n, const F& column_of) {
+    for (int i = 0; i < COLUMNS; ++i) zero = fmaf(sums[i], 0.0f, zero);
+    if (zero == 0.0f) return;
+    uint32_t again = 0;
 #pragma unroll
-    for (int i = 0; i < COLUMNS; ++i) sums[i] = 0.0f;
+    for (int i = 0; i < COLUMNS; ++i)
+        if (column_of(i) < n && !isfinite(sums[i])) {
+            again |= 1u << i;
+            sums[i] = 0.0f;
+        }
+    if (again == 0) return;                     // (columns that are none)
 #pragma unroll 1
     for (int r = 0; r < rank; ++r) {
         const float value = to_float<bf16>(u[r]) + to_float<bf16>(u[padded + r]);
 #pragma unroll
         for (int i = 0; i < COLUMNS; ++i)
-            if (column_of(i) < n) sums[i] = fmaf(value, to_float<bf16>(b[(int64_t)column_of(i) * rank + r]), sums[i]);
+            if (again >> i & 1u) sums[i] = fmaf(value, to_float<bf16>(b[(int64_t)column_of(i) * rank + r]), sums[i]);
     }
 }
 
@@ -589,7 +593,7 @@ __device__ __forceinline__ void expand_rows(const Expand& s, int adapter, const 
             float add[8];
 #pragma unroll
             for (int j = 0; j < NT; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
-            if (!all_finite(add, 8)) sums_again(add, u[h], padded, b, s.rank, s.n, [&](int i) { return tile * 32 + 8 * t + i; });
+            mend_sums(add, u[h], padded, b, s.rank, s.n, [&](int i) { return tile * 32 + 8 * t + i; });
             float v[8];
             if constexpr (sizeof(Y) == 2) {
                 unpack_bf16x8(now[h][0], v);

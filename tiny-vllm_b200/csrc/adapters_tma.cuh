@@ -258,10 +258,9 @@ __global__ void __launch_bounds__(TMA_THREADS, 4) expand_tma_kernel(const __grid
                             float add[16];
 #pragma unroll
                             for (int j = 0; j < 8; ++j) { add[2 * j] = sums[j][2 * h]; add[2 * j + 1] = sums[j][2 * h + 1]; }
-                            if (!all_finite(add, 16))
-                                sums_again(add, reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + rows[h]) * 2 * padded, padded,
-                                           reinterpret_cast<const bf16*>(s.up) + (int64_t)distinct[d] * s.n * s.rank, s.rank, s.n,
-                                           [&](int c) { return (tile0 + i) * S::COLUMNS + c / 2 * 8 + 2 * t + c % 2; });
+                            mend_sums(add, reinterpret_cast<const bf16*>(s.u) + (int64_t)(row0 + rows[h]) * 2 * padded, padded,
+                                      reinterpret_cast<const bf16*>(s.up) + (int64_t)distinct[d] * s.n * s.rank, s.rank, s.n,
+                                      [&](int c) { return (tile0 + i) * S::COLUMNS + c / 2 * 8 + 2 * t + c % 2; });
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
                                 const uint32_t to = swizzled(y_s, rows[h], j) + 4 * t, v = load_shared_32(to);
