@@ -76,17 +76,22 @@ __device__ __forceinline__ int shared_of_group(const Attend& a, int group) {
     return (int)min((int64_t)max(__ldcg(a.shared_lens + group), 0), (int64_t)a.width * a.page_size);
 }
 // The groups of a warp's lanes, 32 at a time: where the starts fall, a group begins (and ends) no earlier than the largest before it, so
-// that no token stands in two groups, whatever the starts are, and no row has two writers.  `upto`: the end of the groups before.
+// that no token stands in two groups, whatever the starts are, and no row has two writers.  `upto`: the end of the groups before.  (The
+// rare case apart: inline it costs 0.2 us of 6.9 where no group is looked at, 0.3 of 31.1 in three groups of 13.)
+__device__ __noinline__ int2 raise_starts(int start, int end, int upto) {
+    int top = start;
+    for (int d = 1; d < 32; d <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, top, d);
+        if ((int)(threadIdx.x & 31) >= d) top = max(top, other);
+    }
+    start = max(top, upto);
+    return make_int2(start, max(start, end));
+}
 __device__ __forceinline__ void keep_ascending(int& start, int& end, int& upto) {
     if (__any_sync(0xffffffffu, start > end || start < upto)) {
-        int top = start;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int other = __shfl_up_sync(0xffffffffu, top, d);
-            if ((int)(threadIdx.x & 31) >= d) top = max(top, other);
-        }
-        start = max(top, upto);
-        end = max(start, end);
+        const int2 raised = raise_starts(start, end, upto);
+        start = raised.x;
+        end = raised.y;
     }
     upto = __shfl_sync(0xffffffffu, end, 31);
 }
