@@ -33,7 +33,7 @@ def fake(monkeypatch):
 def test_an_eager_launch_is_checked_once(fake, part):
     kernels.check_finished_launches()
     assert fake["reads"] == []
-    getattr(kernels, f"_note_{part}_launch")()
+    getattr(kernels, f"_note_{part}_launch")(1)
     kernels.check_finished_launches()
     kernels.check_finished_launches()
     assert fake["reads"] == [part]
@@ -42,7 +42,7 @@ def test_an_eager_launch_is_checked_once(fake, part):
 @pytest.mark.parametrize("part", PARTS)
 def test_every_replay_of_a_recorded_launch_is_checked(fake, part):
     fake["capturing"] = True
-    getattr(kernels, f"_note_{part}_launch")()
+    getattr(kernels, f"_note_{part}_launch")(1)
     fake["capturing"] = False
     for _ in range(3):                                     # replays
         kernels.check_finished_launches()
@@ -50,7 +50,7 @@ def test_every_replay_of_a_recorded_launch_is_checked(fake, part):
     fake["codes"][part] = 5                                # a wait of the next one gives up
     with pytest.raises(kernels.KernelError, match=f"{'add_' if part == 'adapters' else ''}{part}.*code 5"):
         kernels.check_finished_launches()
-    getattr(kernels, f"_note_{part}_launch")()             # an eager launch in between changes nothing
+    getattr(kernels, f"_note_{part}_launch")(1)             # an eager launch in between changes nothing
     kernels.check_finished_launches()
     kernels.check_finished_launches()
     assert fake["reads"] == [part] * 6

@@ -2054,7 +2054,8 @@ def logit_rules(logits: torch.Tensor, *, slots: torch.Tensor, penalties: torch.T
     ``bias_values`` (int32 and float32 [slots, up to 1024]; token -1: none) are added (a token named twice gets both, in
     their order).  Last, with ``masks`` (int32 [masks, at least vocab / 32 words]: bit v % 32 of word v // 32 is token v)
     and ``mask_rows`` (int32 [slots]; a number outside the masks: all tokens), tokens whose bit is 0 become -inf, whatever
-    they were; a mask of zeros leaves -inf alone.  Tokens outside the vocabulary are passed over.
+    they were; a mask of zeros leaves -inf alone (as a penalty beyond float32 does for the token it is for; from a row of nothing
+    else token 0 is drawn).  Tokens outside the vocabulary are passed over.
 
     Computed in float32 and rounded once to the type of the logits.  ``out``: where the result goes, ``logits`` itself
     among others (in place); else a new tensor."""
@@ -2143,18 +2144,19 @@ def add_adapters(y: torch.Tensor, x: torch.Tensor, down: torch.Tensor, up: torch
         dtype_tag(out.dtype), _pdl("gemm"))
     _check(_fn("adapters", "tvb_add_adapters", _PACKED)(call, stream), "add_adapters", 2)
     if tag == BF16 and m > ADAPTERS_FEW_ROWS:
-        _note_adapters_launch()
+        _note_adapters_launch(stream)
 
 
 _adapters_unchecked = _adapters_captured = False
 
 
-def _note_adapters_launch() -> None:
+def _note_adapters_launch(stream: int) -> None:
     """Kernels with bounded waits were launched, or recorded: a graph's replays are not seen here, so from then on every check reads
-    their status word."""
+    their status word.  (The default stream, 0, is never recorded.)"""
     global _adapters_unchecked, _adapters_captured
     _adapters_unchecked = True
-    _adapters_captured = _adapters_captured or torch.cuda.is_current_stream_capturing()
+    if stream and not _adapters_captured:
+        _adapters_captured = torch.cuda.is_current_stream_capturing()
 
 
 def adapters_status() -> int:
@@ -2180,11 +2182,12 @@ _SHARED_CALL = struct.Struct("@PqPPPPPPPPPqiiiiiiiiiiiiif")
 _attention_shared_unchecked = _attention_shared_captured = False
 
 
-def _note_attention_shared_launch() -> None:
+def _note_attention_shared_launch(stream: int) -> None:
     """As :func:`_note_adapters_launch`."""
     global _attention_shared_unchecked, _attention_shared_captured
     _attention_shared_unchecked = True
-    _attention_shared_captured = _attention_shared_captured or torch.cuda.is_current_stream_capturing()
+    if stream and not _attention_shared_captured:
+        _attention_shared_captured = torch.cuda.is_current_stream_capturing()
 
 
 def attention_shared_status() -> int:
@@ -2223,7 +2226,8 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     if page_size < 1 or not _is(key_cache, dtype, pages, num_kv, page_size, head_dim) \
             or value_cache.dtype is not dtype or value_cache.shape != cache_shape or not value_cache.is_contiguous():
         raise KernelError("attention_shared: caches must be contiguous [pages, num_kv, page_size, head_dim] of the type of q")
-    if (key_cache.data_ptr() | value_cache.data_ptr()) % 16:
+    keys_at, values_at = key_cache.data_ptr(), value_cache.data_ptr()
+    if (keys_at | values_at) % 16:
         raise KernelError("attention_shared: the caches must start on 16 bytes")
     if tokens < 0 or not _is(positions, torch.int32, tokens) or not _is(token_row, torch.int32, tokens):
         raise KernelError("attention_shared: token_row and positions must be contiguous int32 [tokens]")
@@ -2260,13 +2264,13 @@ def attention_shared(q: torch.Tensor, q_token_stride: int, key_cache: torch.Tens
     need, launches = _shared_plan(tokens, groups, num_q, num_kv, head_dim, pages, page_size, max_shared, max_own, tag)
     scratch = torch.empty(need, dtype=torch.float32, device=q.device) if need else None
     call = _SHARED_CALL.pack(
-        q_at, q_token_stride, key_cache.data_ptr(), value_cache.data_ptr(), block_tables.data_ptr(), token_row.data_ptr(),
+        q_at, q_token_stride, keys_at, values_at, block_tables.data_ptr(), token_row.data_ptr(),
         positions.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
         out.data_ptr(), out.stride()[0], table_shape[0], table_shape[1], groups, tokens, pages, page_size, num_q,
         num_kv, head_dim, max_shared, max_own, tag, _pdl("attention_shared"), scale)
     _check(_fn("attention_shared", "tvb_attention_shared", _PACKED)(call, stream), "attention_shared", launches)
     if tag == BF16:
-        _note_attention_shared_launch()
+        _note_attention_shared_launch(stream)
     return out
 
 
