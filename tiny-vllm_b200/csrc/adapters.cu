@@ -11,7 +11,7 @@
 // registers: a thread takes 16 bytes, eight neighbouring k, of each row, and which k a fragment's place stands for is permuted
 // alike in both operands.  More rows go 64 a CTA through a ring in shared memory: tensor-map copies fill it where types, ranks and
 // alignment allow (adapters_tma.cuh, which has its own `expand` too), else cp.async.  u leaves in two bfloat16 whose sum is u
-// to 2^-17 of it, so that no rounding of u is seen beside that of the result.  A row takes the sums of its own adapter
+// to 2^-16 of it, so that no rounding of u is seen beside that of a bfloat16 result.  A row takes the sums of its own adapter
 // alone: what other adapters hold, infinities among them, does not reach it.
 // float32: the float32 cores.
 //
@@ -744,7 +744,7 @@ template <int VEC> __global__ void __launch_bounds__(THREADS) expand_f32_kernel(
     __shared__ int ids[ROWS], distinct[ROWS];
     float* u = reinterpret_cast<float*>(raw);                                   // [ROWS][rank]
     const int row0 = blockIdx.y * ROWS, rows = min(ROWS, s.m - row0), column = blockIdx.x * THREADS + threadIdx.x;
-    // before `shrink` is through (see expand_kernel): the adapters, y, and B on its way into L2
+    // before `shrink` is through (see expand_rows): the adapters, y, and B on its way into L2
     const int count = find_adapters<ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);
     float* y = reinterpret_cast<float*>(s.out) + (int64_t)row0 * s.ldo + column;
     float old[ROWS];

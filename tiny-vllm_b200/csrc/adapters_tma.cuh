@@ -9,7 +9,7 @@
 //           (Rows without an adapter go out as they came in.)
 //
 // Bound by the instructions between the copies as much as by the traffic of x and y through L2: 4099 rows, 4096 -> 4096, rank 64
-// take 17 us for shrink and 23 us for expand, where 101 MB pass, 15 us at the speed of HBM (the kernels of adapters.cu: 27 and
+// take 17 us for shrink and 24 us for expand (1 of it the look at whether every sum is finite, mend_sums), where 101 MB pass, 15 us at the speed of HBM (the kernels of adapters.cu: 27 and
 // 33 us).  Without the rests of u, which bfloat16 accuracy of the sum would allow and float32 accuracy of u does not, expand
 // would save 5 us.  Measured and not taken: 4, 8 and 11 tiles of y a CTA (rows without an adapter leave their SM idle: 1 to 5 us
 // more), longer rings and fewer CTAs an SM (1 to 3 us more), more pieces of k (3 us more).
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(TMA_THREADS, 4) expand_tma_kernel(const __grid
         prefetch_tensormap(&map_out);
         prefetch_tensormap(&map_b);
     }
-    // (before `shrink` is through, see expand_kernel: the adapters here, the first tiles of y and B below)
+    // (before `shrink` is through, see expand_rows: the adapters here, the first tiles of y and B below)
     const int count = find_adapters<TMA_ROWS>(s.ids, s.m, s.adapters, row0, ids, distinct);       // (its barriers: ours are set up)
     if (warp < WARPS || count == 0) {
         pdl_wait();

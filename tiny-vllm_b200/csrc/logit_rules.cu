@@ -6,7 +6,8 @@
 //   x = x + (sum of the request's biases of v)
 //   x = -inf                                                          if the request's mask has a zero bit at v
 //
-// in float32, rounded once to the type of the logits.  The counts are made anew from the request's tokens in every call:
+// in float32, rounded once to the type of the logits.  Biases come behind the penalties, so that one adds what it says whether its token
+// was seen or not (before them, a penalty for repetition would divide or multiply it too).  The counts are made anew from the request's tokens in every call:
 // a CTA takes one slice of one row, counts the tokens that fall into it in shared memory (a word a token: the count, one
 // bit for "in the prompt", one for "has a bias"), and then passes over its slice once.  Integer atomics and one thread a
 // logit: the result does not depend on the order in which anything runs.
