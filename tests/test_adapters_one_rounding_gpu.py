@@ -42,13 +42,24 @@ def test_any_k(k, m, adapters):
     assert (memory[:, :2] == 3).all() and (memory[:, 98:] == 3).all()
 
 
-@pytest.mark.parametrize("k", [40, 43])
-def test_a_weight_that_lies_the_other_way(k):
+@pytest.mark.parametrize("m", [5, 200, 300])
+@pytest.mark.parametrize("k", [1, 40, 43])
+def test_a_weight_that_lies_the_other_way(k, m):
     for n, more in ((91, {}), (96, dict(out_dtype=torch.float32))):
-        s = made(300, k, n, 8, 3)
+        s = made(m, k, n, 8, 3)
         s["weight"] = s["weight"].t().contiguous().t()
-        assert s["weight"].stride(0) == 1
+        assert k == 1 or s["weight"].stride(0) == 1
         check_once(adapted(**s, **more), s)
+
+
+@pytest.mark.parametrize("m", [5, 300])
+def test_one_column_of_x(m):
+    """k = 1: the rows are single values, however far apart their (only) columns stand."""
+    for n, more in ((91, {}), (96, dict(out_dtype=torch.float32)), (96, {})):
+        s = made(m, 1, n, 8, 3)
+        s["x"] = torch.zeros(4, m, dtype=BF16, device=DEV).t()[:, :1].copy_(s["x"])
+        assert s["x"].stride() == (1, m)
+        check(adapted(**s, **more), s)
 
 
 def test_captured():

@@ -66,11 +66,11 @@ def _linear_f32(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None,
 
 def _projection_f32(x: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None, weight_constant: bool) -> torch.Tensor:
     """:func:`linear` of bfloat16 operands with a float32 result that has not passed through bfloat16.  More than 256 rows of a k that is
-    no multiple of 8, or of a weight whose rows are not contiguous, do so there (the library's float32 results want neither): k is filled
-    up with zeros here, which add nothing (1,025 x 3,537 x 1,096: 54 us and 4e-6 off on the whole, 96 us and 0.0023 there; the float32
+    no multiple of 8, or of a weight whose rows are not contiguous, do so there (and fewer of the latter are refused): here k is filled
+    up with zeros, which add nothing, for the library's product with a float32 result (1,025 x 3,537 x 1,096: 54 us and 4e-6 off on the whole, 96 us and 0.0023 there; the float32
     cores 437 us)."""
     k = x.shape[1]
-    if x.shape[0] <= 256 or k % 8 == 0 and weight.stride(1) == 1:
+    if x.stride(1) == 1 and weight.stride(1) == 1 and (x.shape[0] <= 256 or k % 8 == 0):
         return linear(x, weight, out_dtype=torch.float32, out=out, weight_constant=weight_constant)
     if k % 8:
         x, weight = (torch.nn.functional.pad(t, (0, -k % 8)) for t in (x, weight))
