@@ -399,7 +399,8 @@ extern "C" int tvb_gemm_small_m(const void* x, long long ldx, const void* w, lon
                                 const void* add_stream, float* squares_out, const void* next_weight,
                                 long long next_bytes, int pdl, void* stream) {
     if (m <= 0 || n <= 0) return 0;
-    if (m > 32 || k <= 0 || k % 8 || ldx % 8 || ldw % 8 || mode < 0 || mode > 2 || n > 65535 * 16)
+    if (m > 32 || k <= 0 || k % 8 || ldx % 8 || ldw % 8 || mode < 0 || mode > 2 || n > 65535 * 16 ||
+        (((uintptr_t)x | (uintptr_t)w | (uintptr_t)residual) & 15))
         return TVB_BAD_ARGUMENT;
     if (norm_weight && ldx != k) return TVB_BAD_ARGUMENT;
     if (row_squares && (!norm_weight || residual || residual_out || square_tiles <= 0)) return TVB_BAD_ARGUMENT;

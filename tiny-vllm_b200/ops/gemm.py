@@ -84,7 +84,8 @@ def small(x: torch.Tensor, weight: torch.Tensor) -> bool:
     limit = SMALL_M_MAX_WEIGHT_BYTES if x.shape[0] <= 8 else SMALL_M_MAX_WEIGHT_BYTES_OVER_8_ROWS
     return (x.shape[0] <= SMALL_M_DISPATCH_ROWS and weight.numel() * weight.element_size() <= limit
             and x.shape[1] % 8 == 0 and x.stride(1) == 1
-            and x.stride(0) % 8 == 0 and weight.stride(1) == 1 and weight.stride(0) % 8 == 0)
+            and x.stride(0) % 8 == 0 and weight.stride(1) == 1 and weight.stride(0) % 8 == 0
+            and (x.data_ptr() | weight.data_ptr()) % 16 == 0)
 
 
 def linear_bf16(x: torch.Tensor, weight: torch.Tensor, *, out_dtype: torch.dtype,

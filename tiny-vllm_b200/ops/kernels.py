@@ -2627,6 +2627,8 @@ def gemm_small_m(x: torch.Tensor, w: torch.Tensor, mode: int = GEMM_BF16, *,
     if m < 1 or m > SMALL_M_MAX_ROWS or k % 8 or x.stride(0) % 8 or w.stride(0) % 8:
         raise KernelError(f"gemm_small_m takes up to {SMALL_M_MAX_ROWS} rows (and one at least), k and row strides "
                           f"multiples of 8 (m {m}, k {k})")
+    if (x.data_ptr() | w.data_ptr() | (_ptr(residual) or 0)) % 16:
+        raise KernelError("gemm_small_m wants x, w and the residual on 16 bytes")
     if mode == GEMM_SILU and rows % 2:
         raise KernelError("gemm_small_m: a [gate | up] weight has an even number of rows")
     n = rows // 2 if mode == GEMM_SILU else rows

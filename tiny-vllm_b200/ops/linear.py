@@ -208,7 +208,7 @@ def linear_norm(hidden: torch.Tensor | None, residual: torch.Tensor | None, norm
         return (linear_silu if silu else linear)(x, weight, weight_constant=weight_constant), residual
     if (hidden.dtype == torch.bfloat16 and weight.dtype == torch.bfloat16 and hidden.is_contiguous()
             and getattr(norm, "folds_into_product", False) and gemm.small(hidden, weight)
-            and hidden.shape[0] <= FUSED_NORM_MAX_ROWS
+            and hidden.shape[0] <= FUSED_NORM_MAX_ROWS and (residual is None or residual.data_ptr() % 16 == 0)
             and kernels.gemm_small_m_takes_norm(hidden.shape[0], hidden.shape[1])):
         mode = kernels.GEMM_SILU if silu else kernels.GEMM_BF16
         out, stream = kernels.gemm_small_m(hidden, weight, mode, norm_weight=norm.weight,
